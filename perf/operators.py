@@ -299,7 +299,7 @@ def _plain_store(st: dict, x, pos, row, codes, scale, token_axis: int):
     amax = new.abs().amax(dim=(1, 3))                                  # [n, hkv]
     start = torch.full((n,), page, device=DEV).scatter_reduce(0, row, pos % page, "amin")
     begun = (start > 0)[:, None]                                       # holds earlier tokens
-    inv_new = qmax / amax.clamp(min=EPS)
+    inv_new = torch.full_like(amax, qmax) / amax.clamp(min=EPS)        # one rounding
     s_old = scale[touched]
     mant, exp = torch.frexp(amax / (qmax * s_old))
     grow = torch.where(mant > 0.5, exp, exp - 1).clamp(min=0) * begun
