@@ -26,6 +26,8 @@ SOURCES = [
     CSRC / "cbq_w8a16.hip",
     CSRC / "cbq_w8a16_f32.hip",
     CSRC / "cbq_gemm.hip",
+    CSRC / "cbq_kv_append.hip",
+    CSRC / "cbq_kv_attend.hip",
 ]
 
 WS_CTRL_BYTES = 16384
@@ -41,7 +43,8 @@ MM_B_KN, MM_B_NK = 0, 1
 _P, _I64, _I32, _F, _SZ = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float,
                            ctypes.c_size_t)
 
-# name -> (restype, argtypes); must match include/cublade_quant.h.
+# name -> (restype, argtypes); must match include/cublade_quant.h (KV_SIGNATURES:
+# include/cublade_kv.h).
 SIGNATURES = {
     "cbq_last_error": (ctypes.c_char_p, []),
     "cbq_abi_version": (_I32, []),
@@ -75,6 +78,38 @@ SIGNATURES = {
     "cbq_mm": (_I32, [_P, _P, _I32, _I32, _I64, _I64, _I64, _P, _I32, _P, _SZ, _P]),
 }
 
+# include/cublade_kv.h: the 8-bit paged key/value cache.
+KV_INT8, KV_FP8 = 0, 1
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("num_pages", _I64),
+                ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("store", ctypes.c_int32)]
+
+
+class KvBatch(ctypes.Structure):
+    _fields_ = [("page_table", _P), ("table_stride", _I64), ("lengths", _P), ("cu", _P),
+                ("tokens", _I64), ("batch", ctypes.c_int32), ("max_pages", ctypes.c_int32)]
+
+
+class KvHeads(ctypes.Structure):
+    _fields_ = [("data", _P), ("token_stride", _I64), ("head_stride", _I64)]
+
+
+class KvRope(ctypes.Structure):
+    _fields_ = [("cos_table", _P), ("sin_table", _P), ("positions", _P), ("rows", _I64),
+                ("rot_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32)]
+
+
+# Structures are passed by address (ctypes.byref).
+KV_SIGNATURES = {
+    "cbq_kv_append": (_I32, [_P, _P, _I32, _P, _P, _P, _I32, _P, _P, _P]),
+    "cbq_kv_dequant": (_I32, [_P, _P, _I64, _P, _P, _I32, _P]),
+    "cbq_kv_attend_ws_bytes": (_SZ, [_P, _P, _I32, _I64]),
+    "cbq_kv_attend": (_I32, [_P, _P, _I32, _P, _I32, _F, _I32, _I64, _I64, _P, _SZ, _P, _P, _P]),
+}
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -93,7 +128,7 @@ def lib() -> ctypes.CDLL:
                     raise RuntimeError(
                         f"cublade: {LIB_NAME} has ABI version {ver}, these bindings need major "
                         f"version {ABI_MAJOR} (rebuild the library)")
-                for name, (res, args) in SIGNATURES.items():
+                for name, (res, args) in {**SIGNATURES, **KV_SIGNATURES}.items():
                     fn = getattr(L, name)
                     fn.restype = res
                     fn.argtypes = args
