@@ -52,12 +52,16 @@ struct KvAttendArg {
   const float* vs;
   char* out;
   float* lse;
-  float* po;               // [splits, tokens * hq, d] unnormalised partial outputs
-  float2* pml;             // [splits, tokens * hq] their (m, sum)
-  int64_t window;
+  float* po;               // [splits, prows, d] unnormalised partial outputs
+  float2* pml;             // [splits, prows] their (m, sum)
+  int64_t prows;           // partial rows: items * hkv * rows of a tile
   float scale_log2e;
   int hkv, hq, rep, d, page;
-  int causal, bf16, splits, tiles;
+  int causal, bf16, negate, splits;
+  int window;              // 0: none
+  int tile_rows;           // query rows of a workgroup
+  int64_t items;           // row tiles of this launch, at most
+  int64_t row_min, row_max;   // this launch's sequences have row_min .. row_max rows
 };
 
 // 8 codes -> 8 exact fp16.
@@ -99,37 +103,50 @@ __device__ __forceinline__ float sum_groups(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
+__device__ __forceinline__ float max_halves(float v) {
+  const uint32_t u = __float_as_uint(v);
+  const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+  return fmaxf(__uint_as_float(a.x), __uint_as_float(a.y));
+}
+
 // Bytes of a word that are E4M3 NaN (0x7f, 0xff), as a mask of their high bits.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
 
-// The keys a query row sees: [lo, hi).
+// The keys a query row sees: [lo, hi). (Lengths are int32, and a call's rows of
+// one kv head fewer than 2^31.)
 struct KeyRange {
-  int64_t lo, hi;
+  int lo, hi;
 };
 
-__device__ __forceinline__ KeyRange keys_of(const KvAttendArg& a, int64_t len, int64_t n,
-                                            int64_t i) {
+// Tokens that a row of the page table can hold (key indices and ends of steps
+// stay int32).
+__device__ __forceinline__ int64_t capacity(const KvAttendArg& a) {
+  const int64_t c = static_cast<int64_t>(a.m.max_pages) << a.m.page_shift;
+  return c < INT32_MAX - 1024 ? c : INT32_MAX - 1024;
+}
+
+__device__ __forceinline__ KeyRange keys_of(const KvAttendArg& a, int len, int n, int i) {
   KeyRange r;
   r.lo = 0;
   r.hi = len;
   if (a.causal) {
-    const int64_t end = len - n + i + 1;
+    const int end = len - n + i + 1;
     r.hi = end < 0 ? 0 : end;
     if (a.window > 0 && end > a.window) r.lo = end - a.window;
   }
   return r;
 }
 
-// Writes one row's 4 outputs (finished or partial).
-__device__ __forceinline__ void put_row(const KvAttendArg& a, int64_t row, int split, int d0,
-                                        f4 o, float m, float l, bool bad) {
+// Writes 4 outputs of one row: finished ones, or the partial row `prow` of a
+// split of the keys.
+__device__ __forceinline__ void put_row(const KvAttendArg& a, int64_t row, int64_t prow, int split,
+                                        int d0, f4 o, float m, float l, bool bad) {
   if (a.splits > 1) {
-    *reinterpret_cast<f4*>(a.po + (static_cast<int64_t>(split) * a.m.tokens * a.hq + row) * a.d + d0) = o;
-    if (d0 == 0)
-      a.pml[static_cast<int64_t>(split) * a.m.tokens * a.hq + row] =
-          bad ? make_float2(0.0f, __builtin_nanf("")) : make_float2(m, l);
+    const int64_t at = split * a.prows + prow;
+    *reinterpret_cast<f4*>(a.po + at * a.d + d0) = o;
+    if (d0 == 0) a.pml[at] = bad ? make_float2(0.0f, __builtin_nanf("")) : make_float2(m, l);
     return;
   }
   const bool none = m == kNegInf;
@@ -144,12 +161,81 @@ __device__ __forceinline__ void put_row(const KvAttendArg& a, int64_t row, int s
     a.lse[row] = bad ? __builtin_nanf("") : none ? kNegInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
+// One row's queries as fp16 operands, N pieces of 8 dimensions (piece k from
+// dim(k)), and the factor cq of its scores. bf16 queries are scaled to fp16 by a
+// power of two per row (row_max: the maximum over the lanes that share the row);
+// the factor takes it back. A negative scale of the scores is the queries' sign
+// here, so that the factor is not negative.
+template <int N, typename Dim, typename Max, typename Piece>
+__device__ __forceinline__ void load_q(const KvAttendArg& a, const char* qp, bool has, Dim dim,
+                                       Max row_max, float& cq, Piece piece) {
+  cq = a.scale_log2e;
+  float amax = 0.0f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (has && dim(k) < a.d) raw = *reinterpret_cast<const uint4*>(qp + 2 * dim(k));
+    piece(k) = u32x4{raw.x, raw.y, raw.z, raw.w} ^ (a.negate ? 0x80008000u : 0u);
+    if (a.bf16) {
+      float f[8];
+      cvt8<kBF16>(Raw8<kBF16>{raw}, f);
+      amax = absmax8(f, amax);
+    }
+  }
+  if (!a.bf16) return;
+  amax = row_max(amax);
+  const int e = static_cast<int>(__float_as_uint(amax) >> 23);   // biased exponent
+  float up = 1.0f;
+  if (e > 0 && e < 254) {     // amax * up in [1, 2)
+    up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
+    cq *= __uint_as_float(static_cast<uint32_t>(e) << 23);
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const u32x4 r = piece(k);
+    float f[8];
+    cvt8<kBF16>(Raw8<kBF16>{make_uint4(r.x, r.y, r.z, r.w)}, f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] *= up;
+    const uint4 w = pack8_out<kF16>(f);
+    piece(k) = u32x4{w.x, w.y, w.z, w.w};
+  }
+}
+
+// A sequence's query rows (row = new token * rep + head in its group) in tiles.
 struct RowTiles {
-  int rep;
+  int rep, tile_rows;
+  int64_t lo, hi;
   __device__ int64_t operator()(const KvSeq& s) const {
-    return (s.n * rep + kRowTile - 1) / kRowTile;
+    const int r = s.n * rep;
+    return r >= lo && r <= hi ? (r + tile_rows - 1) / tile_rows : 0;
   }
 };
+
+// The tile of rows with number `item` of a launch: its sequence (b < 0: there is
+// no such tile) and first row.
+struct KvTile {
+  int b;
+  KvSeq s;
+  int rows, r_first;
+};
+
+__device__ __forceinline__ KvTile tile_of(const KvAttendArg& a, int64_t item) {
+  KvTile t;
+  int64_t tile;
+  if (a.m.cu == nullptr) {
+    const int per = (a.rep + a.tile_rows - 1) / a.tile_rows;
+    t.b = static_cast<int>(item / per);
+    tile = item % per;
+  } else {
+    t.b = kv_find(a.m, item, tile, RowTiles{a.rep, a.tile_rows, a.row_min, a.row_max});
+    if (t.b < 0) return t;
+  }
+  t.s = kv_seq(a.m, t.b);
+  t.rows = static_cast<int>(t.s.n) * a.rep;
+  t.r_first = static_cast<int>(tile) * a.tile_rows;
+  return t;
+}
 
 // One workgroup: 16 query rows of one kv head (row = new token * rep + head in
 // the group) and one range of the keys. Its 4 waves take steps of 64 keys in
@@ -169,35 +255,28 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
   const int64_t rest = blockIdx.x / a.splits;
   const int h = rest % a.hkv;
   const int64_t item = rest / a.hkv;
-  int64_t tile;
-  int b;
-  if (a.m.cu == nullptr) {
-    b = static_cast<int>(item / a.tiles);
-    tile = item % a.tiles;
-  } else {
-    b = kv_find(a.m, item, tile, RowTiles{a.rep});
-    if (b < 0) return;
-  }
-  const KvSeq s = kv_seq(a.m, b);
-  const int64_t cap = static_cast<int64_t>(a.m.max_pages) << a.m.page_shift;
+  const KvTile tl = tile_of(a, item);
+  if (tl.b < 0) return;
+  const int b = tl.b;
+  const KvSeq s = tl.s;
+  const int64_t cap = capacity(a);
   const bool bad = s.len > cap;      // keys that no page can hold
-  const int64_t len = s.len < 0 ? 0 : bad ? cap : s.len;
-  const int64_t rows = s.n * a.rep;
-  const int64_t r_first = tile * kRowTile;
-  const int64_t r_last = r_first + kRowTile - 1 < rows ? r_first + kRowTile - 1 : rows - 1;
-  const int64_t r = r_first + n16;
+  const int len = static_cast<int>(s.len < 0 ? 0 : bad ? cap : s.len);
+  const int rows = tl.rows, r_first = tl.r_first, n = static_cast<int>(s.n);
+  const int r_last = r_first + kRowTile - 1 < rows ? r_first + kRowTile - 1 : rows - 1;
+  const int r = r_first + n16;
   const bool has_row = r < rows;
-  const int64_t ti = r / a.rep;      // the row's new token
-  const int head = h * a.rep + static_cast<int>(r - ti * a.rep);
-  const KeyRange mine = keys_of(a, len, s.n, ti);
-  const KeyRange kf = keys_of(a, len, s.n, r_first / a.rep);
-  const KeyRange kl = keys_of(a, len, s.n, r_last / a.rep);
+  const int ti = r / a.rep;      // the row's new token
+  const int head = h * a.rep + r - ti * a.rep;
+  const KeyRange mine = keys_of(a, len, n, ti);
+  const KeyRange kf = keys_of(a, len, n, r_first / a.rep);
+  const KeyRange kl = keys_of(a, len, n, r_last / a.rep);
 
-  const int64_t kb = kf.lo / kStep, ke = (kl.hi + kStep - 1) / kStep;
-  int64_t per = (ke - kb + a.splits - 1) / a.splits;
+  const int kb = kf.lo / kStep, ke = (kl.hi + kStep - 1) / kStep;
+  int per = (ke - kb + a.splits - 1) / a.splits;
   per = per < 4 ? 4 : per;
-  const int64_t s0 = kb + split * per;
-  const int64_t s1 = s0 + per < ke ? s0 + per : ke;
+  const int s0 = kb + split * per;
+  const int s1 = s0 + per < ke ? s0 + per : ke;
 
   f4 o[ND] = {};
   float m = kNegInf, l = 0.0f;
@@ -205,56 +284,24 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
   if (s0 + wave < s1) {
     // the queries as fp16, and what the scores are multiplied by
     u32x4 qf[2 * NC];
-    float cq = a.scale_log2e;
-    {
-      float f[2 * NC][8];
-      float amax = 0.0f;
-      const char* qp = a.q + (s.tok0 + ti) * a.qts + head * a.qhs;
-#pragma unroll
-      for (int c = 0; c < 2 * NC; ++c) {
-        const int d0 = 64 * (c >> 1) + 16 * g + 8 * (c & 1);
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (has_row && d0 < d) raw = *reinterpret_cast<const uint4*>(qp + 2 * d0);
-        if (a.bf16) {
-          Raw8<kBF16> w{raw};
-          cvt8<kBF16>(w, f[c]);
-          amax = absmax8(f[c], amax);
-        } else {
-          qf[c] = u32x4{raw.x, raw.y, raw.z, raw.w};
-        }
-      }
-      if (a.bf16) {
-        amax = max_groups(amax);
-        const int e = static_cast<int>(__float_as_uint(amax) >> 23);   // biased exponent
-        float up = 1.0f;
-        if (e > 0 && e < 254) {     // amax * up in [1, 2)
-          up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
-          cq *= __uint_as_float(static_cast<uint32_t>(e) << 23);
-        }
-#pragma unroll
-        for (int c = 0; c < 2 * NC; ++c) {
-          float x[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[k] = f[c][k] * up;
-          const uint4 w = pack8_out<kF16>(x);
-          qf[c] = u32x4{w.x, w.y, w.z, w.w};
-        }
-      }
-    }
+    float cq;
+    load_q<2 * NC>(a, a.q + (s.tok0 + ti) * a.qts + head * a.qhs, has_row,
+                   [&](int c) { return 64 * (c >> 1) + 16 * g + 8 * (c & 1); },
+                   [](float v) { return max_groups(v); }, cq, [&](int c) -> u32x4& { return qf[c]; });
 
-    const int64_t last_block = (kl.hi - 1) >> 4;
-    auto block_of = [&](int64_t st, int quarter) {
-      const int64_t bl = st * 4 + quarter;
+    const int last_block = (kl.hi - 1) >> 4;
+    auto block_of = [&](int st, int quarter) {
+      const int bl = st * 4 + quarter;
       return bl < last_block ? bl : last_block;
     };
-    auto page_of = [&](int64_t bl) { return a.m.table[b * a.m.tstride + ((bl << 4) >> a.m.page_shift)]; };
+    auto page_of = [&](int bl) { return a.m.table[b * a.m.tstride + ((bl << 4) >> a.m.page_shift)]; };
     auto valid = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.m.num_pages); };
     u32x4 kr[4][NC];
     float ksc = 0.0f, vsc = 1.0f;
     int id_v = 0;
     // Row r of tile t is the key 16 (r / 4) + 4 t + r % 4 of the step.
-    auto load_k = [&](int64_t st, int idk, int idv) {
-      const int64_t bl = block_of(st, n16 >> 2);
+    auto load_k = [&](int st, int idk, int idv) {
+      const int bl = block_of(st, n16 >> 2);
       const int64_t at = static_cast<int64_t>(valid(idk) ? idk : 0) * a.hkv + h;
       const uint8_t* p = a.kc + (at * a.page + ((bl << 4) & (a.page - 1)) + (n16 & 3)) * d + 16 * g;
 #pragma unroll
@@ -276,12 +323,12 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
       next_v = page_of(block_of(s0 + wave + 4, g));
     }
 
-    for (int64_t st = s0 + wave; st < s1; st += 4) {
-      const int64_t tb = st * kStep;
+    for (int st = s0 + wave; st < s1; st += 4) {
+      const int tb = st * kStep;
       // this step's values
       u32x4 vr[ND];
       {
-        const int64_t bl = block_of(st, g);
+        const int bl = block_of(st, g);
         const uint8_t* p = a.vc + ((static_cast<int64_t>(id_v) * a.hkv + h) * d + n16) * a.page +
                            ((bl << 4) & (a.page - 1));
 #pragma unroll
@@ -320,7 +367,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int64_t j = tb + 16 * g + 4 * t + i;
+            const int j = tb + 16 * g + 4 * t + i;
             if (j < mine.lo || j >= mine.hi) y[t][i] = kNegInf;
           }
       }
@@ -370,7 +417,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
               uint32_t w = 0;
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                const int64_t j = tb + 16 * g + 2 * e + k;
+                const int j = tb + 16 * g + 2 * e + k;
                 if (j >= mine.lo && j < mine.hi) w |= 0x3c00u << (16 * k);
               }
               if (e < 4) seen0[e] = w;
@@ -413,7 +460,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
   for (int t = 0; t < ND; ++t) *reinterpret_cast<f4*>(&so[wave][n16][16 * t + 4 * g]) = o[t];
   __syncthreads();
   const int row = threadIdx.x >> 4;
-  const int64_t rr = r_first + row;
+  const int rr = r_first + row;
   if (rr >= rows) return;
   float mm = kNegInf, ll = 0.0f, f[4];
 #pragma unroll
@@ -429,17 +476,340 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
     f4 v = {};
 #pragma unroll
     for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f4*>(&so[w][row][d0]) * f[w];
-    put_row(a, orow, split, d0, v, mm, ll, bad);
+    put_row(a, orow, (item * a.hkv + h) * kRowTile + row, split, d0, v, mm, ll, bad);
   }
 }
 
-// Joins the splits' partial results: one wave per row.
-__global__ __launch_bounds__(kBlock) void k_kv_attend_join(const KvAttendArg a, int64_t rows) {
+// ---------------------------------------------------------------------------
+// Many query rows: prompts and chunks of them.
+// ---------------------------------------------------------------------------
+// A workgroup takes 4 * 32 * CT rows of one kv head, a wave 32 * CT of them in
+// CT column tiles of 32; the workgroup goes through the keys 64 at a time. Codes
+// are widened to fp16 once per workgroup, on their way from registers to LDS (K
+// rows [64 keys][DP], V^T rows [DP][64 keys]; every row has 16 bytes more than it
+// needs, so an odd number of 16-byte chunks: equal chunks of 16 consecutive rows
+// lie in distinct banks, and every access is a base register plus a constant), in
+// two buffers. Codes are loaded two steps ahead, their page ids three; one barrier
+// ends a step.
+//
+// Row r of a score tile of 32 keys is the key with bits 2 and 3 of r swapped: a
+// lane's scores 8 u .. 8 u + 7 are then the keys 16 u + 8 (lane / 32) .. + 7, the
+// operand of the second product's step u. Each such 16 keys lie in one page, so
+// their scales are the same in the whole wave.
+template <int ST, int DP, int CT>
+__global__ __launch_bounds__(kBlock, DP * CT <= 128 ? 2 : 1) void k_kv_attend_long(const KvAttendArg a) {
+  constexpr int ROWS = 4 * 32 * CT;
+  constexpr int NS = DP / 16;          // steps of 16 dimensions in the scores
+  constexpr int ND = DP / 32;          // tiles of 32 dimensions
+  constexpr int NL = DP / 64;          // 16-code loads per thread and side
+  constexpr int KR = DP / 8 + 1, VR = kStep / 8 + 1;   // 16-byte chunks of a row
+  __shared__ u32x4 lk[2][kStep * KR];
+  __shared__ u32x4 lv[2][DP * VR];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int n32 = lane & 31, hf = lane >> 5;
+
+  const int h = blockIdx.x % a.hkv;
+  const int64_t rest = blockIdx.x / a.hkv;
+  const int split = rest % a.splits;
+  const int64_t item = a.items - 1 - rest / a.splits;   // a causal prompt's longest rows first
+  const KvTile tl = tile_of(a, item);
+  if (tl.b < 0) return;
+  const int b = tl.b;
+  const KvSeq s = tl.s;
+  const int64_t cap = capacity(a);
+  const bool bad = s.len > cap;
+  const int len = static_cast<int>(s.len < 0 ? 0 : bad ? cap : s.len);
+  const int rows = tl.rows, r_first = tl.r_first, n = static_cast<int>(s.n);
+  const int r_last = r_first + ROWS - 1 < rows ? r_first + ROWS - 1 : rows - 1;
+  const int all_hi = keys_of(a, len, n, r_last / a.rep).hi;
+  const int kb = keys_of(a, len, n, r_first / a.rep).lo / kStep;
+  const int ke = (all_hi + kStep - 1) / kStep;
+  int per = (ke - kb + a.splits - 1) / a.splits;
+  const int s0 = kb + split * per;
+  const int s1 = s0 + per < ke ? s0 + per : ke;
+
+  // this wave's rows
+  const int w_first = r_first + wave * 32 * CT;
+  const bool w_any = w_first < rows;
+  const int w_last = w_first + 32 * CT - 1 < rows ? w_first + 32 * CT - 1 : rows - 1;
+  const KeyRange wf = keys_of(a, len, n, (w_any ? w_first : w_last) / a.rep);
+  const KeyRange wl = keys_of(a, len, n, w_last / a.rep);
+  KeyRange mine[CT];
+  int64_t orow[CT];
+  bool has[CT];
+  f16x o[ND][CT] = {};
+  float m[CT], l[CT], cq[CT];
+  u32x4 qf[NS][CT];
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const int r = w_first + 32 * c + n32;
+    has[c] = r < rows;
+    const int ti = (has[c] ? r : rows - 1) / a.rep;
+    const int head = h * a.rep + (has[c] ? r : rows - 1) - ti * a.rep;
+    mine[c] = keys_of(a, len, n, ti);
+    orow[c] = (s.tok0 + ti) * a.hq + head;
+    m[c] = kNegInf;
+    l[c] = 0.0f;
+    const char* qp = a.q + (s.tok0 + ti) * a.qts + head * a.qhs;
+    load_q<NS>(a, qp, has[c], [&](int k) { return 16 * k + 8 * hf; },
+               [](float v) { return max_halves(v); }, cq[c], [&](int k) -> u32x4& { return qf[k][c]; });
+  }
+
+  const int last_block = (all_hi - 1) >> 4;
+  const int shift = a.m.page_shift;
+  const int32_t* trow = a.m.table + b * a.m.tstride;
+  auto valid = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.m.num_pages); };
+  // Block bl of 16 keys (those past the last are read as the last, masked): its
+  // page id and its place in the page. Ids of a step's four blocks are loaded
+  // steps before the codes that need them.
+  auto clamp_block = [&](int bl) { return bl < last_block ? bl : last_block; };
+  auto place_of = [&](int bl) { return (clamp_block(bl) << 4) & (a.page - 1); };
+  auto load_ids = [&](int st, int (&id)[4]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) id[q] = trow[(clamp_block(st * 4 + q) << 4) >> shift];
+  };
+  auto pick = [](const int (&id)[4], int q) {
+    const int lo = q & 1 ? id[1] : id[0], hi = q & 1 ? id[3] : id[2];
+    return q & 2 ? hi : lo;
+  };
+  auto head_of = [&](int id) { return static_cast<int64_t>(valid(id) ? id : 0) * a.hkv + h; };
+  auto load_scales = [&](const int (&id)[4], float (&ks)[4], float (&vs)[4]) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      ks[q] = a.ks[head_of(id[q])];
+      if (!valid(id[q])) ks[q] = __builtin_nanf("");
+      vs[q] = a.vs[head_of(id[q])];
+    }
+  };
+  u32x4 rk[NL], rv[NL];
+  // thread -> 16 codes of key kt, dimensions 16 kc ..; of dimension vd, keys 16 vb ..
+  constexpr int KC = DP / 16;          // 16-code pieces of a key
+  auto load_k = [&](int st, const int (&id)[4]) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int u = tid + kBlock * i, key = u / KC, kc = u % KC;
+      rk[i] = u32x4{0, 0, 0, 0};
+      if (16 * kc < a.d)
+        rk[i] = *reinterpret_cast<const u32x4*>(
+            a.kc + (head_of(pick(id, key >> 4)) * a.page + place_of(st * 4 + (key >> 4)) + (key & 15)) * a.d + 16 * kc);
+    }
+  };
+  auto load_v = [&](int st, const int (&id)[4]) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int u = tid + kBlock * i, vb = u & 3, vd = u >> 2;
+      rv[i] = u32x4{0, 0, 0, 0};
+      if (vd < a.d)
+        rv[i] = *reinterpret_cast<const u32x4*>(
+            a.vc + (head_of(pick(id, vb)) * a.d + vd) * a.page + place_of(st * 4 + vb));
+    }
+  };
+  auto store_k = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int u = tid + kBlock * i, key = u / KC, kc = u % KC;
+      lk[buf][key * KR + 2 * kc] = widen8<ST>(rk[i].x, rk[i].y);
+      lk[buf][key * KR + 2 * kc + 1] = widen8<ST>(rk[i].z, rk[i].w);
+    }
+  };
+  auto store_v = [&](int buf) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int u = tid + kBlock * i, vb = u & 3, vd = u >> 2;
+      lv[buf][vd * VR + 2 * vb] = widen8<ST>(rv[i].x, rv[i].y);
+      lv[buf][vd * VR + 2 * vb + 1] = widen8<ST>(rv[i].z, rv[i].w);
+    }
+  };
+  const int krow = (n32 & 0x13) | ((n32 & 4) << 1) | ((n32 & 8) >> 1);
+  f16x sc[2][CT];
+  auto scores = [&](int buf, f16x (&out)[2][CT]) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int c = 0; c < CT; ++c) out[kt][c] = f16x{};
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const int key = 32 * kt + krow;
+        const u32x4 kk = lk[buf][key * KR + 2 * k + hf];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) out[kt][c] = mfma32x32x16<kF16>(kk, qf[k][c], out[kt][c]);
+      }
+  };
+
+  if (s0 < s1) {
+    int id1[4], id2[4];                // of steps st + 1, st + 2
+    float ksc[4], vsc[4], ksn[4] = {}, vsn[4] = {};
+    load_ids(s0, id1);
+    load_ids(s0 + 1, id2);
+    load_k(s0, id1);
+    load_v(s0, id1);
+    load_scales(id1, ksc, vsc);
+    store_k(0);
+    store_v(0);
+    load_k(s0 + 1, id2);               // (steps past the range read its end again, unused)
+    load_v(s0 + 1, id2);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) id1[q] = id2[q];
+    load_ids(s0 + 2, id2);
+    __syncthreads();
+
+    for (int st = s0; st < s1; ++st) {
+      const int buf = (st - s0) & 1;
+      const int tb = st * kStep;
+      load_scales(id1, ksn, vsn);
+      float vsx[4], lvs[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        vsx[q] = vsc[q] < kTinyScale ? kTinyScale : vsc[q];
+        lvs[q] = __builtin_amdgcn_logf(vsx[q]);
+      }
+      const bool active = w_any && tb < wl.hi && tb + kStep > wf.lo;
+      const bool masked = tb + kStep > wf.hi || tb < wl.lo;
+      u32x4 p[4][CT];
+      if (active) {
+        scores(buf, sc);
+        __builtin_amdgcn_sched_barrier(0);
+        if (masked) {
+          // scores become y, those of keys that the row does not see -infinity
+#pragma unroll
+          for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int j = tb + 32 * kt + 16 * (i >> 3) + 8 * hf + (i & 7);
+                if (j < mine[c].lo || j >= mine[c].hi) sc[kt][c][i] = kNegInf;
+              }
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          float mx = kNegInf;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float t = sc[q >> 1][c][8 * (q & 1)];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) t = fmaxf(t, sc[q >> 1][c][8 * (q & 1) + i]);
+            const float y = __builtin_fmaf(t, cq[c] * ksc[q], lvs[q]);
+            mx = fmaxf(mx, t == kNegInf ? kNegInf : y);
+          }
+          mx = max_halves(mx);
+          const bool raise = mx > m[c] + kRaise;
+          if (__any(raise)) {
+            const float to = raise ? mx : m[c];
+            const float f = raise ? __builtin_amdgcn_exp2f(m[c] - to) : 1.0f;
+            m[c] = to;
+            l[c] *= f;
+#pragma unroll
+            for (int t = 0; t < ND; ++t) o[t][c] *= f;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {
+          const float ref = m[c] == kNegInf ? 0.0f : m[c];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float f = cq[c] * ksc[q], off = lvs[q] - ref;
+            float w[8];
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const float x = sc[q >> 1][c][8 * (q & 1) + i];
+              w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, f, off));
+              if (masked && x == kNegInf) w[i] = 0.0f;   // whatever the scale is
+              sum += w[i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[q][c][i] = pack2_out<kF16>(w[2 * i], w[2 * i + 1]);
+            l[c] += sum == 0.0f ? 0.0f : sum * (1.0f / vsx[q]);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < ND; ++t)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int vd = 32 * t + n32;
+            u32x4 vv = lv[buf][vd * VR + 2 * q + hf];
+            if constexpr (ST == kKvFp8) {
+              // NaN values must reach only the rows that see their key
+              if (masked) {
+                u32x4 ind = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  if ((vv[i] & 0x7fffu) > 0x7c00u) ind[i] |= 0x3c00u;
+                  if ((vv[i] & 0x7fff0000u) > 0x7c000000u) ind[i] |= 0x3c000000u;
+                  vv[i] &= ~((ind[i] >> 10) * 0x1111u);   // 0x3c00 >> 10 = 0xf
+                }
+                if (__any((ind.x | ind.y | ind.z | ind.w) != 0)) {
+#pragma unroll
+                  for (int c = 0; c < CT; ++c) {
+                    u32x4 seen;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                      const int j = tb + 16 * q + 8 * hf + 2 * i;
+                      seen[i] = (j >= mine[c].lo && j < mine[c].hi ? 0x3c00u : 0u) |
+                                (j + 1 >= mine[c].lo && j + 1 < mine[c].hi ? 0x3c000000u : 0u);
+                    }
+                    const f16x cnt = mfma32x32x16<kF16>(ind, seen, f16x{});
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                      if (cnt[i] > 0.0f) o[t][c][i] = __builtin_nanf("");
+                  }
+                }
+              }
+            }
+#pragma unroll
+            for (int c = 0; c < CT; ++c) o[t][c] = mfma32x32x16<kF16>(vv, p[q][c], o[t][c]);
+          }
+      }
+      if (st + 1 < s1) {
+        store_k(buf ^ 1);
+        store_v(buf ^ 1);
+        load_k(st + 2, id2);
+        load_v(st + 2, id2);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          ksc[q] = ksn[q];
+          vsc[q] = vsn[q];
+          id1[q] = id2[q];
+        }
+        load_ids(st + 3, id2);
+      }
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < CT; ++c) {
+    const float sum = l[c] + __shfl_xor(l[c], 32, 64);
+    if (!has[c]) continue;
+#pragma unroll
+    for (int t = 0; t < ND; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int d0 = 32 * t + 8 * q + 4 * hf;
+        if (d0 < a.d)
+          put_row(a, orow[c], (item * a.hkv + h) * ROWS + wave * 32 * CT + 32 * c + n32, split, d0,
+                  f4{o[t][c][4 * q], o[t][c][4 * q + 1], o[t][c][4 * q + 2], o[t][c][4 * q + 3]},
+                  m[c], sum, bad);
+      }
+  }
+}
+
+// Joins the splits' partial results: a wave per row, a workgroup per 4 rows of a
+// tile. Lane l reads split l's maximum and sum.
+__global__ __launch_bounds__(kBlock) void k_kv_attend_join(const KvAttendArg a) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
+  const int quads = a.tile_rows / 4;
+  const int row = (blockIdx.x % quads) * 4 + (threadIdx.x >> 6);
+  const int64_t rest = blockIdx.x / quads;
+  const int h = rest % a.hkv;
+  const int64_t item = rest / a.hkv;
+  const KvTile tl = tile_of(a, item);
+  if (tl.b < 0 || tl.r_first + row >= tl.rows) return;
+  const int64_t prow = (item * a.hkv + h) * a.tile_rows + row;
   float2 ml = make_float2(kNegInf, 0.0f);
-  if (lane < a.splits) ml = a.pml[lane * rows + row];
+  if (lane < a.splits) ml = a.pml[lane * a.prows + prow];
   float m = ml.x;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
@@ -452,32 +822,60 @@ __global__ __launch_bounds__(kBlock) void k_kv_attend_join(const KvAttendArg a, 
   for (int s = 0; s < a.splits; ++s) {
     const float fs = __shfl(f, s, 64);   // with all lanes active: those past d have a split's factor
     if (fs != 0.0f && d0 < a.d)
-      acc += *reinterpret_cast<const f4*>(a.po + (s * rows + row) * a.d + d0) * fs;
+      acc += *reinterpret_cast<const f4*>(a.po + (s * a.prows + prow) * a.d + d0) * fs;
   }
+  const int ti = (tl.r_first + row) / a.rep;
+  const int64_t orow = (tl.s.tok0 + ti) * a.hq + h * a.rep + (tl.r_first + row - ti * a.rep);
   KvAttendArg one = a;
   one.splits = 1;
-  if (d0 < a.d) put_row(one, row, 0, d0, acc, m, l, false);
+  if (d0 < a.d) put_row(one, orow, 0, 0, d0, acc, m, l, false);
 }
+
+// What one call launches: k_kv_attend_rows for the sequences of few rows,
+// k_kv_attend_long for the others (items 0: not launched).
+struct KvPlan {
+  int64_t row_items, long_items;
+  int row_splits, long_splits;
+  int long_tile;
+};
+
+constexpr int64_t kShortRows = 64;
 
 int padded_dim(int d) { return (d + 63) / 64 * 64; }
+int column_tiles(int) { return 1; }
 
-// Workgroups for whole rows, before the keys are split.
-int64_t row_items(const cbq_kv_batch* b, int rep) {
-  if (b->cu == nullptr) return static_cast<int64_t>(b->batch) * cdiv(rep, kRowTile);
-  return std::min<int64_t>(b->tokens * rep / kRowTile + b->batch, b->tokens * cdiv(rep, kRowTile));
-}
-
-int choose_splits(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t max_length) {
+KvPlan plan_of(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t max_length) {
+  KvPlan p = {};
+  const int64_t rows = b->tokens * rep;
+  p.long_tile = 128 * column_tiles(c->head_dim);
+  if (b->cu == nullptr) {
+    p.row_items = b->batch * cdiv(rep, kRowTile);
+  } else {
+    // n rows make at most n / t + 1 tiles of t
+    const bool one = b->batch == 1;
+    if (!one || rows <= kShortRows)
+      p.row_items = std::min(rows / kRowTile + b->batch, b->batch * cdiv(kShortRows, kRowTile));
+    if (rows > kShortRows)
+      p.long_items = one ? cdiv(rows, p.long_tile)
+                         : rows / p.long_tile + std::min<int64_t>(b->batch, rows / (kShortRows + 1));
+  }
   const int64_t cap = static_cast<int64_t>(b->max_pages) * c->page_size;
   const int64_t len = max_length > 0 ? std::min(max_length, cap) : cap;
-  const int64_t wgs = std::max<int64_t>(1, row_items(b, rep) * c->kv_heads);
-  const int64_t want = cdiv(2 * device_cus(), wgs);
-  const int64_t most = cdiv(cdiv(len, kStep), 4);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxSplits})));
+  const int64_t cus = device_cus();
+  p.row_splits = p.long_splits = 1;
+  if (p.row_items > 0) {
+    const int64_t want = cdiv(2 * cus, p.row_items * c->kv_heads);
+    p.row_splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, cdiv(cdiv(len, kStep), 4), kMaxSplits})));
+  }
+  if (p.long_items > 0) {
+    const int64_t want = cus / (p.long_items * c->kv_heads);
+    p.long_splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, cdiv(len, 8 * kStep), kMaxSplits})));
+  }
+  return p;
 }
 
-size_t split_bytes(const cbq_kv_cache* c, const cbq_kv_batch* b, int q_heads) {
-  return static_cast<size_t>(b->tokens) * q_heads * (c->head_dim + 2) * 4;
+size_t partial_bytes(const cbq_kv_cache* c, int64_t items, int tile) {
+  return static_cast<size_t>(items) * c->kv_heads * tile * (c->head_dim + 2) * 4;
 }
 
 }  // namespace
@@ -490,8 +888,11 @@ extern "C" size_t cbq_kv_attend_ws_bytes(const cbq_kv_cache* cache, const cbq_kv
   if (cache == nullptr || batch == nullptr || cache->kv_heads <= 0 || q_heads <= 0 ||
       q_heads % cache->kv_heads != 0 || batch->tokens <= 0)
     return CBQ_WS_CTRL_BYTES;
-  const int splits = choose_splits(cache, batch, q_heads / cache->kv_heads, max_length);
-  return CBQ_WS_CTRL_BYTES + (splits > 1 ? splits * split_bytes(cache, batch, q_heads) : 0);
+  const KvPlan p = plan_of(cache, batch, q_heads / cache->kv_heads, max_length);
+  size_t n = 0;
+  if (p.row_splits > 1) n += p.row_splits * partial_bytes(cache, p.row_items, kRowTile);
+  if (p.long_splits > 1) n += p.long_splits * partial_bytes(cache, p.long_items, p.long_tile);
+  return CBQ_WS_CTRL_BYTES + n;
 }
 
 extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batch, int dtype,
@@ -512,6 +913,7 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   CBQ_REQUIRE(out != nullptr && aligned(out, 16), "kv attend: out must be given, 16-byte aligned");
   CBQ_REQUIRE(ws == nullptr || aligned(ws, 256), "kv attend: workspace must be 256-byte aligned");
   const int rep = q_heads / cache->kv_heads;
+  CBQ_REQUIRE(batch->tokens * rep < (int64_t{1} << 31) - 512, "kv attend: too many tokens for one call");
   KvAttendArg a = {};
   a.m = kv_batch_of(cache, batch);
   if (cache->num_pages == 0) a.m.max_pages = 0;   // nothing to read: sequences with tokens give NaN
@@ -524,8 +926,9 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   a.vs = cache->v_scale;
   a.out = static_cast<char*>(out);
   a.lse = lse;
-  a.window = window;
-  a.scale_log2e = scale * kLog2e;
+  a.window = static_cast<int>(std::min<int64_t>(window, INT32_MAX));
+  a.negate = scale < 0.0f;
+  a.scale_log2e = __builtin_fabsf(scale) * kLog2e;
   a.hkv = cache->kv_heads;
   a.hq = q_heads;
   a.rep = rep;
@@ -533,42 +936,62 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   a.page = cache->page_size;
   a.causal = causal != 0;
   a.bf16 = dtype == CBQ_BF16;
-  a.tiles = static_cast<int>(cdiv(rep, kRowTile));
-  int splits = choose_splits(cache, batch, rep, max_length);
-  const size_t each = split_bytes(cache, batch, q_heads);
-  const size_t room = ws != nullptr && ws_bytes > CBQ_WS_CTRL_BYTES ? ws_bytes - CBQ_WS_CTRL_BYTES : 0;
-  splits = static_cast<int>(std::min<size_t>(splits, room / each));
-  if (splits < 1) splits = 1;
-  a.splits = splits;
-  const int64_t rows = batch->tokens * q_heads;
-  if (splits > 1) {
-    a.po = reinterpret_cast<float*>(static_cast<char*>(ws) + CBQ_WS_CTRL_BYTES);
-    a.pml = reinterpret_cast<float2*>(a.po + static_cast<int64_t>(splits) * rows * a.d);
-  }
-  const int64_t blocks = row_items(batch, rep) * a.hkv * splits;
-  CBQ_REQUIRE(blocks < (int64_t{1} << 31), "kv attend: too many tokens for one call");
-  const dim3 grid(static_cast<uint32_t>(blocks));
+  const KvPlan p = plan_of(cache, batch, rep, max_length);
+  size_t room = ws != nullptr && ws_bytes > CBQ_WS_CTRL_BYTES ? ws_bytes - CBQ_WS_CTRL_BYTES : 0;
+  char* scratch = static_cast<char*>(ws) + CBQ_WS_CTRL_BYTES;
   hipStream_t st = as_stream(stream);
-  auto launch = [&](auto stc) {
-    constexpr int ST = decltype(stc)::value;
-    auto one = [&](auto dpc) {
-      constexpr int DP = decltype(dpc)::value;
+  // One launch over `items` tiles of `tile` rows, the keys in `splits` ranges (as
+  // many as the workspace has room for), and the launch that joins them.
+  auto run = [&](int64_t items, int tile, int splits, auto kernel) -> int {
+    const size_t each = partial_bytes(cache, items, tile);
+    splits = std::max(1, static_cast<int>(std::min<size_t>(splits, room / each)));
+    a.items = items;
+    a.tile_rows = tile;
+    a.splits = splits;
+    a.prows = items * a.hkv * tile;
+    if (splits > 1) {
+      a.pml = reinterpret_cast<float2*>(scratch);
+      a.po = reinterpret_cast<float*>(a.pml + splits * a.prows);   // 16-byte aligned: prows is even
+      scratch += splits * each;
+      room -= splits * each;
+    }
+    const int blocks = items * a.hkv * splits;
+    const int64_t joins = items * a.hkv * (tile / 4);
+    CBQ_REQUIRE(blocks < (int64_t{1} << 31) && joins < (int64_t{1} << 31),
+                "kv attend: too many tokens for one call");
+    const dim3 grid(static_cast<uint32_t>(blocks));
+    auto by_dim = [&](auto stc) {
+      switch (padded_dim(a.d)) {
+        case 64: kernel(grid, stc, std::integral_constant<int, 64>{}); break;
+        case 128: kernel(grid, stc, std::integral_constant<int, 128>{}); break;
+        case 192: kernel(grid, stc, std::integral_constant<int, 192>{}); break;
+        default: kernel(grid, stc, std::integral_constant<int, 256>{}); break;
+      }
+    };
+    if (cache->store == CBQ_KV_INT8) by_dim(std::integral_constant<int, kKvInt8>{});
+    else by_dim(std::integral_constant<int, kKvFp8>{});
+    if (int rc = launch_status("cbq_kv_attend")) return rc;
+    if (splits == 1) return CBQ_OK;
+    k_kv_attend_join<<<dim3(static_cast<uint32_t>(joins)), kBlock, 0, st>>>(a);
+    return launch_status("cbq_kv_attend");
+  };
+  if (p.row_items > 0) {
+    a.row_min = 1;
+    a.row_max = kShortRows;
+    const int rc = run(p.row_items, kRowTile, p.row_splits, [&](dim3 grid, auto stc, auto dpc) {
+      constexpr int ST = decltype(stc)::value, DP = decltype(dpc)::value;
       if (a.d == DP) k_kv_attend_rows<ST, DP, true><<<grid, kBlock, 0, st>>>(a);
       else k_kv_attend_rows<ST, DP, false><<<grid, kBlock, 0, st>>>(a);
-    };
-    switch (padded_dim(a.d)) {
-      case 64: one(std::integral_constant<int, 64>{}); break;
-      case 128: one(std::integral_constant<int, 128>{}); break;
-      case 192: one(std::integral_constant<int, 192>{}); break;
-      default: one(std::integral_constant<int, 256>{}); break;
-    }
-  };
-  if (cache->store == CBQ_KV_INT8) launch(std::integral_constant<int, kKvInt8>{});
-  else launch(std::integral_constant<int, kKvFp8>{});
-  if (int rc = launch_status("cbq_kv_attend")) return rc;
-  if (splits > 1) {
-    k_kv_attend_join<<<dim3(static_cast<uint32_t>(cdiv(rows, 4))), kBlock, 0, st>>>(a, rows);
-    return launch_status("cbq_kv_attend");
+    });
+    if (rc) return rc;
+  }
+  if (p.long_items > 0) {
+    a.row_min = kShortRows + 1;
+    a.row_max = int64_t{1} << 62;
+    return run(p.long_items, p.long_tile, p.long_splits, [&](dim3 grid, auto stc, auto dpc) {
+      constexpr int ST = decltype(stc)::value, DP = decltype(dpc)::value;
+      k_kv_attend_long<ST, DP, 1><<<grid, kBlock, 0, st>>>(a);
+    });
   }
   return CBQ_OK;
 }
