@@ -32,11 +32,15 @@ constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kMaxSplits = 64;      // one lane of the joining wave each
 constexpr int kRowTile = 16;        // query rows of a workgroup
+constexpr int kLongTile = 128;      // the same in k_kv_attend_long
 constexpr int kStep = 64;           // keys of a wave's step
 // The running maximum is raised only when a tile exceeds it by 2^8: weights
 // then stay below 2^8, far from fp16's 65504, and most steps do not touch the
 // accumulators.
 constexpr float kRaise = 8.0f;
+// k_kv_attend_long: the most that a lane's 32 weights of a step may sum to
+// before the maximum is raised (none is past fp16's range then).
+constexpr float kMostWeight = 0x1p14f;
 // A scale below this counts as this: log2 of a page scale of 0 (a page of a
 // zero-filled pool, which stands for zeros) must stay finite. append's scales
 // are at least 1e-12 / 448 > 2^-49.
@@ -101,6 +105,10 @@ __device__ __forceinline__ float max_groups(float v) {
 __device__ __forceinline__ float sum_groups(float v) {
   v += __shfl_xor(v, 16, 64);
   return v + __shfl_xor(v, 32, 64);
+}
+
+__device__ __forceinline__ float read_lane(float v, int l) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), l));
 }
 
 __device__ __forceinline__ float max_halves(float v) {
@@ -483,9 +491,8 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
 // ---------------------------------------------------------------------------
 // Many query rows: prompts and chunks of them.
 // ---------------------------------------------------------------------------
-// A workgroup takes 4 * 32 * CT rows of one kv head, a wave 32 * CT of them in
-// CT column tiles of 32; the workgroup goes through the keys 64 at a time. Codes
-// are widened to fp16 once per workgroup, on their way from registers to LDS (K
+// A workgroup takes 128 rows of one kv head, a wave 32 of them; the workgroup
+// goes through the keys 64 at a time. Codes are widened to fp16 once per workgroup, on their way from registers to LDS (K
 // rows [64 keys][DP], V^T rows [DP][64 keys]; every row has 16 bytes more than it
 // needs, so an odd number of 16-byte chunks: equal chunks of 16 consecutive rows
 // lie in distinct banks, and every access is a base register plus a constant), in
@@ -496,16 +503,18 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
 // lane's scores 8 u .. 8 u + 7 are then the keys 16 u + 8 (lane / 32) .. + 7, the
 // operand of the second product's step u. Each such 16 keys lie in one page, so
 // their scales are the same in the whole wave.
-template <int ST, int DP, int CT>
-__global__ __launch_bounds__(kBlock, DP * CT <= 128 ? 2 : 1) void k_kv_attend_long(const KvAttendArg a) {
-  constexpr int ROWS = 4 * 32 * CT;
+template <int ST, int DP, bool EXACT>
+__global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_long(const KvAttendArg a) {
   constexpr int NS = DP / 16;          // steps of 16 dimensions in the scores
   constexpr int ND = DP / 32;          // tiles of 32 dimensions
   constexpr int NL = DP / 64;          // 16-code loads per thread and side
-  constexpr int KR = DP / 8 + 1, VR = kStep / 8 + 1;   // 16-byte chunks of a row
+  constexpr int KC = DP / 16;          // 16-code pieces of a key
+  constexpr int KR = DP / 8 + 1, VR = kStep / 8 + 1;   // 16-byte chunks of a row in LDS
+  const int d = EXACT ? DP : a.d;
   __shared__ u32x4 lk[2][kStep * KR];
   __shared__ u32x4 lv[2][DP * VR];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, hf = lane >> 5;
 
   const int h = blockIdx.x % a.hkv;
@@ -514,227 +523,201 @@ __global__ __launch_bounds__(kBlock, DP * CT <= 128 ? 2 : 1) void k_kv_attend_lo
   const int64_t item = a.items - 1 - rest / a.splits;   // a causal prompt's longest rows first
   const KvTile tl = tile_of(a, item);
   if (tl.b < 0) return;
-  const int b = tl.b;
   const KvSeq s = tl.s;
   const int64_t cap = capacity(a);
   const bool bad = s.len > cap;
   const int len = static_cast<int>(s.len < 0 ? 0 : bad ? cap : s.len);
   const int rows = tl.rows, r_first = tl.r_first, n = static_cast<int>(s.n);
-  const int r_last = r_first + ROWS - 1 < rows ? r_first + ROWS - 1 : rows - 1;
+  const int r_last = r_first + kLongTile - 1 < rows ? r_first + kLongTile - 1 : rows - 1;
   const int all_hi = keys_of(a, len, n, r_last / a.rep).hi;
   const int kb = keys_of(a, len, n, r_first / a.rep).lo / kStep;
   const int ke = (all_hi + kStep - 1) / kStep;
-  int per = (ke - kb + a.splits - 1) / a.splits;
+  const int per = (ke - kb + a.splits - 1) / a.splits;
   const int s0 = kb + split * per;
   const int s1 = s0 + per < ke ? s0 + per : ke;
 
-  // this wave's rows
-  const int w_first = r_first + wave * 32 * CT;
+  // this wave's rows, and this lane's
+  const int w_first = r_first + wave * 32;
   const bool w_any = w_first < rows;
-  const int w_last = w_first + 32 * CT - 1 < rows ? w_first + 32 * CT - 1 : rows - 1;
+  const int w_last = w_first + 31 < rows ? w_first + 31 : rows - 1;
   const KeyRange wf = keys_of(a, len, n, (w_any ? w_first : w_last) / a.rep);
   const KeyRange wl = keys_of(a, len, n, w_last / a.rep);
-  KeyRange mine[CT];
-  int64_t orow[CT];
-  bool has[CT];
-  f16x o[ND][CT] = {};
-  float m[CT], l[CT], cq[CT];
-  u32x4 qf[NS][CT];
-#pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    const int r = w_first + 32 * c + n32;
-    has[c] = r < rows;
-    const int ti = (has[c] ? r : rows - 1) / a.rep;
-    const int head = h * a.rep + (has[c] ? r : rows - 1) - ti * a.rep;
-    mine[c] = keys_of(a, len, n, ti);
-    orow[c] = (s.tok0 + ti) * a.hq + head;
-    m[c] = kNegInf;
-    l[c] = 0.0f;
-    const char* qp = a.q + (s.tok0 + ti) * a.qts + head * a.qhs;
-    load_q<NS>(a, qp, has[c], [&](int k) { return 16 * k + 8 * hf; },
-               [](float v) { return max_halves(v); }, cq[c], [&](int k) -> u32x4& { return qf[k][c]; });
-  }
+  const bool has = w_first + n32 < rows;
+  const int r = has ? w_first + n32 : rows - 1;
+  const int ti = r / a.rep;
+  const int head = h * a.rep + r - ti * a.rep;
+  const KeyRange mine = keys_of(a, len, n, ti);
+  f16x o[ND] = {};
+  float m = kNegInf, l = 0.0f, cq;
+  u32x4 qf[NS];
+  load_q<NS>(a, a.q + (s.tok0 + ti) * a.qts + head * a.qhs, has, [&](int k) { return 16 * k + 8 * hf; },
+             [](float v) { return max_halves(v); }, cq, [&](int k) -> u32x4& { return qf[k]; });
 
+  // A step's 64 keys are four blocks of 16 (those past the last are read as the
+  // last, masked). Lane l keeps the page id and scales of block l % 4.
   const int last_block = (all_hi - 1) >> 4;
   const int shift = a.m.page_shift;
-  const int32_t* trow = a.m.table + b * a.m.tstride;
-  auto valid = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.m.num_pages); };
-  // Block bl of 16 keys (those past the last are read as the last, masked): its
-  // page id and its place in the page. Ids of a step's four blocks are loaded
-  // steps before the codes that need them.
-  auto clamp_block = [&](int bl) { return bl < last_block ? bl : last_block; };
-  auto place_of = [&](int bl) { return (clamp_block(bl) << 4) & (a.page - 1); };
-  auto load_ids = [&](int st, int (&id)[4]) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) id[q] = trow[(clamp_block(st * 4 + q) << 4) >> shift];
+  const int32_t* trow = a.m.table + tl.b * a.m.tstride;
+  auto block_of = [&](int st, int q) {
+    const int bl = st * 4 + q;
+    return bl < last_block ? bl : last_block;
   };
-  auto pick = [](const int (&id)[4], int q) {
-    const int lo = q & 1 ? id[1] : id[0], hi = q & 1 ? id[3] : id[2];
-    return q & 2 ? hi : lo;
-  };
-  auto head_of = [&](int id) { return static_cast<int64_t>(valid(id) ? id : 0) * a.hkv + h; };
-  auto load_scales = [&](const int (&id)[4], float (&ks)[4], float (&vs)[4]) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      ks[q] = a.ks[head_of(id[q])];
-      if (!valid(id[q])) ks[q] = __builtin_nanf("");
-      vs[q] = a.vs[head_of(id[q])];
-    }
-  };
+  auto id_of = [&](int st) { return trow[(block_of(st, lane & 3) << 4) >> shift]; };
+  auto known = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.m.num_pages); };
   u32x4 rk[NL], rv[NL];
-  // thread -> 16 codes of key kt, dimensions 16 kc ..; of dimension vd, keys 16 vb ..
-  constexpr int KC = DP / 16;          // 16-code pieces of a key
-  auto load_k = [&](int st, const int (&id)[4]) {
+  const int kdim = 16 * (lane % KC), kkey = lane / KC;   // of this lane's first piece of a block of keys
+  // Wave w takes the keys of block w, all threads the values: lane's block l % 4
+  // of dimension tid / 4.
+  auto load_codes = [&](int st, int id) {
+    id = known(id) ? id : 0;
+    const int idk = __builtin_amdgcn_readlane(id, wave);
+    const uint8_t* kp = a.kc + ((static_cast<int64_t>(idk) * a.hkv + h) * a.page +
+                                ((block_of(st, wave) << 4) & (a.page - 1))) * d;
+    const uint8_t* vp = a.vc + (static_cast<int64_t>(id) * a.hkv + h) * a.page * d +
+                        ((block_of(st, lane & 3) << 4) & (a.page - 1)) + (tid >> 2) * a.page;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int u = tid + kBlock * i, key = u / KC, kc = u % KC;
-      rk[i] = u32x4{0, 0, 0, 0};
-      if (16 * kc < a.d)
-        rk[i] = *reinterpret_cast<const u32x4*>(
-            a.kc + (head_of(pick(id, key >> 4)) * a.page + place_of(st * 4 + (key >> 4)) + (key & 15)) * a.d + 16 * kc);
+      const int e = lane + 64 * i;
+      const int key = 64 % KC == 0 ? kkey + 64 / KC * i : e / KC;
+      const int dim = 64 % KC == 0 ? kdim : 16 * (e % KC);
+      if (!EXACT) rk[i] = u32x4{0, 0, 0, 0};
+      if (EXACT || dim < d) rk[i] = *reinterpret_cast<const u32x4*>(kp + (key * d + dim));
+      if (!EXACT) rv[i] = u32x4{0, 0, 0, 0};
+      if (EXACT || (tid >> 2) + 64 * i < d) rv[i] = *reinterpret_cast<const u32x4*>(vp + 64 * i * a.page);
     }
   };
-  auto load_v = [&](int st, const int (&id)[4]) {
+  auto store_codes = [&](int buf) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int u = tid + kBlock * i, vb = u & 3, vd = u >> 2;
-      rv[i] = u32x4{0, 0, 0, 0};
-      if (vd < a.d)
-        rv[i] = *reinterpret_cast<const u32x4*>(
-            a.vc + (head_of(pick(id, vb)) * a.d + vd) * a.page + place_of(st * 4 + vb));
-    }
-  };
-  auto store_k = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int u = tid + kBlock * i, key = u / KC, kc = u % KC;
-      lk[buf][key * KR + 2 * kc] = widen8<ST>(rk[i].x, rk[i].y);
-      lk[buf][key * KR + 2 * kc + 1] = widen8<ST>(rk[i].z, rk[i].w);
-    }
-  };
-  auto store_v = [&](int buf) {
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int u = tid + kBlock * i, vb = u & 3, vd = u >> 2;
-      lv[buf][vd * VR + 2 * vb] = widen8<ST>(rv[i].x, rv[i].y);
-      lv[buf][vd * VR + 2 * vb + 1] = widen8<ST>(rv[i].z, rv[i].w);
+      const int e = lane + 64 * i;
+      const int key = 64 % KC == 0 ? kkey + 64 / KC * i : e / KC;
+      const int dim = 64 % KC == 0 ? kdim : 16 * (e % KC);
+      u32x4* kp = &lk[buf][(16 * wave + key) * KR + dim / 8];
+      kp[0] = widen8<ST>(rk[i].x, rk[i].y);
+      kp[1] = widen8<ST>(rk[i].z, rk[i].w);
+      u32x4* vp = &lv[buf][((tid >> 2) + 64 * i) * VR + 2 * (lane & 3)];
+      vp[0] = widen8<ST>(rv[i].x, rv[i].y);
+      vp[1] = widen8<ST>(rv[i].z, rv[i].w);
     }
   };
   const int krow = (n32 & 0x13) | ((n32 & 4) << 1) | ((n32 & 8) >> 1);
-  f16x sc[2][CT];
-  auto scores = [&](int buf, f16x (&out)[2][CT]) {
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int c = 0; c < CT; ++c) out[kt][c] = f16x{};
-#pragma unroll
-    for (int k = 0; k < NS; ++k)
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        const int key = 32 * kt + krow;
-        const u32x4 kk = lk[buf][key * KR + 2 * k + hf];
-#pragma unroll
-        for (int c = 0; c < CT; ++c) out[kt][c] = mfma32x32x16<kF16>(kk, qf[k][c], out[kt][c]);
-      }
-  };
 
   if (s0 < s1) {
-    int id1[4], id2[4];                // of steps st + 1, st + 2
-    float ksc[4], vsc[4], ksn[4] = {}, vsn[4] = {};
-    load_ids(s0, id1);
-    load_ids(s0 + 1, id2);
-    load_k(s0, id1);
-    load_v(s0, id1);
-    load_scales(id1, ksc, vsc);
-    store_k(0);
-    store_v(0);
-    load_k(s0 + 1, id2);               // (steps past the range read its end again, unused)
-    load_v(s0 + 1, id2);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) id1[q] = id2[q];
-    load_ids(s0 + 2, id2);
+    int id = id_of(s0), id_next = id_of(s0 + 1);     // (steps past the range read its end again, unused)
+    load_codes(s0, id);
+    auto scale_at = [&](const float* p, int i) { return p[static_cast<int64_t>(known(i) ? i : 0) * a.hkv + h]; };
+    float ks = known(id) ? scale_at(a.ks, id) : __builtin_nanf(""), vs = scale_at(a.vs, id);
+    store_codes(0);
+    load_codes(s0 + 1, id_next);
+    id = id_next;
+    id_next = id_of(s0 + 2);
     __syncthreads();
 
     for (int st = s0; st < s1; ++st) {
       const int buf = (st - s0) & 1;
       const int tb = st * kStep;
-      load_scales(id1, ksn, vsn);
-      float vsx[4], lvs[4];
+      // this step's scales, one block of 16 keys per lane; the next ones
+      vs = vs < kTinyScale ? kTinyScale : vs;
+      const float lane_lvs = __builtin_amdgcn_logf(vs), lane_ivs = __builtin_amdgcn_rcpf(vs);
+      float ksq[4], lvs[4], ivs[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        vsx[q] = vsc[q] < kTinyScale ? kTinyScale : vsc[q];
-        lvs[q] = __builtin_amdgcn_logf(vsx[q]);
+        ksq[q] = read_lane(ks, q);
+        lvs[q] = read_lane(lane_lvs, q);
+        ivs[q] = read_lane(lane_ivs, q);
       }
-      const bool active = w_any && tb < wl.hi && tb + kStep > wf.lo;
-      const bool masked = tb + kStep > wf.hi || tb < wl.lo;
-      u32x4 p[4][CT];
-      if (active) {
-        scores(buf, sc);
+      ks = known(id) ? scale_at(a.ks, id) : __builtin_nanf("");
+      vs = scale_at(a.vs, id);
+
+      if (w_any && tb < wl.hi && tb + kStep > wf.lo) {
+        const bool masked = tb + kStep > wf.hi || tb < wl.lo;
+        f16x sc[2];
+#pragma unroll
+        for (int k = 0; k < NS; ++k)
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) {
+            const u32x4 kk = lk[buf][(32 * kt + krow) * KR + 2 * k + hf];
+            sc[kt] = mfma32x32x16<kF16>(kk, qf[k], k == 0 ? f16x{} : sc[kt]);
+          }
         __builtin_amdgcn_sched_barrier(0);
-        if (masked) {
-          // scores become y, those of keys that the row does not see -infinity
+        auto hidden = [&](int q, int i) {
+          const int j = tb + 16 * q + 8 * hf + i;
+          return j < mine.lo || j >= mine.hi;
+        };
+        // Weights against the maximum so far: as long as none is past fp16's
+        // range it stays (their sum tells); else, and at first, it is raised to
+        // the step's own and the weights are made again.
+        u32x4 p[4];
+        float part[4];
+        auto weigh = [&](auto mask) {
+          const float ref = m == kNegInf ? 0.0f : m;
 #pragma unroll
-          for (int c = 0; c < CT; ++c)
+          for (int q = 0; q < 4; ++q) {
+            const float f = cq * ksq[q], off = lvs[q] - ref;
+            part[q] = 0.0f;
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
+            for (int i = 0; i < 4; ++i) {
+              float w[2];
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int j = tb + 32 * kt + 16 * (i >> 3) + 8 * hf + (i & 7);
-                if (j < mine[c].lo || j >= mine[c].hi) sc[kt][c][i] = kNegInf;
+              for (int e = 0; e < 2; ++e) {
+                const float x = sc[q >> 1][8 * (q & 1) + 2 * i + e];
+                w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, f, off));
+                if (mask.value && hidden(q, 2 * i + e)) w[e] = 0.0f;   // whatever its scale is
               }
-        }
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
+              p[q][i] = pack2_out<kF16>(w[0], w[1]);
+              part[q] += w[0] + w[1];   // before their rounding: the sum also counts what is far below
+                                        // fp16's range here and large once divided by its scale
+            }
+          }
+        };
+        auto raise = [&](auto mask, bool mine_needs) {
+          // a row whose two lanes need no raising stays as it is, whatever the
+          // wave's other rows do
+          const bool needs = max_halves(mine_needs ? 1.0f : 0.0f) != 0.0f;
           float mx = kNegInf;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            float t = sc[q >> 1][c][8 * (q & 1)];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) t = fmaxf(t, sc[q >> 1][c][8 * (q & 1) + i]);
-            const float y = __builtin_fmaf(t, cq[c] * ksc[q], lvs[q]);
-            mx = fmaxf(mx, t == kNegInf ? kNegInf : y);
-          }
-          mx = max_halves(mx);
-          const bool raise = mx > m[c] + kRaise;
-          if (__any(raise)) {
-            const float to = raise ? mx : m[c];
-            const float f = raise ? __builtin_amdgcn_exp2f(m[c] - to) : 1.0f;
-            m[c] = to;
-            l[c] *= f;
-#pragma unroll
-            for (int t = 0; t < ND; ++t) o[t][c] *= f;
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          const float ref = m[c] == kNegInf ? 0.0f : m[c];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float f = cq[c] * ksc[q], off = lvs[q] - ref;
-            float w[8];
-            float sum = 0.0f;
+            const float f = cq * ksq[q];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const float x = sc[q >> 1][c][8 * (q & 1) + i];
-              w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, f, off));
-              if (masked && x == kNegInf) w[i] = 0.0f;   // whatever the scale is
-              sum += w[i];
+              const float y = __builtin_fmaf(sc[q >> 1][8 * (q & 1) + i], f, lvs[q]);
+              mx = fmaxf(mx, mask.value && hidden(q, i) ? kNegInf : y);
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[q][c][i] = pack2_out<kF16>(w[2 * i], w[2 * i + 1]);
-            l[c] += sum == 0.0f ? 0.0f : sum * (1.0f / vsx[q]);
           }
-        }
+          const float top = fmaxf(max_halves(mx), m);
+          mx = needs ? top : m;
+          const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - mx);
+          m = mx;
+          l *= f;
 #pragma unroll
-        for (int t = 0; t < ND; ++t)
+          for (int t = 0; t < ND; ++t) o[t] *= f;
+        };
+        auto soften = [&](auto mask) {
+          weigh(mask);
+          const float sum = (part[0] + part[1]) + (part[2] + part[3]);
+          const bool needs = !(sum <= kMostWeight) || m == kNegInf;
+          if (__any(needs)) {
+            raise(mask, needs);
+            weigh(mask);
+          }
+        };
+        if (masked) soften(std::true_type{});
+        else soften(std::false_type{});
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int vd = 32 * t + n32;
-            u32x4 vv = lv[buf][vd * VR + 2 * q + hf];
-            if constexpr (ST == kKvFp8) {
-              // NaN values must reach only the rows that see their key
-              if (masked) {
-                u32x4 ind = {0, 0, 0, 0};
+        for (int q = 0; q < 4; ++q) l += part[q] == 0.0f ? 0.0f : part[q] * ivs[q];
+        __builtin_amdgcn_sched_barrier(0);
+
+        bool checked = false;
+        if constexpr (ST == kKvFp8) {
+          if (masked) {
+            // NaN values must reach only the rows that see their key (0 x NaN is NaN)
+            checked = true;
+#pragma unroll
+            for (int t = 0; t < ND; ++t)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                u32x4 vv = lv[buf][(32 * t + n32) * VR + 2 * q + hf];
+                u32x4 ind = {0, 0, 0, 0};      // 1 at NaN values
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   if ((vv[i] & 0x7fffu) > 0x7c00u) ind[i] |= 0x3c00u;
@@ -742,58 +725,48 @@ __global__ __launch_bounds__(kBlock, DP * CT <= 128 ? 2 : 1) void k_kv_attend_lo
                   vv[i] &= ~((ind[i] >> 10) * 0x1111u);   // 0x3c00 >> 10 = 0xf
                 }
                 if (__any((ind.x | ind.y | ind.z | ind.w) != 0)) {
+                  u32x4 seen;
 #pragma unroll
-                  for (int c = 0; c < CT; ++c) {
-                    u32x4 seen;
+                  for (int i = 0; i < 4; ++i)
+                    seen[i] = (hidden(q, 2 * i) ? 0u : 0x3c00u) | (hidden(q, 2 * i + 1) ? 0u : 0x3c000000u);
+                  const f16x cnt = mfma32x32x16<kF16>(ind, seen, f16x{});
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                      const int j = tb + 16 * q + 8 * hf + 2 * i;
-                      seen[i] = (j >= mine[c].lo && j < mine[c].hi ? 0x3c00u : 0u) |
-                                (j + 1 >= mine[c].lo && j + 1 < mine[c].hi ? 0x3c000000u : 0u);
-                    }
-                    const f16x cnt = mfma32x32x16<kF16>(ind, seen, f16x{});
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                      if (cnt[i] > 0.0f) o[t][c][i] = __builtin_nanf("");
-                  }
+                  for (int i = 0; i < 16; ++i)
+                    if (cnt[i] > 0.0f) o[t][i] = __builtin_nanf("");
                 }
+                o[t] = mfma32x32x16<kF16>(vv, p[q], o[t]);
               }
-            }
-#pragma unroll
-            for (int c = 0; c < CT; ++c) o[t][c] = mfma32x32x16<kF16>(vv, p[q][c], o[t][c]);
           }
+        }
+        if (!checked) {
+#pragma unroll
+          for (int t = 0; t < ND; ++t)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              o[t] = mfma32x32x16<kF16>(lv[buf][(32 * t + n32) * VR + 2 * q + hf], p[q], o[t]);
+        }
       }
       if (st + 1 < s1) {
-        store_k(buf ^ 1);
-        store_v(buf ^ 1);
-        load_k(st + 2, id2);
-        load_v(st + 2, id2);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          ksc[q] = ksn[q];
-          vsc[q] = vsn[q];
-          id1[q] = id2[q];
-        }
-        load_ids(st + 3, id2);
+        store_codes(buf ^ 1);
+        load_codes(st + 2, id_next);
+        id = id_next;
+        id_next = id_of(st + 3);
       }
       __syncthreads();
     }
   }
+  const float sum = l + __shfl_xor(l, 32, 64);
+  if (!has) return;
+  const int64_t orow = (s.tok0 + ti) * a.hq + head;
 #pragma unroll
-  for (int c = 0; c < CT; ++c) {
-    const float sum = l[c] + __shfl_xor(l[c], 32, 64);
-    if (!has[c]) continue;
+  for (int t = 0; t < ND; ++t)
 #pragma unroll
-    for (int t = 0; t < ND; ++t)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int d0 = 32 * t + 8 * q + 4 * hf;
-        if (d0 < a.d)
-          put_row(a, orow[c], (item * a.hkv + h) * ROWS + wave * 32 * CT + 32 * c + n32, split, d0,
-                  f4{o[t][c][4 * q], o[t][c][4 * q + 1], o[t][c][4 * q + 2], o[t][c][4 * q + 3]},
-                  m[c], sum, bad);
-      }
-  }
+    for (int q = 0; q < 4; ++q) {
+      const int d0 = 32 * t + 8 * q + 4 * hf;
+      if (EXACT || d0 < d)
+        put_row(a, orow, (item * a.hkv + h) * kLongTile + wave * 32 + n32, split, d0,
+                f4{o[t][4 * q], o[t][4 * q + 1], o[t][4 * q + 2], o[t][4 * q + 3]}, m, sum, bad);
+    }
 }
 
 // Joins the splits' partial results: a wave per row, a workgroup per 4 rows of a
@@ -836,18 +809,15 @@ __global__ __launch_bounds__(kBlock) void k_kv_attend_join(const KvAttendArg a) 
 struct KvPlan {
   int64_t row_items, long_items;
   int row_splits, long_splits;
-  int long_tile;
 };
 
 constexpr int64_t kShortRows = 64;
 
 int padded_dim(int d) { return (d + 63) / 64 * 64; }
-int column_tiles(int) { return 1; }
 
 KvPlan plan_of(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t max_length) {
   KvPlan p = {};
   const int64_t rows = b->tokens * rep;
-  p.long_tile = 128 * column_tiles(c->head_dim);
   if (b->cu == nullptr) {
     p.row_items = b->batch * cdiv(rep, kRowTile);
   } else {
@@ -856,8 +826,8 @@ KvPlan plan_of(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t ma
     if (!one || rows <= kShortRows)
       p.row_items = std::min(rows / kRowTile + b->batch, b->batch * cdiv(kShortRows, kRowTile));
     if (rows > kShortRows)
-      p.long_items = one ? cdiv(rows, p.long_tile)
-                         : rows / p.long_tile + std::min<int64_t>(b->batch, rows / (kShortRows + 1));
+      p.long_items = one ? cdiv(rows, kLongTile)
+                         : rows / kLongTile + std::min<int64_t>(b->batch, rows / (kShortRows + 1));
   }
   const int64_t cap = static_cast<int64_t>(b->max_pages) * c->page_size;
   const int64_t len = max_length > 0 ? std::min(max_length, cap) : cap;
@@ -891,7 +861,7 @@ extern "C" size_t cbq_kv_attend_ws_bytes(const cbq_kv_cache* cache, const cbq_kv
   const KvPlan p = plan_of(cache, batch, q_heads / cache->kv_heads, max_length);
   size_t n = 0;
   if (p.row_splits > 1) n += p.row_splits * partial_bytes(cache, p.row_items, kRowTile);
-  if (p.long_splits > 1) n += p.long_splits * partial_bytes(cache, p.long_items, p.long_tile);
+  if (p.long_splits > 1) n += p.long_splits * partial_bytes(cache, p.long_items, kLongTile);
   return CBQ_WS_CTRL_BYTES + n;
 }
 
@@ -988,9 +958,10 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   if (p.long_items > 0) {
     a.row_min = kShortRows + 1;
     a.row_max = int64_t{1} << 62;
-    return run(p.long_items, p.long_tile, p.long_splits, [&](dim3 grid, auto stc, auto dpc) {
+    return run(p.long_items, kLongTile, p.long_splits, [&](dim3 grid, auto stc, auto dpc) {
       constexpr int ST = decltype(stc)::value, DP = decltype(dpc)::value;
-      k_kv_attend_long<ST, DP, 1><<<grid, kBlock, 0, st>>>(a);
+      if (a.d == DP) k_kv_attend_long<ST, DP, true><<<grid, kBlock, 0, st>>>(a);
+      else k_kv_attend_long<ST, DP, false><<<grid, kBlock, 0, st>>>(a);
     });
   }
   return CBQ_OK;
