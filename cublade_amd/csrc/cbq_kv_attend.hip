@@ -32,7 +32,6 @@ constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kLog2e = 1.44269504088896341f;
 constexpr int kMaxSplits = 64;      // one lane of the joining wave each
 constexpr int kRowTile = 16;        // query rows of a workgroup
-constexpr int kLongTile = 128;      // the same in k_kv_attend_long
 constexpr int kStep = 64;           // keys of a wave's step
 // The running maximum is raised only when a tile exceeds it by 2^8: weights
 // then stay below 2^8, far from fp16's 65504, and most steps do not touch the
@@ -105,6 +104,13 @@ __device__ __forceinline__ float max_groups(float v) {
 __device__ __forceinline__ float sum_groups(float v) {
   v += __shfl_xor(v, 16, 64);
   return v + __shfl_xor(v, 32, 64);
+}
+
+// v, hidden from the optimiser: what is computed from it stays where it is (the
+// masks of rare steps would otherwise be prepared in every step).
+__device__ __forceinline__ int opaque(int v) {
+  asm("" : "+v"(v));
+  return v;
 }
 
 __device__ __forceinline__ float read_lane(float v, int l) {
@@ -236,8 +242,10 @@ __device__ __forceinline__ KvTile tile_of(const KvAttendArg& a, int64_t item) {
     t.b = static_cast<int>(item / per);
     tile = item % per;
   } else {
-    t.b = kv_find(a.m, item, tile, RowTiles{a.rep, a.tile_rows, a.row_min, a.row_max});
+    t.b = __builtin_amdgcn_readfirstlane(
+        kv_find(a.m, item, tile, RowTiles{a.rep, a.tile_rows, a.row_min, a.row_max}));
     if (t.b < 0) return t;
+    tile = __builtin_amdgcn_readfirstlane(static_cast<int>(tile));   // the same in all lanes
   }
   t.s = kv_seq(a.m, t.b);
   t.rows = static_cast<int>(t.s.n) * a.rep;
@@ -503,16 +511,19 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
 // lane's scores 8 u .. 8 u + 7 are then the keys 16 u + 8 (lane / 32) .. + 7, the
 // operand of the second product's step u. Each such 16 keys lie in one page, so
 // their scales are the same in the whole wave.
-template <int ST, int DP, bool EXACT>
-__global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_long(const KvAttendArg a) {
+template <int ST, int DP, bool EXACT, int NW>
+__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_kv_attend_long(const KvAttendArg a) {
+  constexpr int kLongTile = 32 * NW;
   constexpr int NS = DP / 16;          // steps of 16 dimensions in the scores
   constexpr int ND = DP / 32;          // tiles of 32 dimensions
-  constexpr int NL = DP / 64;          // 16-code loads per thread and side
+  constexpr int NL = DP / (16 * NW);   // 16-code loads per thread and side
   constexpr int KC = DP / 16;          // 16-code pieces of a key
   constexpr int KR = DP / 8 + 1, VR = kStep / 8 + 1;   // 16-byte chunks of a row in LDS
   const int d = EXACT ? DP : a.d;
   __shared__ u32x4 lk[2][kStep * KR];
   __shared__ u32x4 lv[2][DP * VR];
+  __shared__ uint16_t lnan[2][ST == kKvFp8 ? DP * 4 : 1];
+  __shared__ int lnan_any[2][NW];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, hf = lane >> 5;
@@ -565,37 +576,63 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_long(co
   auto id_of = [&](int st) { return trow[(block_of(st, lane & 3) << 4) >> shift]; };
   auto known = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.m.num_pages); };
   u32x4 rk[NL], rv[NL];
-  const int kdim = 16 * (lane % KC), kkey = lane / KC;   // of this lane's first piece of a block of keys
-  // Wave w takes the keys of block w, all threads the values: lane's block l % 4
-  // of dimension tid / 4.
+  // NW / 4 waves take the keys of each block, all threads the values: lane's block
+  // l % 4 of dimension tid / 4.
+  const int kblock = wave / (NW / 4), kfirst = (wave % (NW / 4)) * (DP / (NW / 4));
   auto load_codes = [&](int st, int id) {
     id = known(id) ? id : 0;
-    const int idk = __builtin_amdgcn_readlane(id, wave);
+    const int idk = __builtin_amdgcn_readlane(id, kblock);
     const uint8_t* kp = a.kc + ((static_cast<int64_t>(idk) * a.hkv + h) * a.page +
-                                ((block_of(st, wave) << 4) & (a.page - 1))) * d;
+                                ((block_of(st, kblock) << 4) & (a.page - 1))) * d;
     const uint8_t* vp = a.vc + (static_cast<int64_t>(id) * a.hkv + h) * a.page * d +
                         ((block_of(st, lane & 3) << 4) & (a.page - 1)) + (tid >> 2) * a.page;
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int e = lane + 64 * i;
-      const int key = 64 % KC == 0 ? kkey + 64 / KC * i : e / KC;
-      const int dim = 64 % KC == 0 ? kdim : 16 * (e % KC);
+      const int e = kfirst + lane + 64 * i, key = e / KC, dim = 16 * (e % KC);
       if (!EXACT) rk[i] = u32x4{0, 0, 0, 0};
       if (EXACT || dim < d) rk[i] = *reinterpret_cast<const u32x4*>(kp + (key * d + dim));
       if (!EXACT) rv[i] = u32x4{0, 0, 0, 0};
-      if (EXACT || (tid >> 2) + 64 * i < d) rv[i] = *reinterpret_cast<const u32x4*>(vp + 64 * i * a.page);
+      if (EXACT || (tid >> 2) + 16 * NW * i < d) rv[i] = *reinterpret_cast<const u32x4*>(vp + 16 * NW * i * a.page);
     }
   };
-  auto store_codes = [&](int buf) {
+  // In steps that some row of the workgroup does not see whole, NaN values (FP8)
+  // are left out of lv, so that they reach only the rows that see their key (0 x
+  // NaN is NaN), and lnan holds a bit for each.
+  const int g_hi = keys_of(a, len, n, r_first / a.rep).hi, g_lo = keys_of(a, len, n, r_last / a.rep).lo;
+  auto group_masked = [&](int st) { return st * kStep + kStep > g_hi || st * kStep < g_lo; };
+  auto nan_in_step = [&](int buf) {
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) any |= lnan_any[buf][w];
+    return __builtin_amdgcn_readfirstlane(any) != 0;
+  };
+  auto store_codes = [&](int buf, int st) {
+    if constexpr (ST == kKvFp8) {
+      if (group_masked(st)) {
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          uint32_t bits = 0;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t nb = nan_bytes(rv[i][w]) >> 7;
+            bits |= (nb * 0x01020408u >> 24 & 0xfu) << (4 * w);   // bytes 0 .. 3 to bits 0 .. 3
+            rv[i][w] &= ~(nb * 0xffu);
+          }
+          lnan[buf][((tid >> 2) + 16 * NW * i) * 4 + (lane & 3)] = static_cast<uint16_t>(bits);
+          any |= bits;
+        }
+        const int found = __any(any != 0);
+        if (lane == 0) lnan_any[buf][wave] = found;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
-      const int e = lane + 64 * i;
-      const int key = 64 % KC == 0 ? kkey + 64 / KC * i : e / KC;
-      const int dim = 64 % KC == 0 ? kdim : 16 * (e % KC);
-      u32x4* kp = &lk[buf][(16 * wave + key) * KR + dim / 8];
+      const int e = kfirst + lane + 64 * i, key = e / KC, dim = 16 * (e % KC);
+      u32x4* kp = &lk[buf][(16 * kblock + key) * KR + dim / 8];
       kp[0] = widen8<ST>(rk[i].x, rk[i].y);
       kp[1] = widen8<ST>(rk[i].z, rk[i].w);
-      u32x4* vp = &lv[buf][((tid >> 2) + 64 * i) * VR + 2 * (lane & 3)];
+      u32x4* vp = &lv[buf][((tid >> 2) + 16 * NW * i) * VR + 2 * (lane & 3)];
       vp[0] = widen8<ST>(rv[i].x, rv[i].y);
       vp[1] = widen8<ST>(rv[i].z, rv[i].w);
     }
@@ -607,7 +644,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_long(co
     load_codes(s0, id);
     auto scale_at = [&](const float* p, int i) { return p[static_cast<int64_t>(known(i) ? i : 0) * a.hkv + h]; };
     float ks = known(id) ? scale_at(a.ks, id) : __builtin_nanf(""), vs = scale_at(a.vs, id);
-    store_codes(0);
+    store_codes(0, s0);
     load_codes(s0 + 1, id_next);
     id = id_next;
     id_next = id_of(s0 + 2);
@@ -632,6 +669,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_long(co
       if (w_any && tb < wl.hi && tb + kStep > wf.lo) {
         const bool masked = tb + kStep > wf.hi || tb < wl.lo;
         f16x sc[2];
+        __builtin_amdgcn_s_setprio(1);   // a wave at its products goes before one at its weights
 #pragma unroll
         for (int k = 0; k < NS; ++k)
 #pragma unroll
@@ -639,11 +677,12 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_long(co
             const u32x4 kk = lk[buf][(32 * kt + krow) * KR + 2 * k + hf];
             sc[kt] = mfma32x32x16<kF16>(kk, qf[k], k == 0 ? f16x{} : sc[kt]);
           }
+        __builtin_amdgcn_s_setprio(0);
         __builtin_amdgcn_sched_barrier(0);
-        auto hidden = [&](int q, int i) {
-          const int j = tb + 16 * q + 8 * hf + i;
-          return j < mine.lo || j >= mine.hi;
-        };
+        // key tb + 16 q + 8 hf + i is outside [lo, hi)
+        const int before = mine.lo - tb - 8 * hf;
+        const uint32_t wide = static_cast<uint32_t>(mine.hi - mine.lo);
+        auto hidden = [&](int q, int i, int from) { return static_cast<uint32_t>(16 * q + i - from) >= wide; };
         // Weights against the maximum so far: as long as none is past fp16's
         // range it stays (their sum tells); else, and at first, it is raised to
         // the step's own and the weights are made again.
@@ -651,6 +690,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_long(co
         float part[4];
         auto weigh = [&](auto mask) {
           const float ref = m == kNegInf ? 0.0f : m;
+          const int hide = mask.value ? opaque(before) : 0;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const float f = cq * ksq[q], off = lvs[q] - ref;
@@ -662,7 +702,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_long(co
               for (int e = 0; e < 2; ++e) {
                 const float x = sc[q >> 1][8 * (q & 1) + 2 * i + e];
                 w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, f, off));
-                if (mask.value && hidden(q, 2 * i + e)) w[e] = 0.0f;   // whatever its scale is
+                if (mask.value && hidden(q, 2 * i + e, hide)) w[e] = 0.0f;   // whatever its scale is
               }
               p[q][i] = pack2_out<kF16>(w[0], w[1]);
               part[q] += w[0] + w[1];   // before their rounding: the sum also counts what is far below
@@ -670,10 +710,14 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_long(co
             }
           }
         };
-        auto raise = [&](auto mask, bool mine_needs) {
+        if (masked) weigh(std::true_type{});
+        else weigh(std::false_type{});
+        const bool needs_here = !((part[0] + part[1]) + (part[2] + part[3]) <= kMostWeight) || m == kNegInf;
+        if (__any(needs_here)) {
           // a row whose two lanes need no raising stays as it is, whatever the
           // wave's other rows do
-          const bool needs = max_halves(mine_needs ? 1.0f : 0.0f) != 0.0f;
+          const bool needs = max_halves(needs_here ? 1.0f : 0.0f) != 0.0f;
+          const int hide = opaque(before);
           float mx = kNegInf;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
@@ -681,7 +725,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_long(co
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const float y = __builtin_fmaf(sc[q >> 1][8 * (q & 1) + i], f, lvs[q]);
-              mx = fmaxf(mx, mask.value && hidden(q, i) ? kNegInf : y);
+              mx = fmaxf(mx, hidden(q, i, hide) ? kNegInf : y);
             }
           }
           const float top = fmaxf(max_halves(mx), m);
@@ -691,63 +735,46 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_long(co
           l *= f;
 #pragma unroll
           for (int t = 0; t < ND; ++t) o[t] *= f;
-        };
-        auto soften = [&](auto mask) {
-          weigh(mask);
-          const float sum = (part[0] + part[1]) + (part[2] + part[3]);
-          const bool needs = !(sum <= kMostWeight) || m == kNegInf;
-          if (__any(needs)) {
-            raise(mask, needs);
-            weigh(mask);
-          }
-        };
-        if (masked) soften(std::true_type{});
-        else soften(std::false_type{});
+          weigh(std::true_type{});
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) l += part[q] == 0.0f ? 0.0f : part[q] * ivs[q];
         __builtin_amdgcn_sched_barrier(0);
 
-        bool checked = false;
-        if constexpr (ST == kKvFp8) {
-          if (masked) {
-            // NaN values must reach only the rows that see their key (0 x NaN is NaN)
-            checked = true;
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int t = 0; t < ND; ++t)
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                u32x4 vv = lv[buf][(32 * t + n32) * VR + 2 * q + hf];
-                u32x4 ind = {0, 0, 0, 0};      // 1 at NaN values
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  if ((vv[i] & 0x7fffu) > 0x7c00u) ind[i] |= 0x3c00u;
-                  if ((vv[i] & 0x7fff0000u) > 0x7c000000u) ind[i] |= 0x3c000000u;
-                  vv[i] &= ~((ind[i] >> 10) * 0x1111u);   // 0x3c00 >> 10 = 0xf
-                }
-                if (__any((ind.x | ind.y | ind.z | ind.w) != 0)) {
-                  u32x4 seen;
-#pragma unroll
-                  for (int i = 0; i < 4; ++i)
-                    seen[i] = (hidden(q, 2 * i) ? 0u : 0x3c00u) | (hidden(q, 2 * i + 1) ? 0u : 0x3c000000u);
-                  const f16x cnt = mfma32x32x16<kF16>(ind, seen, f16x{});
-#pragma unroll
-                  for (int i = 0; i < 16; ++i)
-                    if (cnt[i] > 0.0f) o[t][i] = __builtin_nanf("");
-                }
-                o[t] = mfma32x32x16<kF16>(vv, p[q], o[t]);
-              }
-          }
-        }
-        if (!checked) {
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
           for (int t = 0; t < ND; ++t)
+            o[t] = mfma32x32x16<kF16>(lv[buf][(32 * t + n32) * VR + 2 * q + hf], p[q], o[t]);
+        __builtin_amdgcn_s_setprio(0);
+        if constexpr (ST == kKvFp8) {
+          if (group_masked(st) && nan_in_step(buf)) {
+            // the count of NaN values that a row sees in each dimension
+            const int hide = opaque(before);
+#pragma unroll 1
+            for (int q = 0; q < 4; ++q) {
+              u32x4 seen;
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              o[t] = mfma32x32x16<kF16>(lv[buf][(32 * t + n32) * VR + 2 * q + hf], p[q], o[t]);
+              for (int i = 0; i < 4; ++i)
+                seen[i] = (hidden(q, 2 * i, hide) ? 0u : 0x3c00u) | (hidden(q, 2 * i + 1, hide) ? 0u : 0x3c000000u);
+#pragma unroll
+              for (int t = 0; t < ND; ++t) {
+                const uint32_t bits = static_cast<uint32_t>(lnan[buf][(32 * t + n32) * 4 + q]) >> (8 * hf);
+                u32x4 ind;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  ind[i] = (bits >> (2 * i) & 1u) * 0x3c00u + (bits >> (2 * i + 1) & 1u) * 0x3c000000u;
+                const f16x cnt = mfma32x32x16<kF16>(ind, seen, f16x{});
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] += cnt[i] > 0.0f ? __builtin_nanf("") : 0.0f;
+              }
+            }
+          }
         }
       }
       if (st + 1 < s1) {
-        store_codes(buf ^ 1);
+        store_codes(buf ^ 1, st + 1);
         load_codes(st + 2, id_next);
         id = id_next;
         id_next = id_of(st + 3);
@@ -809,14 +836,18 @@ __global__ __launch_bounds__(kBlock) void k_kv_attend_join(const KvAttendArg a) 
 struct KvPlan {
   int64_t row_items, long_items;
   int row_splits, long_splits;
+  int long_tile;   // rows
 };
 
 constexpr int64_t kShortRows = 64;
+
+constexpr int long_waves(int dp) { return dp == 128 ? 8 : 4; }
 
 int padded_dim(int d) { return (d + 63) / 64 * 64; }
 
 KvPlan plan_of(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t max_length) {
   KvPlan p = {};
+  p.long_tile = 32 * long_waves(padded_dim(c->head_dim));
   const int64_t rows = b->tokens * rep;
   if (b->cu == nullptr) {
     p.row_items = b->batch * cdiv(rep, kRowTile);
@@ -826,8 +857,8 @@ KvPlan plan_of(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t ma
     if (!one || rows <= kShortRows)
       p.row_items = std::min(rows / kRowTile + b->batch, b->batch * cdiv(kShortRows, kRowTile));
     if (rows > kShortRows)
-      p.long_items = one ? cdiv(rows, kLongTile)
-                         : rows / kLongTile + std::min<int64_t>(b->batch, rows / (kShortRows + 1));
+      p.long_items = one ? cdiv(rows, p.long_tile)
+                         : rows / p.long_tile + std::min<int64_t>(b->batch, rows / (kShortRows + 1));
   }
   const int64_t cap = static_cast<int64_t>(b->max_pages) * c->page_size;
   const int64_t len = max_length > 0 ? std::min(max_length, cap) : cap;
@@ -861,7 +892,7 @@ extern "C" size_t cbq_kv_attend_ws_bytes(const cbq_kv_cache* cache, const cbq_kv
   const KvPlan p = plan_of(cache, batch, q_heads / cache->kv_heads, max_length);
   size_t n = 0;
   if (p.row_splits > 1) n += p.row_splits * partial_bytes(cache, p.row_items, kRowTile);
-  if (p.long_splits > 1) n += p.long_splits * partial_bytes(cache, p.long_items, kLongTile);
+  if (p.long_splits > 1) n += p.long_splits * partial_bytes(cache, p.long_items, p.long_tile);
   return CBQ_WS_CTRL_BYTES + n;
 }
 
@@ -958,10 +989,11 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   if (p.long_items > 0) {
     a.row_min = kShortRows + 1;
     a.row_max = int64_t{1} << 62;
-    return run(p.long_items, kLongTile, p.long_splits, [&](dim3 grid, auto stc, auto dpc) {
+    return run(p.long_items, p.long_tile, p.long_splits, [&](dim3 grid, auto stc, auto dpc) {
       constexpr int ST = decltype(stc)::value, DP = decltype(dpc)::value;
-      if (a.d == DP) k_kv_attend_long<ST, DP, true><<<grid, kBlock, 0, st>>>(a);
-      else k_kv_attend_long<ST, DP, false><<<grid, kBlock, 0, st>>>(a);
+      constexpr int NW = long_waves(DP);
+      if (a.d == DP) k_kv_attend_long<ST, DP, true, NW><<<grid, 64 * NW, 0, st>>>(a);
+      else k_kv_attend_long<ST, DP, false, NW><<<grid, 64 * NW, 0, st>>>(a);
     });
   }
   return CBQ_OK;
