@@ -796,13 +796,18 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_kv_attend_long(c
     }
 }
 
-// Joins the splits' partial results: a wave per row, a workgroup per 4 rows of a
-// tile. Lane l reads split l's maximum and sum.
+// Joins the splits' partial results. A wave (WIDE: a workgroup, of whose waves
+// each takes every fourth split) per row; lane l reads split l's maximum and sum,
+// then all lanes read 4 dimensions of 8 splits at a time. (One split at a time, a
+// load behind a load, took 24 us for 64 splits.)
+template <bool WIDE>
 __global__ __launch_bounds__(kBlock) void k_kv_attend_join(const KvAttendArg a) {
+  constexpr int PER = WIDE ? 1 : 4;     // rows of a workgroup
   const int lane = threadIdx.x & 63;
-  const int quads = a.tile_rows / 4;
-  const int row = (blockIdx.x % quads) * 4 + (threadIdx.x >> 6);
-  const int64_t rest = blockIdx.x / quads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int parts = a.tile_rows / PER;
+  const int row = (blockIdx.x % parts) * PER + (WIDE ? 0 : wave);
+  const int64_t rest = blockIdx.x / parts;
   const int h = rest % a.hkv;
   const int64_t item = rest / a.hkv;
   const KvTile tl = tile_of(a, item);
@@ -817,18 +822,36 @@ __global__ __launch_bounds__(kBlock) void k_kv_attend_join(const KvAttendArg a) 
   float l = ml.y * f;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o, 64);
-  const int d0 = 4 * lane;
+  const int d0 = 4 * lane < a.d ? 4 * lane : 0;
   f4 acc = {};
-  for (int s = 0; s < a.splits; ++s) {
-    const float fs = __shfl(f, s, 64);   // with all lanes active: those past d have a split's factor
-    if (fs != 0.0f && d0 < a.d)
-      acc += *reinterpret_cast<const f4*>(a.po + (s * a.prows + prow) * a.d + d0) * fs;
+  constexpr int STEP = WIDE ? 4 : 1;
+  for (int s0 = WIDE ? wave : 0; s0 < a.splits; s0 += 8 * STEP) {
+    f4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int s = s0 + k * STEP < a.splits ? s0 + k * STEP : s0;
+      v[k] = *reinterpret_cast<const f4*>(a.po + (s * a.prows + prow) * a.d + d0);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int s = s0 + k * STEP;
+      const float fs = s < a.splits ? read_lane(f, s) : 0.0f;   // s is the same in the wave
+      if (s < a.splits) acc += v[k] * fs;
+    }
+  }
+  if constexpr (WIDE) {
+    __shared__ f4 part[3][64];
+    if (wave > 0) part[wave - 1][lane] = acc;
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 0; w < 3; ++w) acc += part[w][lane];
   }
   const int ti = (tl.r_first + row) / a.rep;
   const int64_t orow = (tl.s.tok0 + ti) * a.hq + h * a.rep + (tl.r_first + row - ti * a.rep);
   KvAttendArg one = a;
   one.splits = 1;
-  if (d0 < a.d) put_row(one, orow, 0, 0, d0, acc, m, l, false);
+  if (4 * lane < a.d) put_row(one, orow, 0, 0, d0, acc, m, l, false);
 }
 
 // What one call launches: k_kv_attend_rows for the sequences of few rows,
@@ -957,7 +980,8 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
       room -= splits * each;
     }
     const int blocks = items * a.hkv * splits;
-    const int64_t joins = items * a.hkv * (tile / 4);
+    const bool wide = splits > 8;
+    const int64_t joins = items * a.hkv * (wide ? tile : tile / 4);
     CBQ_REQUIRE(blocks < (int64_t{1} << 31) && joins < (int64_t{1} << 31),
                 "kv attend: too many tokens for one call");
     const dim3 grid(static_cast<uint32_t>(blocks));
@@ -973,7 +997,8 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
     else by_dim(std::integral_constant<int, kKvFp8>{});
     if (int rc = launch_status("cbq_kv_attend")) return rc;
     if (splits == 1) return CBQ_OK;
-    k_kv_attend_join<<<dim3(static_cast<uint32_t>(joins)), kBlock, 0, st>>>(a);
+    if (wide) k_kv_attend_join<true><<<dim3(static_cast<uint32_t>(joins)), kBlock, 0, st>>>(a);
+    else k_kv_attend_join<false><<<dim3(static_cast<uint32_t>(joins)), kBlock, 0, st>>>(a);
     return launch_status("cbq_kv_attend");
   };
   if (p.row_items > 0) {
