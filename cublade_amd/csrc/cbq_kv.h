@@ -47,31 +47,31 @@ __device__ __forceinline__ KvSeq kv_seq(const KvBatch& m, int b) {
   return s;
 }
 
-// Finds the sequence that owns work item `idx` when sequence b has count(b,
-// seq) items and items are numbered sequence after sequence: returns b and
-// sets rel to the item's number within it, or returns -1 past the last. All 64
-// lanes of a wave call it with the same idx: 64 sequences at a time, a scan
-// over the lanes.
+// Finds the sequence that owns work item `idx` when sequence b has count(seq)
+// items and items are numbered sequence after sequence: returns b and sets rel to
+// the item's number within it, or returns -1 past the last. Counts and their sum
+// are below 2^31. All 64 lanes of a wave call it with the same idx: 64 sequences
+// at a time, a scan over the lanes.
 template <typename Count>
-__device__ __forceinline__ int kv_find(const KvBatch& m, int64_t idx, int64_t& rel, Count count) {
+__device__ __forceinline__ int kv_find(const KvBatch& m, int idx, int& rel, Count count) {
   const int lane = threadIdx.x & 63;
-  int64_t run = 0;
+  int run = 0;
   for (int b0 = 0; b0 < m.batch; b0 += 64) {
-    int64_t c = 0;
+    int c = 0;
     if (b0 + lane < m.batch) c = count(kv_seq(m, b0 + lane));
-    int64_t incl = c;
+    int incl = c;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const int64_t up = __shfl_up(incl, o, 64);
+      const int up = __shfl_up(incl, o, 64);
       if (lane >= o) incl += up;
     }
     const uint64_t past = __ballot(run + incl > idx);
     if (past != 0) {
-      const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
-      rel = idx - run - __shfl(incl - c, l, 64);
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(past)) - 1);
+      rel = idx - run - __builtin_amdgcn_readlane(incl - c, l);
       return b0 + l;
     }
-    run += __shfl(incl, 63, 64);
+    run += __builtin_amdgcn_readlane(incl, 63);
   }
   return -1;
 }

@@ -293,10 +293,10 @@ __device__ void append_page(const KvAppendArg& a, int b, int64_t pnum, int h, fl
 // Number of pages of a sequence that get new tokens.
 struct TouchedPages {
   int shift;
-  __device__ int64_t operator()(const KvSeq& s) const {
+  __device__ int operator()(const KvSeq& s) const {
     const int64_t first = s.len - s.n > 0 ? s.len - s.n : 0;
     if (s.n == 0 || s.len <= first) return 0;
-    return ((s.len - 1) >> shift) - (first >> shift) + 1;
+    return static_cast<int>(((s.len - 1) >> shift) - (first >> shift)) + 1;
   }
 };
 
@@ -304,12 +304,12 @@ template <int ST, int DT>
 __global__ __launch_bounds__(kBlock) void k_kv_append(const KvAppendArg a) {
   __shared__ float red[kBlock / kWave];
   if (blockIdx.x < a.kv_blocks) {
-    const int64_t item = blockIdx.x / (2 * a.hkv);
+    const int item = blockIdx.x / (2 * a.hkv);
     const int hv = blockIdx.x % (2 * a.hkv);
-    int64_t rel = 0;
+    int rel = 0;
     int b;
     if (a.m.cu == nullptr) {
-      b = static_cast<int>(item);
+      b = item;
       if (a.m.lengths[b] <= 0) return;
     } else {
       b = kv_find(a.m, item, rel, TouchedPages{a.m.page_shift});
@@ -329,9 +329,9 @@ __global__ __launch_bounds__(kBlock) void k_kv_append(const KvAppendArg a) {
     at = static_cast<int64_t>(a.m.lengths[tok]) - 1;
   } else {
     // The token's sequence: as in kv_find, by the tokens each one brings.
-    int64_t rel = 0;
-    const int b = kv_find(a.m, tok - (a.m.cu[0] > 0 ? a.m.cu[0] : 0), rel,
-                          [](const KvSeq& s) { return s.n; });
+    int rel = 0;
+    const int b = kv_find(a.m, static_cast<int>(tok) - (a.m.cu[0] > 0 ? a.m.cu[0] : 0), rel,
+                          [](const KvSeq& s) { return static_cast<int>(s.n); });
     if (b >= 0) {
       const KvSeq s = kv_seq(a.m, b);
       at = s.len - s.n + rel;

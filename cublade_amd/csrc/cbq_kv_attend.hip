@@ -63,8 +63,8 @@ struct KvAttendArg {
   int causal, bf16, negate, splits;
   int window;              // 0: none
   int tile_rows;           // query rows of a workgroup
-  int64_t items;           // row tiles of this launch, at most
-  int64_t row_min, row_max;   // this launch's sequences have row_min .. row_max rows
+  int items;               // row tiles of this launch, at most
+  int row_min, row_max;       // this launch's sequences have row_min .. row_max rows
 };
 
 // 8 codes -> 8 exact fp16.
@@ -219,9 +219,9 @@ __device__ __forceinline__ void load_q(const KvAttendArg& a, const char* qp, boo
 // A sequence's query rows (row = new token * rep + head in its group) in tiles.
 struct RowTiles {
   int rep, tile_rows;
-  int64_t lo, hi;
-  __device__ int64_t operator()(const KvSeq& s) const {
-    const int r = s.n * rep;
+  int lo, hi;
+  __device__ int operator()(const KvSeq& s) const {
+    const int r = static_cast<int>(s.n) * rep;
     return r >= lo && r <= hi ? (r + tile_rows - 1) / tile_rows : 0;
   }
 };
@@ -234,43 +234,45 @@ struct KvTile {
   int rows, r_first;
 };
 
-__device__ __forceinline__ KvTile tile_of(const KvAttendArg& a, int64_t item) {
+__device__ __forceinline__ KvTile tile_of(const KvAttendArg& a, int item) {
   KvTile t;
-  int64_t tile;
+  int tile;
   if (a.m.cu == nullptr) {
     const int per = (a.rep + a.tile_rows - 1) / a.tile_rows;
-    t.b = static_cast<int>(item / per);
+    t.b = item / per;
     tile = item % per;
   } else {
-    t.b = __builtin_amdgcn_readfirstlane(
-        kv_find(a.m, item, tile, RowTiles{a.rep, a.tile_rows, a.row_min, a.row_max}));
+    t.b = kv_find(a.m, item, tile, RowTiles{a.rep, a.tile_rows, a.row_min, a.row_max});
     if (t.b < 0) return t;
-    tile = __builtin_amdgcn_readfirstlane(static_cast<int>(tile));   // the same in all lanes
   }
   t.s = kv_seq(a.m, t.b);
   t.rows = static_cast<int>(t.s.n) * a.rep;
-  t.r_first = static_cast<int>(tile) * a.tile_rows;
+  t.r_first = tile * a.tile_rows;
   return t;
 }
 
 // One workgroup: 16 query rows of one kv head (row = new token * rep + head in
 // the group) and one range of the keys. Its 4 waves take steps of 64 keys in
 // turn, each with its own maximum, sum and accumulators, joined at the end.
-// DP: head_dim padded to a multiple of 64; EXACT: head_dim is DP.
-template <int ST, int DP, bool EXACT>
+// DP: head_dim padded to a multiple of 64; EXACT: head_dim is DP; NT: no other
+// workgroup reads the codes, and they are loaded past the caches (5.8 instead of
+// 5.2 TB/s for 128 sequences of 1000 tokens; slower where several tiles of rows
+// read the same codes).
+template <int ST, int DP, bool EXACT, bool NT>
 __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(const KvAttendArg a) {
   constexpr int NC = DP / 64;      // 16-byte chunks of a key per lane
   constexpr int ND = DP / 16;      // tiles of 16 dimensions
   const int d = EXACT ? DP : a.d;
   __shared__ __attribute__((aligned(16))) float so[4][kRowTile][DP + 4];
   __shared__ float sml[4][kRowTile][2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, g = lane >> 4;
 
   const int split = blockIdx.x % a.splits;
-  const int64_t rest = blockIdx.x / a.splits;
+  const int rest = blockIdx.x / a.splits;
   const int h = rest % a.hkv;
-  const int64_t item = rest / a.hkv;
+  const int item = rest / a.hkv;
   const KvTile tl = tile_of(a, item);
   if (tl.b < 0) return;
   const int b = tl.b;
@@ -312,6 +314,10 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
     };
     auto page_of = [&](int bl) { return a.m.table[b * a.m.tstride + ((bl << 4) >> a.m.page_shift)]; };
     auto valid = [&](int id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.m.num_pages); };
+    auto load16 = [](const uint8_t* p) {
+      if constexpr (NT) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+      else return *reinterpret_cast<const u32x4*>(p);
+    };
     u32x4 kr[4][NC];
     float ksc = 0.0f, vsc = 1.0f;
     int id_v = 0;
@@ -325,7 +331,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           kr[t][c] = u32x4{0, 0, 0, 0};
-          if (64 * c + 16 * g < d) kr[t][c] = *reinterpret_cast<const u32x4*>(p + 4 * t * d + 64 * c);
+          if (64 * c + 16 * g < d) kr[t][c] = load16(p + 4 * t * d + 64 * c);
         }
       const int64_t sat = static_cast<int64_t>(valid(idv) ? idv : 0) * a.hkv + h;
       ksc = valid(idv) ? a.ks[sat] : __builtin_nanf("");
@@ -350,7 +356,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
 #pragma unroll
         for (int t = 0; t < ND; ++t) {
           vr[t] = u32x4{0, 0, 0, 0};
-          if (16 * t < d) vr[t] = *reinterpret_cast<const u32x4*>(p + 16 * t * a.page);
+          if (16 * t < d) vr[t] = load16(p + 16 * t * a.page);
         }
       }
       // scores of 64 keys: lane (n16, g) gets keys tb + 16 g + 4 t + i of row n16
@@ -492,7 +498,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
     f4 v = {};
 #pragma unroll
     for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f4*>(&so[w][row][d0]) * f[w];
-    put_row(a, orow, (item * a.hkv + h) * kRowTile + row, split, d0, v, mm, ll, bad);
+    put_row(a, orow, static_cast<int64_t>(item * a.hkv + h) * kRowTile + row, split, d0, v, mm, ll, bad);
   }
 }
 
@@ -529,9 +535,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_kv_attend_long(c
   const int n32 = lane & 31, hf = lane >> 5;
 
   const int h = blockIdx.x % a.hkv;
-  const int64_t rest = blockIdx.x / a.hkv;
+  const int rest = blockIdx.x / a.hkv;
   const int split = rest % a.splits;
-  const int64_t item = a.items - 1 - rest / a.splits;   // a causal prompt's longest rows first
+  const int item = a.items - 1 - rest / a.splits;   // a causal prompt's longest rows first
   const KvTile tl = tile_of(a, item);
   if (tl.b < 0) return;
   const KvSeq s = tl.s;
@@ -791,7 +797,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_kv_attend_long(c
     for (int q = 0; q < 4; ++q) {
       const int d0 = 32 * t + 8 * q + 4 * hf;
       if (EXACT || d0 < d)
-        put_row(a, orow, (item * a.hkv + h) * kLongTile + wave * 32 + n32, split, d0,
+        put_row(a, orow, static_cast<int64_t>(item * a.hkv + h) * kLongTile + wave * 32 + n32, split, d0,
                 f4{o[t][4 * q], o[t][4 * q + 1], o[t][4 * q + 2], o[t][4 * q + 3]}, m, sum, bad);
     }
 }
@@ -807,12 +813,12 @@ __global__ __launch_bounds__(kBlock) void k_kv_attend_join(const KvAttendArg a) 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int parts = a.tile_rows / PER;
   const int row = (blockIdx.x % parts) * PER + (WIDE ? 0 : wave);
-  const int64_t rest = blockIdx.x / parts;
+  const int rest = blockIdx.x / parts;
   const int h = rest % a.hkv;
-  const int64_t item = rest / a.hkv;
+  const int item = rest / a.hkv;
   const KvTile tl = tile_of(a, item);
   if (tl.b < 0 || tl.r_first + row >= tl.rows) return;
-  const int64_t prow = (item * a.hkv + h) * a.tile_rows + row;
+  const int64_t prow = static_cast<int64_t>(item * a.hkv + h) * a.tile_rows + row;
   float2 ml = make_float2(kNegInf, 0.0f);
   if (lane < a.splits) ml = a.pml[lane * a.prows + prow];
   float m = ml.x;
@@ -858,11 +864,20 @@ __global__ __launch_bounds__(kBlock) void k_kv_attend_join(const KvAttendArg a) 
 // k_kv_attend_long for the others (items 0: not launched).
 struct KvPlan {
   int64_t row_items, long_items;
+  int64_t row_max;         // rows of a sequence that k_kv_attend_rows takes, at most
   int row_splits, long_splits;
   int long_tile;   // rows
 };
 
+// Sequences of at most this many rows go to k_kv_attend_rows, and all of them
+// where a sequence has at most kFewRows on average: a second launch then costs
+// more than it could save.
 constexpr int64_t kShortRows = 64;
+constexpr int64_t kFewRows = 32;
+// Workgroups per CU that the keys of few tiles are split for. 2 fit at once
+// (head size 128); with 4 a batch of mixed lengths takes 113 instead of 126 us (64
+// sequences of 100 to 8000 tokens), one sequence the same.
+constexpr int64_t kRowWgs = 4;
 
 constexpr int long_waves(int dp) { return dp == 128 ? 8 : 4; }
 
@@ -877,18 +892,19 @@ KvPlan plan_of(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t ma
   } else {
     // n rows make at most n / t + 1 tiles of t
     const bool one = b->batch == 1;
-    if (!one || rows <= kShortRows)
-      p.row_items = std::min(rows / kRowTile + b->batch, b->batch * cdiv(kShortRows, kRowTile));
-    if (rows > kShortRows)
+    p.row_max = rows <= kFewRows * b->batch ? rows : kShortRows;
+    if (!one || rows <= p.row_max)
+      p.row_items = std::min(rows / kRowTile + b->batch, b->batch * cdiv(p.row_max, kRowTile));
+    if (rows > p.row_max)
       p.long_items = one ? cdiv(rows, p.long_tile)
-                         : rows / p.long_tile + std::min<int64_t>(b->batch, rows / (kShortRows + 1));
+                         : rows / p.long_tile + std::min<int64_t>(b->batch, rows / (p.row_max + 1));
   }
   const int64_t cap = static_cast<int64_t>(b->max_pages) * c->page_size;
   const int64_t len = max_length > 0 ? std::min(max_length, cap) : cap;
   const int64_t cus = device_cus();
   p.row_splits = p.long_splits = 1;
   if (p.row_items > 0) {
-    const int64_t want = cdiv(2 * cus, p.row_items * c->kv_heads);
+    const int64_t want = cdiv(kRowWgs * cus, p.row_items * c->kv_heads);
     p.row_splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, cdiv(cdiv(len, kStep), 4), kMaxSplits})));
   }
   if (p.long_items > 0) {
@@ -969,7 +985,7 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   auto run = [&](int64_t items, int tile, int splits, auto kernel) -> int {
     const size_t each = partial_bytes(cache, items, tile);
     splits = std::max(1, static_cast<int>(std::min<size_t>(splits, room / each)));
-    a.items = items;
+    a.items = static_cast<int>(items);
     a.tile_rows = tile;
     a.splits = splits;
     a.prows = items * a.hkv * tile;
@@ -1003,17 +1019,22 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   };
   if (p.row_items > 0) {
     a.row_min = 1;
-    a.row_max = kShortRows;
+    a.row_max = batch->cu == nullptr ? rep : static_cast<int>(p.row_max);
+    const bool alone = batch->cu == nullptr && rep <= kRowTile;
     const int rc = run(p.row_items, kRowTile, p.row_splits, [&](dim3 grid, auto stc, auto dpc) {
       constexpr int ST = decltype(stc)::value, DP = decltype(dpc)::value;
-      if (a.d == DP) k_kv_attend_rows<ST, DP, true><<<grid, kBlock, 0, st>>>(a);
-      else k_kv_attend_rows<ST, DP, false><<<grid, kBlock, 0, st>>>(a);
+      auto go = [&](auto nt) {
+        if (a.d == DP) k_kv_attend_rows<ST, DP, true, nt.value><<<grid, kBlock, 0, st>>>(a);
+        else k_kv_attend_rows<ST, DP, false, nt.value><<<grid, kBlock, 0, st>>>(a);
+      };
+      if (alone) go(std::true_type{});
+      else go(std::false_type{});
     });
     if (rc) return rc;
   }
   if (p.long_items > 0) {
-    a.row_min = kShortRows + 1;
-    a.row_max = int64_t{1} << 62;
+    a.row_min = static_cast<int>(p.row_max) + 1;
+    a.row_max = INT32_MAX;
     return run(p.long_items, p.long_tile, p.long_splits, [&](dim3 grid, auto stc, auto dpc) {
       constexpr int ST = decltype(stc)::value, DP = decltype(dpc)::value;
       constexpr int NW = long_waves(DP);
