@@ -505,7 +505,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
 // ---------------------------------------------------------------------------
 // Many query rows: prompts and chunks of them.
 // ---------------------------------------------------------------------------
-// A workgroup takes 128 rows of one kv head, a wave 32 of them; the workgroup
+// A workgroup takes 128 or 256 rows of one kv head, a wave 32 of them; it
 // goes through the keys 64 at a time. Codes are widened to fp16 once per workgroup, on their way from registers to LDS (K
 // rows [64 keys][DP], V^T rows [DP][64 keys]; every row has 16 bytes more than it
 // needs, so an odd number of 16-byte chunks: equal chunks of 16 consecutive rows
@@ -879,14 +879,24 @@ constexpr int64_t kFewRows = 32;
 // sequences of 100 to 8000 tokens), one sequence the same.
 constexpr int64_t kRowWgs = 4;
 
-constexpr int long_waves(int dp) { return dp == 128 ? 8 : 4; }
-
 int padded_dim(int d) { return (d + 63) / 64 * 64; }
+
+// Waves of a k_kv_attend_long workgroup for `rows` rows of each kv head. 8 share a
+// step's codes (one workgroup per CU; a prompt of 8192 tokens 588 us, with 4 and two
+// workgroups 627), 4 leave less of the GPU idle in the last round of few
+// workgroups (a batch with 5 prompts of up to 1500 tokens: 105 and 110 us). Other
+// head sizes have registers or loads for 4 only.
+int long_waves(int dp, int64_t rows, int kv_heads, bool one_sequence) {
+  if (dp != 128) return 4;
+  const int64_t cus = device_cus(), wgs = cdiv(rows, 256) * kv_heads;
+  const bool fills = one_sequence && 10 * wgs >= 9 * cus * cdiv(wgs, cus);
+  return fills || wgs >= 3 * cus ? 8 : 4;
+}
 
 KvPlan plan_of(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t max_length) {
   KvPlan p = {};
-  p.long_tile = 32 * long_waves(padded_dim(c->head_dim));
   const int64_t rows = b->tokens * rep;
+  p.long_tile = 32 * long_waves(padded_dim(c->head_dim), rows, c->kv_heads, b->batch == 1);
   if (b->cu == nullptr) {
     p.row_items = b->batch * cdiv(rep, kRowTile);
   } else {
@@ -908,7 +918,7 @@ KvPlan plan_of(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t ma
     p.row_splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, cdiv(cdiv(len, kStep), 4), kMaxSplits})));
   }
   if (p.long_items > 0) {
-    const int64_t want = cus / (p.long_items * c->kv_heads);
+    const int64_t want = (p.long_tile == 256 ? 1 : 2) * cus / (p.long_items * c->kv_heads);
     p.long_splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, cdiv(len, 8 * kStep), kMaxSplits})));
   }
   return p;
@@ -1037,9 +1047,15 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
     a.row_max = INT32_MAX;
     return run(p.long_items, p.long_tile, p.long_splits, [&](dim3 grid, auto stc, auto dpc) {
       constexpr int ST = decltype(stc)::value, DP = decltype(dpc)::value;
-      constexpr int NW = long_waves(DP);
-      if (a.d == DP) k_kv_attend_long<ST, DP, true, NW><<<grid, 64 * NW, 0, st>>>(a);
-      else k_kv_attend_long<ST, DP, false, NW><<<grid, 64 * NW, 0, st>>>(a);
+      auto go = [&](auto nwc) {
+        constexpr int NW = decltype(nwc)::value;
+        if (a.d == DP) k_kv_attend_long<ST, DP, true, NW><<<grid, 64 * NW, 0, st>>>(a);
+        else k_kv_attend_long<ST, DP, false, NW><<<grid, 64 * NW, 0, st>>>(a);
+      };
+      if constexpr (DP == 128) {
+        if (p.long_tile == 256) return go(std::integral_constant<int, 8>{});
+      }
+      go(std::integral_constant<int, 4>{});
     });
   }
   return CBQ_OK;
