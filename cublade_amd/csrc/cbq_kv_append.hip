@@ -3,8 +3,9 @@
 // k_kv_append: one workgroup for each (sequence, page that gets new tokens, kv
 // head, keys or values), which takes the page's new tokens' maximum, settles
 // the page's scale, lowers earlier codes if the scale grew, and writes the new
-// codes; and one workgroup for each new token's queries. A page belongs to one
+// codes; and one wave for each new token's queries. A page's head belongs to one
 // workgroup, so nothing is atomic and results do not depend on order.
+// k_kv_append_step does the same for one new token per sequence.
 //
 // A thread's unit is 4 tokens x 8 dimensions. Keys: neighbouring lanes take
 // neighbouring dimensions (rows of x are read whole, codes written 8 bytes per
@@ -12,6 +13,9 @@
 // groups of 4 tokens, so that a word of 4 tokens' codes of one dimension is
 // made in one thread's registers and stored as it is, without LDS; the 4 lanes
 // that share a token still read 64 consecutive bytes of it.
+#include <algorithm>
+#include <type_traits>
+
 #include "cbq_kv.h"
 
 namespace cbq {
@@ -41,7 +45,9 @@ struct KvAppendArg {
   float* ks;
   float* vs;
   char* q_out;
-  int64_t kv_blocks;   // workgroups for pages; the rest are for queries
+  int64_t kv_blocks;   // k_kv_append: workgroups for pages; the rest are for queries
+  int step_waves;      // k_kv_append_step: waves for keys and values; the rest are for queries
+  int q_waves;         // waves of a token's queries
   int hkv, hq, d, page;
 };
 
@@ -149,6 +155,66 @@ __device__ __forceinline__ uint32_t lower4(uint32_t w, float f, uint32_t keep) {
   return (w & keep) | (n & ~keep);
 }
 
+// A page's scale for new tokens of maximum amax: the scale, what new values are
+// multiplied by, and what earlier codes are.
+struct PageScale {
+  float scale, inv, lower;
+};
+
+template <int ST>
+__device__ __forceinline__ PageScale settle(float amax, float s_old, bool begun) {
+  PageScale p;
+  if (!begun || s_old == 0.0f) {
+    p.inv = inv_scale(amax, kKvEps, kv_qmax<ST>());
+    p.scale = 1.0f / p.inv;
+    p.lower = 0.0f;         // earlier codes, if any, stand for zeros
+    return p;
+  }
+  p.scale = s_old;
+  p.lower = 1.0f;
+  const float t = amax / (kv_qmax<ST>() * s_old);
+  if (t > 1.0f) {
+    int e = 0;
+    const float mant = __builtin_frexpf(t, &e);
+    const int g = mant > 0.5f ? e : e - 1;
+    const bool fin = t < __builtin_inff();
+    p.scale = fin ? __builtin_ldexpf(s_old, g) : __builtin_inff();
+    p.lower = fin ? __builtin_ldexpf(1.0f, -g) : 0.0f;
+  }
+  p.inv = 1.0f / p.scale;
+  return p;
+}
+
+// The first `lo` tokens' codes of a page's head times `lower`, by `n` threads of
+// which this is number `i`; 16 codes at a time: of one token (keys) or 16 tokens of
+// one dimension (values, of which only the first `lo` change).
+template <int ST, bool VALUES>
+__device__ void lower_codes(uint8_t* codes, int lo, int page, int d, float lower, int i, int n) {
+  if constexpr (VALUES) {
+    const int per = page >> 4, used = (lo + 15) >> 4;
+    for (int c = i; c < used * d; c += n) {
+      const int t0 = (c % used) << 4;
+      uint4* p = reinterpret_cast<uint4*>(codes) + (c / used) * per + (t0 >> 4);
+      uint4 w = *p;
+      uint32_t* q = &w.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int left = lo - t0 - 4 * j;   // tokens of this word to change
+        if (left > 0) q[j] = lower4<ST>(q[j], lower, left >= 4 ? 0u : 0xffffffffu << (8 * left));
+      }
+      *p = w;
+    }
+  } else {
+    for (int c = i; c < lo * d / 16; c += n) {
+      uint4* p = reinterpret_cast<uint4*>(codes) + c;
+      uint4 w = *p;
+      w.x = lower4<ST>(w.x, lower, 0u); w.y = lower4<ST>(w.y, lower, 0u);
+      w.z = lower4<ST>(w.z, lower, 0u); w.w = lower4<ST>(w.w, lower, 0u);
+      *p = w;
+    }
+  }
+}
+
 // One page, head and side (keys or values).
 template <int ST, int DT, bool VALUES>
 __device__ void append_page(const KvAppendArg& a, int b, int64_t pnum, int h, float* red) {
@@ -209,51 +275,11 @@ __device__ void append_page(const KvAppendArg& a, int b, int64_t pnum, int h, fl
   const float s_old = *scale;
   amax = block_max(amax, red);
 
-  float inv, sc, lower = 1.0f;
-  if (lo == 0 || s_old == 0.0f) {
-    inv = inv_scale(amax, kKvEps, kv_qmax<ST>());
-    sc = 1.0f / inv;
-    lower = 0.0f;         // earlier codes, if any, stand for zeros
-  } else {
-    sc = s_old;
-    const float t = amax / (kv_qmax<ST>() * s_old);
-    if (t > 1.0f) {
-      int e = 0;
-      const float mant = __builtin_frexpf(t, &e);
-      const int g = mant > 0.5f ? e : e - 1;
-      const bool fin = t < __builtin_inff();
-      sc = fin ? __builtin_ldexpf(s_old, g) : __builtin_inff();
-      lower = fin ? __builtin_ldexpf(1.0f, -g) : 0.0f;
-    }
-    inv = 1.0f / sc;
-  }
+  const PageScale ps = settle<ST>(amax, s_old, lo > 0);
+  const float inv = ps.inv, lower = ps.lower;
 
   if (lo > 0 && lower != 1.0f) {
-    // Earlier codes, 16 at a time: a chunk of one token (keys) or of 16 tokens
-    // of one dimension (values, of which only the first `lo` change).
-    if constexpr (VALUES) {
-      const int per = page >> 4, used = (lo + 15) >> 4;
-      for (int c = threadIdx.x; c < used * d; c += blockDim.x) {
-        const int t0 = (c % used) << 4;
-        uint4* p = reinterpret_cast<uint4*>(codes) + static_cast<int64_t>(c / used) * per + (t0 >> 4);
-        uint4 w = *p;
-        uint32_t* q = &w.x;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int left = lo - t0 - 4 * j;   // tokens of this word to change
-          if (left > 0) q[j] = lower4<ST>(q[j], lower, left >= 4 ? 0u : 0xffffffffu << (8 * left));
-        }
-        *p = w;
-      }
-    } else {
-      for (int c = threadIdx.x; c < lo * d / 16; c += blockDim.x) {
-        uint4* p = reinterpret_cast<uint4*>(codes) + c;
-        uint4 w = *p;
-        w.x = lower4<ST>(w.x, lower, 0u); w.y = lower4<ST>(w.y, lower, 0u);
-        w.z = lower4<ST>(w.z, lower, 0u); w.w = lower4<ST>(w.w, lower, 0u);
-        *p = w;
-      }
-    }
+    lower_codes<ST, VALUES>(codes, lo, page, d, lower, threadIdx.x, blockDim.x);
     __syncthreads();   // a chunk of values may hold new tokens' places
   }
 
@@ -287,7 +313,68 @@ __device__ void append_page(const KvAppendArg& a, int b, int64_t pnum, int h, fl
           *reinterpret_cast<uint2*>(codes + (t0 + j) * d + d0) = encode8<ST>(f[j], inv);
     }
   }
-  if (threadIdx.x == 0) *scale = sc;
+  if (threadIdx.x == 0) *scale = ps.scale;
+}
+
+// The rotated queries of a token, by the wave `wave` of a.q_waves per token. A lane
+// keeps one unit, 8 pairs of dimensions (or 8 dimensions: interleaved pairs, those
+// that are not rotated, and all where the pieces do not fit) of every (64 / units)th
+// head, so the rotation's factors are read once for all of them.
+template <int DT>
+__device__ __forceinline__ void turn_queries(const KvAppendArg& a, int wave) {
+  const int tok = wave / a.q_waves, turn = wave % a.q_waves;
+  if (tok >= a.m.tokens || a.hq == 0) return;
+  int64_t at = -1;
+  if (a.m.cu == nullptr) {
+    at = static_cast<int64_t>(a.m.lengths[tok]) - 1;
+  } else {
+    // The token's sequence, by the tokens that each one brings.
+    int rel = 0;
+    const int b = kv_find(a.m, tok - (a.m.cu[0] > 0 ? a.m.cu[0] : 0), rel,
+                          [](const KvSeq& s) { return static_cast<int>(s.n); });
+    if (b >= 0) {
+      const KvSeq s = kv_seq(a.m, b);
+      at = s.len - s.n + rel;
+    }
+  }
+  const int64_t pos = rope_row(a.rope, tok, at);
+  const int lane = threadIdx.x & 63;
+  const bool pairs = a.rope.vec && !a.rope.interleaved && pos >= 0;
+  const int npairs = pairs ? a.rope.rot >> 4 : 0;
+  const int units = npairs + ((a.d - 16 * npairs) >> 3), heads = 64 / units;
+  const int unit = lane % units;
+  const char* x = a.q.p + tok * a.q.ts;
+  char* out = a.q_out + static_cast<int64_t>(tok) * a.hq * a.d * 2;
+  if (lane >= heads * units) return;
+  if (unit < npairs) {
+    const int half = a.rope.rot >> 1, d0 = 8 * unit;
+    float c[8], sn[8];
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+      *reinterpret_cast<float4*>(c + k) = *reinterpret_cast<const float4*>(a.rope.cos + pos * half + d0 + k);
+      *reinterpret_cast<float4*>(sn + k) = *reinterpret_cast<const float4*>(a.rope.sin + pos * half + d0 + k);
+    }
+    for (int h = turn * heads + lane / units; h < a.hq; h += heads * a.q_waves) {
+      float f[8], g[8], o1[8], o2[8];
+      load8<DT>(x + h * a.q.hs, d0, f);
+      load8<DT>(x + h * a.q.hs, d0 + half, g);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        o1[k] = f[k] * c[k] - g[k] * sn[k];
+        o2[k] = g[k] * c[k] + f[k] * sn[k];
+      }
+      char* p = out + (h * a.d + d0) * 2;
+      *reinterpret_cast<uint4*>(p) = pack8_out<DT>(o1);
+      *reinterpret_cast<uint4*>(p + half * 2) = pack8_out<DT>(o2);
+    }
+  } else {
+    const int d0 = 8 * (unit + npairs);
+    for (int h = turn * heads + lane / units; h < a.hq; h += heads * a.q_waves) {
+      float f[8];
+      turned8<DT>(x + h * a.q.hs, d0, pos, a.rope, f);
+      *reinterpret_cast<uint4*>(out + (h * a.d + d0) * 2) = pack8_out<DT>(f);
+    }
+  }
 }
 
 // Number of pages of a sequence that get new tokens.
@@ -307,14 +394,8 @@ __global__ __launch_bounds__(kBlock) void k_kv_append(const KvAppendArg a) {
     const int item = blockIdx.x / (2 * a.hkv);
     const int hv = blockIdx.x % (2 * a.hkv);
     int rel = 0;
-    int b;
-    if (a.m.cu == nullptr) {
-      b = item;
-      if (a.m.lengths[b] <= 0) return;
-    } else {
-      b = kv_find(a.m, item, rel, TouchedPages{a.m.page_shift});
-      if (b < 0) return;
-    }
+    const int b = kv_find(a.m, item, rel, TouchedPages{a.m.page_shift});
+    if (b < 0) return;
     const KvSeq s = kv_seq(a.m, b);
     const int64_t first = s.len - s.n > 0 ? s.len - s.n : 0;
     const int64_t pnum = (first >> a.m.page_shift) + rel;
@@ -322,29 +403,71 @@ __global__ __launch_bounds__(kBlock) void k_kv_append(const KvAppendArg a) {
     else append_page<ST, DT, false>(a, b, pnum, hv >> 1, red);
     return;
   }
-  // the queries of one token
-  const int64_t tok = blockIdx.x - a.kv_blocks;
-  int64_t at = -1;
-  if (a.m.cu == nullptr) {
-    at = static_cast<int64_t>(a.m.lengths[tok]) - 1;
-  } else {
-    // The token's sequence: as in kv_find, by the tokens each one brings.
-    int rel = 0;
-    const int b = kv_find(a.m, static_cast<int>(tok) - (a.m.cu[0] > 0 ? a.m.cu[0] : 0), rel,
-                          [](const KvSeq& s) { return static_cast<int>(s.n); });
-    if (b >= 0) {
-      const KvSeq s = kv_seq(a.m, b);
-      at = s.len - s.n + rel;
+  turn_queries<DT>(a, (blockIdx.x - a.kv_blocks) * (blockDim.x >> 6) + (threadIdx.x >> 6));
+}
+
+// One new token per sequence. A wave takes one side of a token's 64 / LANES kv
+// heads, LANES lanes a head, 8 dimensions a lane: where the general kernel has a
+// workgroup per head, of which a sixteenth of the lanes have anything to do.
+template <int ST, int DT, int LANES, bool VALUES>
+__device__ __forceinline__ void append_token(const KvAppendArg& a, int b, int h0) {
+  const int lane = threadIdx.x & 63, part = lane % LANES, d0 = 8 * part;
+  const int64_t len = a.m.lengths[b], at = len - 1;
+  if (len <= 0) return;
+  const int pid = kv_page(a.m, b, at >> a.m.page_shift);
+  if (pid < 0) return;
+  const int off = static_cast<int>(at) & (a.page - 1);
+  const int h = h0 + lane / LANES;
+  const bool mine = h < a.hkv && d0 < a.d;
+  const int64_t place = static_cast<int64_t>(pid) * a.hkv + (h < a.hkv ? h : 0);
+  uint8_t* codes = (VALUES ? a.vc : a.kc) + place * a.page * a.d;
+  float* scale = (VALUES ? a.vs : a.ks) + place;
+  const KvHeadsArg& src = VALUES ? a.v : a.k;
+  const float s_old = *scale;
+  float f[8] = {};
+  bool lost = false;
+  if (mine) {
+    const char* row = src.p + b * src.ts + h * src.hs;
+    if (VALUES || a.rope.rot == 0) {
+      load8<DT>(row, d0, f);
+    } else {
+      const int64_t pos = rope_row(a.rope, b, at);
+      lost = pos < 0;
+      turned8<DT>(row, d0, pos, a.rope, f);
     }
   }
-  const int64_t pos = rope_row(a.rope, tok, at);
-  const int per = a.d >> 3;
-  for (int u = threadIdx.x; u < a.hq * per; u += blockDim.x) {
-    const int h = u / per, d0 = (u % per) << 3;
-    float f[8];
-    turned8<DT>(a.q.p + tok * a.q.ts + h * a.q.hs, d0, pos, a.rope, f);
-    *reinterpret_cast<uint4*>(a.q_out + ((tok * a.hq + h) * a.d + d0) * 2) = pack8_out<DT>(f);
+  float amax = absmax8(f, 0.0f);
+  if (lost) amax = __builtin_inff();
+  amax = group_max<LANES>(amax);
+  const PageScale ps = settle<ST>(amax, s_old, off > 0);
+  if (h < a.hkv && off > 0 && ps.lower != 1.0f)
+    lower_codes<ST, VALUES>(codes, off, a.page, a.d, ps.lower, part, LANES);
+  // a chunk of values may hold the new token's place
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  if (!mine) return;
+  const uint2 w = encode8<ST>(f, ps.inv);
+  if constexpr (VALUES) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      codes[(d0 + k) * a.page + off] = static_cast<uint8_t>((k < 4 ? w.x : w.y) >> (8 * (k & 3)));
+  } else {
+    *reinterpret_cast<uint2*>(codes + off * a.d + d0) = w;
   }
+  if (part == 0) *scale = ps.scale;
+}
+
+template <int ST, int DT, int LANES>
+__global__ __launch_bounds__(kBlock) void k_kv_append_step(const KvAppendArg a) {
+  const int wave = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (wave >= a.step_waves) {
+    turn_queries<DT>(a, wave - a.step_waves);
+    return;
+  }
+  constexpr int HEADS = 64 / LANES;
+  const int per = 2 * ((a.hkv + HEADS - 1) / HEADS);     // waves of a token
+  const int b = wave / per, rest = wave % per;
+  if (rest & 1) append_token<ST, DT, LANES, true>(a, b, (rest >> 1) * HEADS);
+  else append_token<ST, DT, LANES, false>(a, b, (rest >> 1) * HEADS);
 }
 
 struct KvDequantArg {
@@ -525,24 +648,46 @@ extern "C" int cbq_kv_append(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   a.hq = has_q ? q_heads : 0;
   a.d = cache->head_dim;
   a.page = cache->page_size;
-  // n new tokens touch at most n pages and at most n / page + 2
   const int64_t T = batch->tokens, B = batch->batch;
-  int64_t pages = batch->cu == nullptr ? B : T / a.page + 2 * B;
-  if (pages > T) pages = T;
-  a.kv_blocks = pages * 2 * a.hkv;
-  const int64_t blocks = a.kv_blocks + (has_q ? T : 0);
-  CBQ_REQUIRE(blocks < (int64_t{1} << 31), "kv append: too many tokens for one call");
-  const int threads = block_for(a.page * a.d / 32);
-  const dim3 grid(static_cast<uint32_t>(blocks));
   hipStream_t st = as_stream(stream);
+  // few tokens: their queries over more waves
+  a.q_waves = T <= 1024 ? 4 : 1;
   const bool f16 = dtype == CBQ_F16;
-  if (cache->store == CBQ_KV_INT8) {
-    if (f16) k_kv_append<kKvInt8, kF16><<<grid, threads, 0, st>>>(a);
-    else k_kv_append<kKvInt8, kBF16><<<grid, threads, 0, st>>>(a);
-  } else {
-    if (f16) k_kv_append<kKvFp8, kF16><<<grid, threads, 0, st>>>(a);
-    else k_kv_append<kKvFp8, kBF16><<<grid, threads, 0, st>>>(a);
+  auto by_type = [&](auto kernel) {
+    if (cache->store == CBQ_KV_INT8) {
+      if (f16) kernel(std::integral_constant<int, kKvInt8>{}, std::integral_constant<int, kF16>{});
+      else kernel(std::integral_constant<int, kKvInt8>{}, std::integral_constant<int, kBF16>{});
+    } else {
+      if (f16) kernel(std::integral_constant<int, kKvFp8>{}, std::integral_constant<int, kF16>{});
+      else kernel(std::integral_constant<int, kKvFp8>{}, std::integral_constant<int, kBF16>{});
+    }
+  };
+  const int64_t q_total = has_q ? T * a.q_waves : 0;
+  if (batch->cu == nullptr) {
+    const int lanes = a.d <= 64 ? 8 : a.d <= 128 ? 16 : 32;
+    const int64_t waves = B * 2 * cdiv(a.hkv, 64 / lanes);
+    CBQ_REQUIRE(waves + q_total < (int64_t{1} << 31) - 4, "kv append: too many tokens for one call");
+    a.step_waves = static_cast<int>(waves);
+    const dim3 grid(static_cast<uint32_t>(cdiv(waves + q_total, 4)));
+    by_type([&](auto stc, auto dtc) {
+      constexpr int ST = decltype(stc)::value, DT = decltype(dtc)::value;
+      if (lanes == 8) k_kv_append_step<ST, DT, 8><<<grid, kBlock, 0, st>>>(a);
+      else if (lanes == 16) k_kv_append_step<ST, DT, 16><<<grid, kBlock, 0, st>>>(a);
+      else k_kv_append_step<ST, DT, 32><<<grid, kBlock, 0, st>>>(a);
+    });
+    return launch_status("cbq_kv_append");
   }
+  // n new tokens touch at most n pages and at most n / page + 2
+  const int64_t pages = std::min(T / a.page + 2 * B, T);
+  const int threads = block_for(a.page * a.d / 32);
+  a.kv_blocks = pages * 2 * a.hkv;
+  const int64_t blocks = a.kv_blocks + cdiv(q_total, threads / 64);
+  CBQ_REQUIRE(blocks < (int64_t{1} << 31) && q_total < (int64_t{1} << 31) - 4,
+              "kv append: too many tokens for one call");
+  const dim3 grid(static_cast<uint32_t>(blocks));
+  by_type([&](auto stc, auto dtc) {
+    k_kv_append<decltype(stc)::value, decltype(dtc)::value><<<grid, threads, 0, st>>>(a);
+  });
   return launch_status("cbq_kv_append");
 }
 
