@@ -14,6 +14,7 @@ import math
 import torch
 
 from ... import _abi
+from ._common import out_like
 
 STORE_CODE = {torch.int8: _abi.KV_INT8, torch.float8_e4m3fn: _abi.KV_FP8}
 _DTYPES = (torch.float16, torch.bfloat16)
@@ -128,7 +129,7 @@ def kv_append(view: _abi.KvCache, dev: torch.device, k: torch.Tensor, v: torch.T
     if q is not None:
         cq, q = _heads(q, dev, dt, None, d, tokens, "q")
         hq = q.size(1)
-        out = torch.empty((tokens, hq, d), dtype=dt, device=dev)
+        out = out_like(q, dt)
     cr = None
     if rope is not None:
         cos, sin = rope
@@ -199,7 +200,7 @@ def kv_attend(view: _abi.KvCache, dev: torch.device, q: torch.Tensor, page_table
     if max_length is not None and max_length < 0:
         raise RuntimeError(f"max_length must not be negative, got {max_length}")
     batch, keep = _batch(dev, tokens, page_table, lengths, cu_q)
-    out = torch.empty((tokens, hq, d), dtype=q.dtype, device=dev)
+    out = out_like(q, q.dtype)
     lse = torch.empty((tokens, hq), dtype=torch.float32, device=dev) if return_lse else None
     if tokens:
         L = _abi.lib()
