@@ -83,6 +83,8 @@ def _batch(dev, tokens: int, page_table, lengths, cu):
         if not cu.is_contiguous():
             cu = cu.contiguous()
         cu_ptr = cu.data_ptr()
+        if batch == 0 and tokens:
+            raise RuntimeError(f"{tokens} tokens of no sequence")
     if stride < width:      # an expanded table
         page_table = page_table.contiguous()
         stride = width

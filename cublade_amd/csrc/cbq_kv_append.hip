@@ -13,6 +13,12 @@
 // groups of 4 tokens, so that a word of 4 tokens' codes of one dimension is
 // made in one thread's registers and stored as it is, without LDS; the 4 lanes
 // that share a token still read 64 consecutive bytes of it.
+//
+// Bound by bytes: the new keys, values and queries in, the queries and codes out.
+// Measured on MI355X, kernel times: 8192 tokens of 32 query and 8 kv heads of 128
+// (185 MB) 38.6 us, 4.8 TB/s, where a copy reaches 5.1; 256 single tokens of 32 and
+// 32 heads of 64 10 us (24 with a workgroup per head); one token 3 us. Reading 128
+// pages of 64 tokens of 8 heads of 128 back (50 MB) 9.8 us, 5.1 TB/s.
 #include <algorithm>
 #include <type_traits>
 

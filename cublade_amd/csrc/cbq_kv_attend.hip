@@ -15,9 +15,19 @@
 // The matrix products compute S^T = K q^T and O^T = V^T w^T. In S^T's result
 // layout a lane holds 4 consecutive rows (keys) of one column (query row) per
 // tile; which cached token stands in which row is free, and chosen so that the
-// lane's keys are 16 consecutive tokens: what it has is then the second
-// product's operand as it is, and its V^T operand is 16 consecutive bytes of
-// one dimension in the transposed page. No operand passes through LDS.
+// lane's keys are consecutive tokens (16 in k_kv_attend_rows, 8 in
+// k_kv_attend_long): what it has is then the second product's operand as it is,
+// and its V^T operand is consecutive codes of one dimension in the transposed
+// page. The weights never leave their registers.
+//
+// Measured on MI355X, one call in a stream of calls (a copy reaches 5.1 TB/s, an
+// fp16 matrix product 1.15 PFLOP/s):
+//   32 query heads over 8 kv heads of 128, INT8, pages of 64 tokens:
+//     one token over 131077            53 us, 5.05 TB/s
+//     a prompt of 8192                590 us, 0.93 PFLOP/s
+//   128 tokens over 900 .. 1100 each, 16 heads of 64   44 us, 5.9 TB/s
+//   64 tokens over 100 .. 8000 each, FP8, pages of 16  113 us, 4.2 TB/s
+//   FP8, 2048 tokens of a prompt over 32768            1.12 ms, 0.95 PFLOP/s
 #include <algorithm>
 #include <type_traits>
 
@@ -251,9 +261,21 @@ __device__ __forceinline__ KvTile tile_of(const KvAttendArg& a, int item) {
   return t;
 }
 
+// ---------------------------------------------------------------------------
+// Few query rows: single tokens, drafted tokens.
+// ---------------------------------------------------------------------------
 // One workgroup: 16 query rows of one kv head (row = new token * rep + head in
 // the group) and one range of the keys. Its 4 waves take steps of 64 keys in
-// turn, each with its own maximum, sum and accumulators, joined at the end.
+// turn, each with its own maximum, sum and accumulators, joined at the end; no
+// operand passes through LDS. Bound by the bytes of the codes (6.3 TB/s from one
+// context length to the next) and about 25 us that a call takes before and after:
+// a workgroup's chain of length, page id, codes, and the joining of its waves and
+// of the ranges. The loads of a step's values and of the next step's keys are in
+// flight together, 16 x 16 bytes a lane at head size 128; more of them (values a
+// step ahead), more workgroups per CU or wider row tiles were slower.
+// Every tile's keys are cut into equally many ranges. Parts of equal length for
+// sequences of mixed lengths, found by each workgroup, even out their time but cost
+// more than that: a scan over the batch takes 4 us.
 // DP: head_dim padded to a multiple of 64; EXACT: head_dim is DP; NT: no other
 // workgroup reads the codes, and they are loaded past the caches (5.8 instead of
 // 5.2 TB/s for 128 sequences of 1000 tokens; slower where several tiles of rows
@@ -505,13 +527,19 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
 // ---------------------------------------------------------------------------
 // Many query rows: prompts and chunks of them.
 // ---------------------------------------------------------------------------
-// A workgroup takes 128 or 256 rows of one kv head, a wave 32 of them; it
-// goes through the keys 64 at a time. Codes are widened to fp16 once per workgroup, on their way from registers to LDS (K
-// rows [64 keys][DP], V^T rows [DP][64 keys]; every row has 16 bytes more than it
-// needs, so an odd number of 16-byte chunks: equal chunks of 16 consecutive rows
-// lie in distinct banks, and every access is a base register plus a constant), in
-// two buffers. Codes are loaded two steps ahead, their page ids three; one barrier
-// ends a step.
+// A workgroup takes 128 or 256 rows of one kv head, a wave 32 of them; it goes
+// through the keys 64 at a time. Codes are widened to fp16 once per workgroup, on
+// their way from registers to LDS (K rows [64 keys][DP], V^T rows [DP][64 keys];
+// every row has 16 bytes more than it needs, so an odd number of 16-byte chunks:
+// equal chunks of 16 consecutive rows lie in distinct banks, and every access is a
+// base register plus a constant), in two buffers. Codes are loaded two steps ahead,
+// their page ids three; one barrier ends a step.
+// Bound by instruction issue: a step's 32 matrix instructions of a wave take 1024
+// cycles of the matrix core but also about 16 each of the issue port that its 260
+// vector instructions (a third of them the 2^x and sums of 32 scores a lane) need,
+// with two waves per SIMD; the matrix cores are busy for 40% of the time, LDS for
+// a quarter. So the steps do without what can be had once: scales sit one block of 16
+// keys per lane, and no maximum is taken as long as the weights fit.
 //
 // Row r of a score tile of 32 keys is the key with bits 2 and 3 of r swapped: a
 // lane's scores 8 u .. 8 u + 7 are then the keys 16 u + 8 (lane / 32) .. + 7, the
@@ -1005,7 +1033,7 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
       scratch += splits * each;
       room -= splits * each;
     }
-    const int blocks = items * a.hkv * splits;
+    const int64_t blocks = items * a.hkv * splits;
     const bool wide = splits > 8;
     const int64_t joins = items * a.hkv * (wide ? tile : tile / 4);
     CBQ_REQUIRE(blocks < (int64_t{1} << 31) && joins < (int64_t{1} << 31),
@@ -1043,7 +1071,7 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
     if (rc) return rc;
   }
   if (p.long_items > 0) {
-    a.row_min = static_cast<int>(p.row_max) + 1;
+    a.row_min = p.row_items > 0 ? static_cast<int>(p.row_max) + 1 : 1;
     a.row_max = INT32_MAX;
     return run(p.long_items, p.long_tile, p.long_splits, [&](dim3 grid, auto stc, auto dpc) {
       constexpr int ST = decltype(stc)::value, DP = decltype(dpc)::value;

@@ -26,7 +26,7 @@ class QuantizedKVCache:
 
     k: codes [num_pages, kv_heads, page_size, head_dim]; v: codes, transposed,
     [num_pages, kv_heads, head_dim, page_size]; k_scale, v_scale: float32
-    [num_pages, kv_heads]. All contiguous, on one device. head_dim: a multiple
+    [num_pages, kv_heads], not negative. All contiguous, on one device. head_dim: a multiple
     of 16 up to 256; page_size: 16, 32, 64, 128 or 256. The tensors are fixed:
     write into them, or make another cache.
     """
@@ -44,6 +44,10 @@ class QuantizedKVCache:
 
     def __delattr__(self, name):
         raise AttributeError(f"QuantizedKVCache.{name} is fixed")
+
+    def __reduce__(self):
+        # pickle and deepcopy make the view of the new tensors anew
+        return QuantizedKVCache, (self.k, self.v, self.k_scale, self.v_scale)
 
     @classmethod
     def empty(cls, num_pages: int, kv_heads: int, head_dim: int, page_size: int = 64,

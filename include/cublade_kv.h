@@ -14,7 +14,7 @@
  *   v       [num_pages, kv_heads, head_dim, page_size]   8-bit codes (transposed:
  *           the attention reads 16 consecutive tokens of one dimension as one
  *           matrix-core operand, with no transposing pass)
- *   k_scale, v_scale [num_pages, kv_heads]
+ *   k_scale, v_scale [num_pages, kv_heads], not negative
  * A code stands for decode(code) * scale: INT8 in [-127, 127], or FP8 E4M3.
  *
  * What is on the device cannot be checked by the host, so the kernels check

@@ -151,6 +151,9 @@ def test_bindings_refuse_bad_tensors():
     cache = QuantizedKVCache.empty(2, 2, 32, 16)
     with pytest.raises(AttributeError):
         cache.k = cache.v
+    import copy
+    other = copy.deepcopy(cache)
+    assert other.k.data_ptr() != cache.k.data_ptr() and other._view.k == other.k.data_ptr()
     dev = "cuda"
     table = torch.zeros(1, 1, dtype=torch.int32, device=dev)
     n = torch.ones(1, dtype=torch.int32, device=dev)
@@ -173,6 +176,7 @@ def test_bindings_refuse_bad_tensors():
     bad("lengths", append_kv, cache, x, x, table, n.repeat(2))
     bad("one new token", append_kv, cache, x.repeat(2, 1, 1), x.repeat(2, 1, 1), table, n)
     bad("offsets", append_kv, cache, x, x, table, n, cu_new=n)
+    bad("no sequence", append_kv, cache, x, x, table[:0], n[:0], cu_new=n)
     bad("rope", append_kv, cache, x, x, table, n, rope=(c32.half(), c32))
     bad("rope", append_kv, cache, x, x, table, n, rope=(c32, c32[:2]))
     bad("rope", append_kv, cache, x, x, table, n, rope=(c32.repeat(1, 2), c32.repeat(1, 2)))
