@@ -844,11 +844,24 @@ __global__ __launch_bounds__(kBlock) void k_kv_attend_join(const KvAttendArg a) 
   const int rest = blockIdx.x / parts;
   const int h = rest % a.hkv;
   const int item = rest / a.hkv;
-  const KvTile tl = tile_of(a, item);
-  if (tl.b < 0 || tl.r_first + row >= tl.rows) return;
   const int64_t prow = static_cast<int64_t>(item * a.hkv + h) * a.tile_rows + row;
+  // What is read does not depend on whose row it is (places of rows that are not
+  // there exist too): all of it is under way before that is looked up.
+  constexpr int STEP = WIDE ? 4 : 1;
+  const int d0 = 4 * lane < a.d ? 4 * lane : 0;
+  f4 v[8];
+  auto load8 = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int s = s0 + k * STEP < a.splits ? s0 + k * STEP : 0;
+      v[k] = *reinterpret_cast<const f4*>(a.po + (s * a.prows + prow) * a.d + d0);
+    }
+  };
   float2 ml = make_float2(kNegInf, 0.0f);
   if (lane < a.splits) ml = a.pml[lane * a.prows + prow];
+  load8(WIDE ? wave : 0);
+  const KvTile tl = tile_of(a, item);
+  if (tl.b < 0 || tl.r_first + row >= tl.rows) return;
   float m = ml.x;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
@@ -856,16 +869,9 @@ __global__ __launch_bounds__(kBlock) void k_kv_attend_join(const KvAttendArg a) 
   float l = ml.y * f;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o, 64);
-  const int d0 = 4 * lane < a.d ? 4 * lane : 0;
   f4 acc = {};
-  constexpr int STEP = WIDE ? 4 : 1;
   for (int s0 = WIDE ? wave : 0; s0 < a.splits; s0 += 8 * STEP) {
-    f4 v[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int s = s0 + k * STEP < a.splits ? s0 + k * STEP : s0;
-      v[k] = *reinterpret_cast<const f4*>(a.po + (s * a.prows + prow) * a.d + d0);
-    }
+    if (s0 >= 8 * STEP) load8(s0);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const int s = s0 + k * STEP;
