@@ -323,9 +323,9 @@ __device__ void append_page(const KvAppendArg& a, int b, int64_t pnum, int h, fl
 }
 
 // The rotated queries of a token, by the wave `wave` of a.q_waves per token. A lane
-// keeps one unit, 8 pairs of dimensions (or 8 dimensions: interleaved pairs, those
-// that are not rotated, and all where the pieces do not fit) of every (64 / units)th
-// head, so the rotation's factors are read once for all of them.
+// keeps one unit, two pieces of 8 dimensions (8 pairs, or 16 that are not rotated),
+// of every (64 / units)th head, so the rotation's factors are read once for all of
+// them. Interleaved pairs, and pieces that do not fit, go one piece at a time.
 template <int DT>
 __device__ __forceinline__ void turn_queries(const KvAppendArg& a, int wave) {
   const int tok = wave / a.q_waves, turn = wave % a.q_waves;
@@ -345,40 +345,42 @@ __device__ __forceinline__ void turn_queries(const KvAppendArg& a, int wave) {
   }
   const int64_t pos = rope_row(a.rope, tok, at);
   const int lane = threadIdx.x & 63;
-  const bool pairs = a.rope.vec && !a.rope.interleaved && pos >= 0;
-  const int npairs = pairs ? a.rope.rot >> 4 : 0;
-  const int units = npairs + ((a.d - 16 * npairs) >> 3), heads = 64 / units;
+  const bool two = a.rope.rot == 0 || (a.rope.vec && !a.rope.interleaved && pos >= 0);
+  const int units = two ? a.d >> 4 : a.d >> 3, heads = 64 / units;
   const int unit = lane % units;
   const char* x = a.q.p + tok * a.q.ts;
   char* out = a.q_out + static_cast<int64_t>(tok) * a.hq * a.d * 2;
   if (lane >= heads * units) return;
-  if (unit < npairs) {
-    const int half = a.rope.rot >> 1, d0 = 8 * unit;
-    float c[8], sn[8];
+  const int h0 = turn * heads + lane / units, hstep = heads * a.q_waves;
+  if (two) {
+    const int half = a.rope.rot >> 1;
+    const bool turned = 8 * unit < half;
+    const int d0 = turned ? 8 * unit : 16 * unit, d1 = turned ? d0 + half : d0 + 8;
+    float c[8] = {}, sn[8] = {};
+    if (turned) {
 #pragma unroll
-    for (int k = 0; k < 8; k += 4) {
-      *reinterpret_cast<float4*>(c + k) = *reinterpret_cast<const float4*>(a.rope.cos + pos * half + d0 + k);
-      *reinterpret_cast<float4*>(sn + k) = *reinterpret_cast<const float4*>(a.rope.sin + pos * half + d0 + k);
+      for (int k = 0; k < 8; k += 4) {
+        *reinterpret_cast<float4*>(c + k) = *reinterpret_cast<const float4*>(a.rope.cos + pos * half + d0 + k);
+        *reinterpret_cast<float4*>(sn + k) = *reinterpret_cast<const float4*>(a.rope.sin + pos * half + d0 + k);
+      }
     }
-    for (int h = turn * heads + lane / units; h < a.hq; h += heads * a.q_waves) {
+    for (int h = h0; h < a.hq; h += hstep) {
       float f[8], g[8], o1[8], o2[8];
       load8<DT>(x + h * a.q.hs, d0, f);
-      load8<DT>(x + h * a.q.hs, d0 + half, g);
+      load8<DT>(x + h * a.q.hs, d1, g);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        o1[k] = f[k] * c[k] - g[k] * sn[k];
-        o2[k] = g[k] * c[k] + f[k] * sn[k];
+        o1[k] = turned ? f[k] * c[k] - g[k] * sn[k] : f[k];
+        o2[k] = turned ? g[k] * c[k] + f[k] * sn[k] : g[k];
       }
-      char* p = out + (h * a.d + d0) * 2;
-      *reinterpret_cast<uint4*>(p) = pack8_out<DT>(o1);
-      *reinterpret_cast<uint4*>(p + half * 2) = pack8_out<DT>(o2);
+      *reinterpret_cast<uint4*>(out + (h * a.d + d0) * 2) = pack8_out<DT>(o1);
+      *reinterpret_cast<uint4*>(out + (h * a.d + d1) * 2) = pack8_out<DT>(o2);
     }
   } else {
-    const int d0 = 8 * (unit + npairs);
-    for (int h = turn * heads + lane / units; h < a.hq; h += heads * a.q_waves) {
+    for (int h = h0; h < a.hq; h += hstep) {
       float f[8];
-      turned8<DT>(x + h * a.q.hs, d0, pos, a.rope, f);
-      *reinterpret_cast<uint4*>(out + (h * a.d + d0) * 2) = pack8_out<DT>(f);
+      turned8<DT>(x + h * a.q.hs, 8 * unit, pos, a.rope, f);
+      *reinterpret_cast<uint4*>(out + (h * a.d + 8 * unit) * 2) = pack8_out<DT>(f);
     }
   }
 }
