@@ -23,11 +23,11 @@
 // Measured on MI355X, one call in a stream of calls (a copy reaches 5.1 TB/s, an
 // fp16 matrix product 1.15 PFLOP/s):
 //   32 query heads over 8 kv heads of 128, INT8, pages of 64 tokens:
-//     one token over 131077            53 us, 5.05 TB/s
-//     a prompt of 8192                590 us, 0.93 PFLOP/s
+//     one token over 131077            52 us, 5.2 TB/s
+//     a prompt of 8192                600 us, 0.92 PFLOP/s
 //   128 tokens over 900 .. 1100 each, 16 heads of 64   44 us, 5.9 TB/s
 //   64 tokens over 100 .. 8000 each, FP8, pages of 16  113 us, 4.2 TB/s
-//   FP8, 2048 tokens of a prompt over 32768            1.12 ms, 0.95 PFLOP/s
+//   FP8, 2048 tokens of a prompt over 32768            1.15 ms, 0.93 PFLOP/s
 #include <algorithm>
 #include <type_traits>
 
@@ -550,7 +550,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_kv_attend_long(c
   constexpr int kLongTile = 32 * NW;
   constexpr int NS = DP / 16;          // steps of 16 dimensions in the scores
   constexpr int ND = DP / 32;          // tiles of 32 dimensions
-  constexpr int NL = DP / (16 * NW);   // 16-code loads per thread and side
+  constexpr int PER = 4 * DP / NW;     // 16-code pieces of a wave and side: a thread's in NL loads
+  constexpr int NL = (PER + 63) / 64;
+  constexpr bool ALL = PER % 64 == 0;  // every lane has a piece in each
   constexpr int KC = DP / 16;          // 16-code pieces of a key
   constexpr int KR = DP / 8 + 1, VR = kStep / 8 + 1;   // 16-byte chunks of a row in LDS
   const int d = EXACT ? DP : a.d;
@@ -623,10 +625,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_kv_attend_long(c
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int e = kfirst + lane + 64 * i, key = e / KC, dim = 16 * (e % KC);
-      if (!EXACT) rk[i] = u32x4{0, 0, 0, 0};
-      if (EXACT || dim < d) rk[i] = *reinterpret_cast<const u32x4*>(kp + (key * d + dim));
-      if (!EXACT) rv[i] = u32x4{0, 0, 0, 0};
-      if (EXACT || (tid >> 2) + 16 * NW * i < d) rv[i] = *reinterpret_cast<const u32x4*>(vp + 16 * NW * i * a.page);
+      const bool here = ALL || lane + 64 * i < PER;
+      if (!EXACT || !ALL) rk[i] = u32x4{0, 0, 0, 0};
+      if (here && (EXACT || dim < d)) rk[i] = *reinterpret_cast<const u32x4*>(kp + (key * d + dim));
+      if (!EXACT || !ALL) rv[i] = u32x4{0, 0, 0, 0};
+      if ((EXACT && ALL) || (tid >> 2) + 16 * NW * i < d) rv[i] = *reinterpret_cast<const u32x4*>(vp + 16 * NW * i * a.page);
     }
   };
   // In steps that some row of the workgroup does not see whole, NaN values (FP8)
@@ -653,7 +656,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_kv_attend_long(c
             bits |= (nb * 0x01020408u >> 24 & 0xfu) << (4 * w);   // bytes 0 .. 3 to bits 0 .. 3
             rv[i][w] &= ~(nb * 0xffu);
           }
-          lnan[buf][((tid >> 2) + 16 * NW * i) * 4 + (lane & 3)] = static_cast<uint16_t>(bits);
+          if (ALL || (tid >> 2) + 16 * NW * i < DP)
+            lnan[buf][((tid >> 2) + 16 * NW * i) * 4 + (lane & 3)] = static_cast<uint16_t>(bits);
           any |= bits;
         }
         const int found = __any(any != 0);
@@ -663,12 +667,16 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_kv_attend_long(c
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int e = kfirst + lane + 64 * i, key = e / KC, dim = 16 * (e % KC);
-      u32x4* kp = &lk[buf][(16 * kblock + key) * KR + dim / 8];
-      kp[0] = widen8<ST>(rk[i].x, rk[i].y);
-      kp[1] = widen8<ST>(rk[i].z, rk[i].w);
-      u32x4* vp = &lv[buf][((tid >> 2) + 16 * NW * i) * VR + 2 * (lane & 3)];
-      vp[0] = widen8<ST>(rv[i].x, rv[i].y);
-      vp[1] = widen8<ST>(rv[i].z, rv[i].w);
+      if (ALL || lane + 64 * i < PER) {
+        u32x4* kp = &lk[buf][(16 * kblock + key) * KR + dim / 8];
+        kp[0] = widen8<ST>(rk[i].x, rk[i].y);
+        kp[1] = widen8<ST>(rk[i].z, rk[i].w);
+      }
+      if (ALL || (tid >> 2) + 16 * NW * i < DP) {
+        u32x4* vp = &lv[buf][((tid >> 2) + 16 * NW * i) * VR + 2 * (lane & 3)];
+        vp[0] = widen8<ST>(rv[i].x, rv[i].y);
+        vp[1] = widen8<ST>(rv[i].z, rv[i].w);
+      }
     }
   };
   const int krow = (n32 & 0x13) | ((n32 & 4) << 1) | ((n32 & 8) >> 1);
@@ -915,6 +923,11 @@ constexpr int64_t kRowWgs = 4;
 
 int padded_dim(int d) { return (d + 63) / 64 * 64; }
 
+// Head sizes of k_kv_attend_long: 65 .. 96 in tiles of 96, without a quarter of
+// 128's products (a batch with 5 prompts of up to 1500 tokens, head size 80: 91 us,
+// padded to 128 95).
+int long_dim(int d) { return d > 64 && d <= 96 ? 96 : padded_dim(d); }
+
 // Waves of a k_kv_attend_long workgroup for `rows` rows of each kv head. 8 share a
 // step's codes (one workgroup per CU; a prompt of 8192 tokens 588 us, with 4 and two
 // workgroups 627), 4 leave less of the GPU idle in the last round of few
@@ -930,7 +943,7 @@ int long_waves(int dp, int64_t rows, int kv_heads, bool one_sequence) {
 KvPlan plan_of(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t max_length) {
   KvPlan p = {};
   const int64_t rows = b->tokens * rep;
-  p.long_tile = 32 * long_waves(padded_dim(c->head_dim), rows, c->kv_heads, b->batch == 1);
+  p.long_tile = 32 * long_waves(long_dim(c->head_dim), rows, c->kv_heads, b->batch == 1);
   if (b->cu == nullptr) {
     p.row_items = b->batch * cdiv(rep, kRowTile);
   } else {
@@ -1026,7 +1039,7 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   hipStream_t st = as_stream(stream);
   // One launch over `items` tiles of `tile` rows, the keys in `splits` ranges (as
   // many as the workspace has room for), and the launch that joins them.
-  auto run = [&](int64_t items, int tile, int splits, auto kernel) -> int {
+  auto run = [&](int64_t items, int tile, int splits, int dim, auto kernel) -> int {
     const size_t each = partial_bytes(cache, items, tile);
     splits = std::max(1, static_cast<int>(std::min<size_t>(splits, room / each)));
     a.items = static_cast<int>(items);
@@ -1046,8 +1059,9 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
                 "kv attend: too many tokens for one call");
     const dim3 grid(static_cast<uint32_t>(blocks));
     auto by_dim = [&](auto stc) {
-      switch (padded_dim(a.d)) {
+      switch (dim) {
         case 64: kernel(grid, stc, std::integral_constant<int, 64>{}); break;
+        case 96: kernel(grid, stc, std::integral_constant<int, 96>{}); break;
         case 128: kernel(grid, stc, std::integral_constant<int, 128>{}); break;
         case 192: kernel(grid, stc, std::integral_constant<int, 192>{}); break;
         default: kernel(grid, stc, std::integral_constant<int, 256>{}); break;
@@ -1065,8 +1079,9 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
     a.row_min = 1;
     a.row_max = batch->cu == nullptr ? rep : static_cast<int>(p.row_max);
     const bool alone = batch->cu == nullptr && rep <= kRowTile;
-    const int rc = run(p.row_items, kRowTile, p.row_splits, [&](dim3 grid, auto stc, auto dpc) {
-      constexpr int ST = decltype(stc)::value, DP = decltype(dpc)::value;
+    const int rc = run(p.row_items, kRowTile, p.row_splits, padded_dim(a.d), [&](dim3 grid, auto stc, auto dpc) {
+      constexpr int ST = decltype(stc)::value;
+      constexpr int DP = decltype(dpc)::value == 96 ? 128 : decltype(dpc)::value;   // (96 does not come)
       auto go = [&](auto nt) {
         if (a.d == DP) k_kv_attend_rows<ST, DP, true, nt.value><<<grid, kBlock, 0, st>>>(a);
         else k_kv_attend_rows<ST, DP, false, nt.value><<<grid, kBlock, 0, st>>>(a);
@@ -1079,7 +1094,7 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   if (p.long_items > 0) {
     a.row_min = p.row_items > 0 ? static_cast<int>(p.row_max) + 1 : 1;
     a.row_max = INT32_MAX;
-    return run(p.long_items, p.long_tile, p.long_splits, [&](dim3 grid, auto stc, auto dpc) {
+    return run(p.long_items, p.long_tile, p.long_splits, long_dim(a.d), [&](dim3 grid, auto stc, auto dpc) {
       constexpr int ST = decltype(stc)::value, DP = decltype(dpc)::value;
       auto go = [&](auto nwc) {
         constexpr int NW = decltype(nwc)::value;

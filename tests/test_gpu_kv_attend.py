@@ -331,3 +331,29 @@ def test_small_workspace_gives_the_same_within_rounding():
                                    lse.data_ptr(), _abi.stream_handle(cache.device)), "attend")
         _kv.assert_attends((o, lse), ref, F16, nbytes)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("store,dt", [(I8, BF16), (F8, F16), (F8, BF16)])
+@pytest.mark.parametrize("d,page", [(80, 16), (96, 32), (96, 256)])
+def test_prompts_of_96_wide_tiles(d, page, store, dt):
+    """Head sizes over 64 and up to 96 with many rows: the tiles are 96 wide, and
+    lanes of a workgroup's second piece have none."""
+    _check(d, page, store, dt, 2, 4, [1, 130, 64, 333, 129], [1, 130, 0, 200, 33])
+    _check(d, page, store, dt, 1, 2, [500], [300], window=70)
+    _check(d, page, store, dt, 2, 2, [200, 90], [200, 70], causal=False)
+
+
+@pytest.mark.parametrize("d", [80, 96])
+@pytest.mark.parametrize("dim", [3, 63, 64, 79])
+def test_nan_value_in_96_wide_tiles(d, dim):
+    """One FP8 NaN value reaches its dimension of the rows that see its token, in
+    either piece of a thread's dimensions."""
+    from cublade_amd.quantization import attend_kv
+    n, rep = 150, 4
+    q, cache, table, (base, _) = _check(d, 32, F8, BF16, 1, rep, [n], [n])
+    j = 101
+    cache.v.view(torch.uint8)[int(table[0, j // 32]), 0, dim, j % 32] = 0x7F
+    o = attend_kv(q, cache, table, _i32([n]), cu_q=_cu([n]))
+    rest = [i for i in range(d) if i != dim]
+    assert bool(o[j:, :, dim].isnan().all())
+    assert torch.equal(o[:j], base[:j]) and torch.equal(o[j:][..., rest], base[j:][..., rest])
