@@ -916,6 +916,13 @@ struct KvPlan {
 // more than it could save.
 constexpr int64_t kShortRows = 64;
 constexpr int64_t kFewRows = 32;
+// Where a window leaves every row at most this many keys, and the sequences make at
+// most a tile per CU, k_kv_attend_long takes all rows in one launch: a single token's
+// tile is then no longer than a prompt's. (A batch of 5 prompts and 15 single tokens
+// over 1024 keys 82 instead of 96 us; 1 and 4 of 128 over 256 keys 44 and 54. Beyond,
+// splitting the single tokens' keys is worth more: over 2048 keys beside short
+// prompts 62 and 40 us in one launch and two, with 496 tiles 88 and 80.)
+constexpr int64_t kSharedKeys = 1024;
 // Workgroups per CU that the keys of few tiles are split for. 2 fit at once
 // (head size 128); with 4 a batch of mixed lengths takes 113 instead of 126 us (64
 // sequences of 100 to 8000 tokens), one sequence the same.
@@ -925,13 +932,13 @@ int padded_dim(int d) { return (d + 63) / 64 * 64; }
 
 // Head sizes of k_kv_attend_long: 65 .. 96 in tiles of 96, without a quarter of
 // 128's products (a batch with 5 prompts of up to 1500 tokens, head size 80: 91 us,
-// padded to 128 95).
+// padded to 128 95, both in two launches).
 int long_dim(int d) { return d > 64 && d <= 96 ? 96 : padded_dim(d); }
 
 // Waves of a k_kv_attend_long workgroup for `rows` rows of each kv head. 8 share a
 // step's codes (one workgroup per CU; a prompt of 8192 tokens 588 us, with 4 and two
 // workgroups 627), 4 leave less of the GPU idle in the last round of few
-// workgroups (a batch with 5 prompts of up to 1500 tokens: 105 and 110 us). Other
+// workgroups (a batch with 5 prompts of up to 1500 tokens, in tiles of 128: 105 and 110 us). Other
 // head sizes have registers or loads for 4 only.
 int long_waves(int dp, int64_t rows, int kv_heads, bool one_sequence) {
   if (dp != 128) return 4;
@@ -940,7 +947,7 @@ int long_waves(int dp, int64_t rows, int kv_heads, bool one_sequence) {
   return fills || wgs >= 3 * cus ? 8 : 4;
 }
 
-KvPlan plan_of(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t max_length) {
+KvPlan plan_of(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t max_length, int64_t window) {
   KvPlan p = {};
   const int64_t rows = b->tokens * rep;
   p.long_tile = 32 * long_waves(long_dim(c->head_dim), rows, c->kv_heads, b->batch == 1);
@@ -955,6 +962,11 @@ KvPlan plan_of(const cbq_kv_cache* c, const cbq_kv_batch* b, int rep, int64_t ma
     if (rows > p.row_max)
       p.long_items = one ? cdiv(rows, p.long_tile)
                          : rows / p.long_tile + std::min<int64_t>(b->batch, rows / (p.row_max + 1));
+    if (p.row_items > 0 && p.long_items > 0 && window > 0 && window <= kSharedKeys &&
+        static_cast<int64_t>(b->batch) * c->kv_heads <= device_cus()) {
+      p.row_items = 0;
+      p.long_items = rows / p.long_tile + std::min<int64_t>(b->batch, rows);
+    }
   }
   const int64_t cap = static_cast<int64_t>(b->max_pages) * c->page_size;
   const int64_t len = max_length > 0 ? std::min(max_length, cap) : cap;
@@ -985,7 +997,7 @@ extern "C" size_t cbq_kv_attend_ws_bytes(const cbq_kv_cache* cache, const cbq_kv
   if (cache == nullptr || batch == nullptr || cache->kv_heads <= 0 || q_heads <= 0 ||
       q_heads % cache->kv_heads != 0 || batch->tokens <= 0)
     return CBQ_WS_CTRL_BYTES;
-  const KvPlan p = plan_of(cache, batch, q_heads / cache->kv_heads, max_length);
+  const KvPlan p = plan_of(cache, batch, q_heads / cache->kv_heads, max_length, 0);   // (a window's one launch has room for fewer splits, at times)
   size_t n = 0;
   if (p.row_splits > 1) n += p.row_splits * partial_bytes(cache, p.row_items, kRowTile);
   if (p.long_splits > 1) n += p.long_splits * partial_bytes(cache, p.long_items, p.long_tile);
@@ -1033,7 +1045,7 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   a.page = cache->page_size;
   a.causal = causal != 0;
   a.bf16 = dtype == CBQ_BF16;
-  const KvPlan p = plan_of(cache, batch, rep, max_length);
+  const KvPlan p = plan_of(cache, batch, rep, max_length, window);
   size_t room = ws != nullptr && ws_bytes > CBQ_WS_CTRL_BYTES ? ws_bytes - CBQ_WS_CTRL_BYTES : 0;
   char* scratch = static_cast<char*>(ws) + CBQ_WS_CTRL_BYTES;
   hipStream_t st = as_stream(stream);

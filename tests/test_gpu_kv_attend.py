@@ -357,3 +357,43 @@ def test_nan_value_in_96_wide_tiles(d, dim):
     rest = [i for i in range(d) if i != dim]
     assert bool(o[j:, :, dim].isnan().all())
     assert torch.equal(o[:j], base[:j]) and torch.equal(o[j:][..., rest], base[j:][..., rest])
+
+
+@pytest.mark.parametrize("store,dt", [(I8, BF16), (F8, F16)])
+@pytest.mark.parametrize("d,page", [(128, 64), (80, 16), (64, 32), (192, 16), (256, 128)])
+@pytest.mark.parametrize("window", [1, 70, 1024])
+def test_window_over_prompts_and_single_tokens(d, page, store, dt, window):
+    """Single tokens, drafted ones and prompts under a window that one launch takes
+    them all with: sequences that bring nothing, hold nothing, or bring more than
+    they hold."""
+    _check(d, page, store, dt, 2, 4, [1300, 900, 1, 0, 40, 65, 700, 3], [150, 1, 1, 0, 9, 1, 33, 1],
+           window=window)
+    _check(d, page, store, dt, 1, 4, [5, 200, 0, 400], [9, 150, 2, 1], window=window)
+
+
+@pytest.mark.parametrize("store,dt", [(I8, BF16), (F8, F16)])
+def test_window_in_two_launches(store, dt):
+    """Windows and batches past what one launch takes."""
+    _check(64, 32, store, dt, 2, 4, [2500, 1900, 70, 2100], [150, 1, 1, 5], window=1500)
+    n = 170
+    _check(64, 16, store, dt, 2, 32, [100 + i for i in range(n)],
+           [64 if i % 40 == 0 else 1 for i in range(n)], window=50)
+
+
+def test_window_of_one_launch_keeps_nan_to_its_rows():
+    """An FP8 NaN value ahead of a window, or outside another sequence, reaches
+    no row; inside, its dimension of the rows that see it."""
+    from cublade_amd.quantization import attend_kv
+    lens, news = [300, 200, 90], [100, 1, 1]
+    q, cache, table, (base, _) = _check(96, 32, F8, F16, 1, 4, lens, news, window=40)
+    args = (table, _i32(lens))
+    v8 = cache.v.view(torch.uint8)
+    v8[int(table[1, 4]), 0, 7, 130 % 32] = 0x7F      # token 130 of 200: before its window
+    o = attend_kv(q, cache, *args, cu_q=_cu(news), window=40)
+    assert torch.equal(o, base)
+    v8[int(table[1, 5]), 0, 7, 170 % 32] = 0x7F      # token 170: inside
+    o = attend_kv(q, cache, *args, cu_q=_cu(news), window=40)
+    assert bool(o[100, :, 7].isnan().all())
+    rest = [i for i in range(96) if i != 7]
+    assert torch.equal(o[100][:, rest], base[100][:, rest])
+    assert torch.equal(o[:100], base[:100]) and torch.equal(o[101:], base[101:])
