@@ -16,7 +16,7 @@
 //
 // Bound by bytes: the new keys, values and queries in, the queries and codes out.
 // Measured on MI355X, kernel times: 8192 tokens of 32 query and 8 kv heads of 128
-// (185 MB) 38.6 us, 4.8 TB/s, where a copy reaches 5.1; 256 single tokens of 32 and
+// (185 MB) 36.8 us, 5.0 TB/s, where a copy reaches 5.1; 256 single tokens of 32 and
 // 32 heads of 64 10 us (24 with a workgroup per head); one token 3 us. Reading 128
 // pages of 64 tokens of 8 heads of 128 back (50 MB) 9.8 us, 5.1 TB/s.
 #include <algorithm>
@@ -250,32 +250,67 @@ __device__ void append_page(const KvAppendArg& a, int b, int64_t pnum, int h, fl
     }
   };
   bool lost = false;   // a token whose position is outside the rotation tables
-  auto fetch = [&](int t, int d0, float (&f)[8]) {
-    const int64_t tok = tokbase + t;
-    const char* row = x + tok * src.ts;
-    if constexpr (VALUES) {
-      load8<DT>(row, d0, f);
-    } else if (a.rope.rot == 0) {
-      load8<DT>(row, d0, f);
+  // A unit's 4 tokens, those that are not new as the nearest new one (they change
+  // no maximum and are not stored): no load waits for another token's branch. (Keys
+  // and values of 7527 tokens in pages of 32, 6 heads of 96: 15 us, 18 with a branch
+  // per token.)
+  auto fetch = [&](int t0, int d0, float (&f)[4][8]) {
+    int off[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) off[j] = t0 + j < lo ? lo : t0 + j < hi ? t0 + j : hi - 1;
+    if (VALUES || a.rope.rot == 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) load8<DT>(x + (tokbase + off[j]) * src.ts, d0, f[j]);
+    } else if (a.rope.vec && !a.rope.interleaved && a.rope.rows > 0) {
+      const int half = a.rope.rot >> 1;
+      const bool turned = d0 < a.rope.rot, low = d0 < half;
+      const int i0 = !turned ? 0 : low ? d0 : d0 - half;
+      const int dg = !turned ? d0 : low ? d0 + half : i0;
+      float g[4][8];
+      int64_t pos[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t tok = tokbase + off[j];
+        load8<DT>(x + tok * src.ts, d0, f[j]);
+        load8<DT>(x + tok * src.ts, dg, g[j]);
+        pos[j] = rope_row(a.rope, tok, page0 + off[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool none = pos[j] < 0;
+        const int64_t at = (none ? 0 : pos[j]) * half + i0;
+        float c[8], sn[8];
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) {
+          *reinterpret_cast<float4*>(c + k) = *reinterpret_cast<const float4*>(a.rope.cos + at + k);
+          *reinterpret_cast<float4*>(sn + k) = *reinterpret_cast<const float4*>(a.rope.sin + at + k);
+        }
+        lost |= none;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float r = f[j][k] * c[k] + g[j][k] * (low ? -sn[k] : sn[k]);
+          f[j][k] = !turned ? f[j][k] : none ? __builtin_nanf("") : r;
+        }
+      }
     } else {
-      const int64_t pos = rope_row(a.rope, tok, page0 + t);
-      lost |= pos < 0;
-      turned8<DT>(row, d0, pos, a.rope, f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t tok = tokbase + off[j], pos = rope_row(a.rope, tok, page0 + off[j]);
+        lost |= pos < 0;
+        turned8<DT>(x + tok * src.ts, d0, pos, a.rope, f[j]);
+      }
     }
   };
 
   float amax = 0.0f;
-  float f[4][8] = {};   // tokens of a unit that are not new are encoded too, and not stored
+  float f[4][8] = {};
   for (int u = threadIdx.x; u < units; u += blockDim.x) {
     int t0, d0;
     unit_of(u, t0, d0);
+    if (t0 + 4 <= lo || t0 >= hi) continue;
+    fetch(t0, d0, f);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (t0 + j >= lo && t0 + j < hi) {
-        fetch(t0 + j, d0, f[j]);
-        amax = absmax8(f[j], amax);
-      }
-    }
+    for (int j = 0; j < 4; ++j) amax = absmax8(f[j], amax);
   }
   if (lost) amax = __builtin_inff();
   const float s_old = *scale;
@@ -294,11 +329,7 @@ __device__ void append_page(const KvAppendArg& a, int b, int64_t pnum, int h, fl
     unit_of(u, t0, d0);
     if (t0 + 4 <= lo || t0 >= hi) continue;
     const bool whole = t0 >= lo && t0 + 4 <= hi;
-    if (units > static_cast<int>(blockDim.x)) {   // else f still holds the only unit
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (t0 + j >= lo && t0 + j < hi) fetch(t0 + j, d0, f[j]);
-    }
+    if (units > static_cast<int>(blockDim.x)) fetch(t0, d0, f);   // else f still holds the only unit
     if constexpr (VALUES) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {

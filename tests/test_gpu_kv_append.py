@@ -274,3 +274,35 @@ def test_offsets_past_32_bits():
     assert int((cache.k[0] != 0).sum()) == 0 and int((cache.v[0] != 0).sum()) == 0
     o, lse = attend_kv(x[:1], cache, last, _i32([page]), return_lse=True)
     _kv.assert_attends((o, lse), _kv.attend_ref(x[:1], cache, last, [page], [1]), torch.float16)
+
+
+@pytest.mark.parametrize("store", [I8, F8])
+@pytest.mark.parametrize("begun", [0, 3, 6])
+def test_rotation_table_ends_inside_a_page(store, begun):
+    """Half of each head rotated, tokens past the table in the second page only:
+    the first page, begun or not, is as without them; their page's keys are lost,
+    its values and all other queries are not."""
+    from cublade_amd.quantization import append_kv
+    g, page, d, rot, n = _gen(11), 32, 64, 32, 45
+    cache = _kv.random_cache(3, 2, d, page, store, g)
+    model = _kv.CacheModel(cache)
+    cos, sin = _kv.tables(37, rot)
+    table, new = _i32([[2, 0]]), n - begun
+    k = torch.randn(new, 2, d, generator=g, device=DEV).bfloat16()
+    v = torch.randn(new, 2, d, generator=g, device=DEV).bfloat16()
+    q = torch.randn(new, 4, d, generator=g, device=DEV).bfloat16()
+    out = append_kv(cache, k, v, table, _i32([n]), cu_new=_cu([new]), rope=(cos, sin), q=q)
+    pos = torch.arange(begun, n, device=DEV)
+    ok = pos.clamp(max=36)
+    model.append(_kv.rotate_f32(k, ok, cos, sin, False), v, table, [n], [new])
+    keep = [1, 2]
+    assert torch.equal(cache.k_scale[keep], model.ks[keep])
+    assert torch.equal(cache.k.view(torch.uint8)[keep], model.k.view(torch.uint8)[keep])
+    assert torch.equal(cache.v_scale, model.vs)
+    assert torch.equal(cache.v.view(torch.uint8).transpose(2, 3), model.v.view(torch.uint8))
+    assert bool(cache.k_scale[0].isinf().all())
+    want = _kv.rotate_f32(q, ok, cos, sin, False).bfloat16()
+    here = pos < 37
+    assert torch.equal(out[here], want[here])
+    assert bool(out[~here][..., :rot].isnan().all())
+    assert torch.equal(out[~here][..., rot:], q[~here][..., rot:])
