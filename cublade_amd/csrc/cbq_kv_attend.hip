@@ -173,7 +173,8 @@ __device__ __forceinline__ void put_row(const KvAttendArg& a, int64_t row, int64
     if (d0 == 0) a.pml[at] = bad ? make_float2(0.0f, __builtin_nanf("")) : make_float2(m, l);
     return;
   }
-  const bool none = m == kNegInf;
+  // (scores that are all NaN raise no maximum either; their sum is NaN)
+  const bool none = m == kNegInf && l == 0.0f;
   float inv = none ? 0.0f : 1.0f / l;
   if (bad) inv = __builtin_nanf("");
   const float f[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};

@@ -397,3 +397,26 @@ def test_window_of_one_launch_keeps_nan_to_its_rows():
     rest = [i for i in range(96) if i != 7]
     assert torch.equal(o[100][:, rest], base[100][:, rest])
     assert torch.equal(o[:100], base[:100]) and torch.equal(o[101:], base[101:])
+
+
+@pytest.mark.parametrize("news", [None, [40, 40, 40, 40]])
+@pytest.mark.parametrize("n", [40, 9000])
+def test_lse_is_nan_where_every_score_is(n, news):
+    """-infinity is the log-sum-exp of rows that see no key, not of rows that
+    see none but NaN scores: queries of NaN, pages that are not in the pool."""
+    from cublade_amd.quantization import attend_kv
+    g = _gen(21)
+    lens = [n, n, n, 0]
+    table, pages = _kv.make_table(lens, 16, g)
+    cache = _kv.random_cache(pages, 1, 64, 16, I8, g)
+    table[1] = -1
+    t = 4 if news is None else sum(news)
+    q = torch.randn(t, 2, 64, generator=g, device=DEV).half()
+    per = t // 4
+    q[:per, 0] = math.nan
+    o, lse = attend_kv(q, cache, table, _i32(lens), cu_q=None if news is None else _cu(news),
+                       return_lse=True)
+    for x in (o, lse):
+        assert bool(x[:per, 0].isnan().all()) and bool(x[:per, 1].isfinite().all())
+        assert bool(x[per:2 * per].isnan().all()) and bool(x[2 * per:3 * per].isfinite().all())
+    assert bool((o[3 * per:] == 0).all()) and bool((lse[3 * per:] == -math.inf).all())
