@@ -178,11 +178,15 @@ __device__ __forceinline__ PageScale settle(float amax, float s_old, bool begun)
   }
   p.scale = s_old;
   p.lower = 1.0f;
-  const float t = amax / (kv_qmax<ST>() * s_old);
+  float t = amax / (kv_qmax<ST>() * s_old);
   if (t > 1.0f) {
+    // A finite maximum may be past fp32's range in units of the smallest scales
+    // (a bf16 number above 3.4e26 after zeros): it then grows by 2^64 more than t.
+    const bool far = t == __builtin_inff();
+    if (far) t = amax * 0x1p-64f / (kv_qmax<ST>() * s_old);
     int e = 0;
     const float mant = __builtin_frexpf(t, &e);
-    const int g = mant > 0.5f ? e : e - 1;
+    const int g = (mant > 0.5f ? e : e - 1) + (far ? 64 : 0);
     const bool fin = t < __builtin_inff();
     p.scale = fin ? __builtin_ldexpf(s_old, g) : __builtin_inff();
     p.lower = fin ? __builtin_ldexpf(1.0f, -g) : 0.0f;

@@ -306,3 +306,31 @@ def test_rotation_table_ends_inside_a_page(store, begun):
     assert torch.equal(out[here], want[here])
     assert bool(out[~here][..., :rot].isnan().all())
     assert torch.equal(out[~here][..., rot:], q[~here][..., rot:])
+
+
+@pytest.mark.parametrize("store", [I8, F8])
+@pytest.mark.parametrize("chunk", [False, True])
+@pytest.mark.parametrize("big", [1e30, 3e38])
+def test_scale_grows_by_more_than_the_range_of_32_bits(store, chunk, big):
+    """The largest finite values after a page's zeros: the scale grows from
+    1e-12 / Q to a finite one at most twice what the values need."""
+    from cublade_amd.quantization import QuantizedKVCache, append_kv, dequantize_kv
+    g = _gen(31)
+    cache = QuantizedKVCache.empty(2, 1, 32, 16, store)
+    zeros = torch.zeros(3, 1, 32, device=DEV, dtype=torch.bfloat16)
+    append_kv(cache, zeros, zeros, _i32([[1]]), _i32([3]), cu_new=_cu([3]))
+    n = 2 if chunk else 1
+    x = ((torch.rand(n, 1, 32, generator=g, device=DEV) * 2 - 1) * big).bfloat16()
+    append_kv(cache, x, x, _i32([[1]]), _i32([3 + n]), cu_new=_cu([n]) if chunk else None)
+    q, amax = _kv.QMAX[store], float(x.abs().max())
+    for s in (float(cache.k_scale[1]), float(cache.v_scale[1])):
+        assert amax / q <= s * (1 + 2.0 ** -22) and s <= 2 * amax / q * (1 + 2.0 ** -22)
+    # half a step of the scale (INT8), or of the code (E4M3: 2^-4 relative, and at
+    # least 2^-10); a bf16 rounding
+    s = float(cache.k_scale[1])
+    for t in dequantize_kv(cache, _i32([1])):
+        assert bool((t[0, 0, :3] == 0).all())
+        want = x[:, 0].double()
+        half = s / 2 if store == I8 else (want.abs() * 2.0 ** -4).clamp(min=s * 2.0 ** -10)
+        assert bool(((t[0, 0, 3:3 + n].double() - want).abs()
+                     <= half * (1 + 2.0 ** -20) + (want.abs() + half) * 2.0 ** -8).all())
