@@ -209,9 +209,10 @@ __device__ __forceinline__ void load_q(const KvAttendArg& a, const char* qp, boo
   }
   if (!a.bf16) return;
   amax = row_max(amax);
-  const int e = static_cast<int>(__float_as_uint(amax) >> 23);   // biased exponent
+  int e = static_cast<int>(__float_as_uint(amax) >> 23);   // biased exponent
   float up = 1.0f;
-  if (e > 0 && e < 254) {     // amax * up in [1, 2)
+  if (e > 0 && e < 255) {     // amax * up in [1, 2); in [2, 4) from 2^127, whose inverse is no normal number
+    e = e < 254 ? e : 253;
     up = __uint_as_float(static_cast<uint32_t>(254 - e) << 23);
     cq *= __uint_as_float(static_cast<uint32_t>(e) << 23);
   }

@@ -420,3 +420,21 @@ def test_lse_is_nan_where_every_score_is(n, news):
         assert bool(x[:per, 0].isnan().all()) and bool(x[:per, 1].isfinite().all())
         assert bool(x[per:2 * per].isnan().all()) and bool(x[2 * per:3 * per].isfinite().all())
     assert bool((o[3 * per:] == 0).all()) and bool((lse[3 * per:] == -math.inf).all())
+
+
+@pytest.mark.parametrize("news", [None, [70]])
+def test_largest_finite_queries(news):
+    """bf16 queries of the last binade, [2^127, 2^128), whose scores are finite."""
+    from cublade_amd.quantization import attend_kv
+    g, lens = _gen(23), [100]
+    table, pages = _kv.make_table(lens, 16, g)
+    cache = _kv.random_cache(pages, 1, 64, 16, I8, g)
+    t, scale = 1 if news is None else 70, 2.0 ** -124
+    q = (torch.rand(t, 4, 64, generator=g, device=DEV) * 2 - 1) * 2.0 ** 127
+    q[:, :, 5] = 2.0 ** 127 * 1.5
+    q = q.bfloat16()
+    got = attend_kv(q, cache, table, _i32(lens), scale=scale, return_lse=True,
+                    cu_q=None if news is None else _cu(news))
+    assert bool(got[0].isfinite().all())
+    ref = _kv.attend_ref(q, cache, table, lens, news or [1], scale=scale)
+    _kv.assert_attends(got, ref, BF16, news)
