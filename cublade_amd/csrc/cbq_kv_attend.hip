@@ -24,10 +24,10 @@
 // fp16 matrix product 1.15 PFLOP/s):
 //   32 query heads over 8 kv heads of 128, INT8, pages of 64 tokens:
 //     one token over 131077            52 us, 5.2 TB/s
-//     a prompt of 8192                605 us, 0.91 PFLOP/s
+//     a prompt of 8192                579 to 609 us, 0.90 to 0.95 PFLOP/s
 //   128 tokens over 900 .. 1100 each, 16 heads of 64   44 us, 5.9 TB/s
 //   64 tokens over 100 .. 8000 each, FP8, pages of 16  113 us, 4.2 TB/s
-//   FP8, 2048 tokens of a prompt over 32768            1.15 ms, 0.93 PFLOP/s
+//   FP8, 2048 tokens of a prompt over 32768            1.11 to 1.15 ms, 0.92 to 0.96 PFLOP/s
 #include <algorithm>
 #include <type_traits>
 
