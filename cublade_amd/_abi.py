@@ -182,19 +182,37 @@ _ws: dict[tuple[int, int], torch.Tensor] = {}
 # the caching allocator has handed to another tensor.
 _ws_retired: list[torch.Tensor] = []
 _ws_lock = threading.Lock()
+_ws_turns: dict[tuple[int, int], threading.RLock] = {}
+
+
+def workspace_lock(device: torch.device):
+    """Lock of (device, current stream)'s workspace: hold it from workspace()
+    until the library call that uses it has returned. Entries queue several
+    kernels that pass data through the workspace, and a ctypes call lets other
+    threads run: without the lock two threads on one stream (every thread's
+    default) could queue theirs in between, and read each other's data."""
+    key = (device_index(device), stream_handle(device))
+    lock = _ws_turns.get(key)
+    if lock is None:
+        with _ws_lock:
+            lock = _ws_turns.setdefault(key, threading.RLock())
+    return lock
 
 
 def workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     """Workspace for (device, current stream), at least ``nbytes`` long,
-    zero-filled when created. The library keeps state in its control block
-    between calls (the one-launch per-tensor quant's call count and slots),
-    so the buffer is reused as-is. A larger request replaces it with a fresh
+    zero-filled when created; taken and used under workspace_lock. The library
+    keeps state in its control block between calls (the one-launch per-tensor
+    quant's call count and slots), so the buffer is reused as-is. A larger request replaces it with a fresh
     zero-filled one (allocated on the same stream, hence ordered); the old
     one is kept alive for graphs captured with it. Growing during a graph
     capture raises: run one call of each captured shape on the capture
     stream first."""
     nbytes = max(int(nbytes), WS_CTRL_BYTES)
     key = (device_index(device), stream_handle(device))
+    buf = _ws.get(key)
+    if buf is not None and buf.numel() >= nbytes:
+        return buf
     with _ws_lock:
         buf = _ws.get(key)
         if buf is None or buf.numel() < nbytes:

@@ -183,7 +183,7 @@ def dequantize_per_group_int8_nd(
     if ng == 0:
         return y
     L = _abi.lib()
-    with _abi.on_device(q.device):
+    with _abi.on_device(q.device), _abi.workspace_lock(q.device):
         ws = _abi.workspace(q.device,
                             L.cbq_dequant_int8_group_nd_ws_bytes(outer, Lq, inner, group_size))
         rc = L.cbq_dequant_int8_group_nd(_abi.ptr(q), _abi.ptr(scale), outer, Lq, inner,

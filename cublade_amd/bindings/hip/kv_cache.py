@@ -208,7 +208,7 @@ def kv_attend(view: _abi.KvCache, dev: torch.device, q: torch.Tensor, page_table
         L = _abi.lib()
         by = ctypes.byref
         ml = max_length or 0
-        with _abi.on_device(dev):
+        with _abi.on_device(dev), _abi.workspace_lock(dev):
             ws = _abi.workspace(dev, L.cbq_kv_attend_ws_bytes(by(view), by(batch), hq, ml))
             rc = L.cbq_kv_attend(by(view), by(batch), _abi.DTYPE_CODE[q.dtype], by(cq), hq,
                                  1.0 / math.sqrt(d) if scale is None else float(scale), bool(causal),

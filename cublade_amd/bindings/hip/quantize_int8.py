@@ -35,7 +35,7 @@ def quantize_per_tensor_int8(
         return q, torch.zeros((), dtype=torch.float32, device=dev)
     scale = torch.empty((), dtype=torch.float32, device=dev)
     L = _abi.lib()
-    with _abi.on_device(dev):
+    with _abi.on_device(dev), _abi.workspace_lock(dev):
         ws = _abi.workspace(dev, L.cbq_quant_tensor_ws_bytes())
         watch = watch_exchange(dev)
         rc = L.cbq_quant_int8_tensor(_abi.ptr(x), code, n, float(eps), _abi.ptr(ws), ws.numel(),
@@ -75,7 +75,7 @@ def quantize_per_channel_int8(
         return q, torch.zeros((nscale,), dtype=torch.float32, device=dev)
     scale = torch.empty((nscale,), dtype=torch.float32, device=dev)
     L = _abi.lib()
-    with _abi.on_device(dev):
+    with _abi.on_device(dev), _abi.workspace_lock(dev):
         ws = _abi.workspace(dev, L.cbq_quant_int8_channel_ws_bytes(C, F, axis))
         rc = L.cbq_quant_int8_channel(_abi.ptr(x), code, C, F, axis, float(eps), _abi.ptr(ws),
                                       ws.numel(), _abi.ptr(q), _abi.ptr(scale),
@@ -166,7 +166,7 @@ def quantize_per_channel_int8_nd(
         return q, torch.zeros((C,), dtype=torch.float32, device=dev)
     scale = torch.empty((C,), dtype=torch.float32, device=dev)
     L = _abi.lib()
-    with _abi.on_device(dev):
+    with _abi.on_device(dev), _abi.workspace_lock(dev):
         ws = _abi.workspace(dev, L.cbq_quant_int8_channel_nd_ws_bytes(outer, C, inner))
         rc = L.cbq_quant_int8_channel_nd(_abi.ptr(x), code, outer, C, inner, float(eps),
                                          _abi.ptr(ws), ws.numel(), _abi.ptr(q), _abi.ptr(scale),
@@ -202,7 +202,7 @@ def quantize_per_group_int8_nd(
     if ng == 0:
         return q, scale
     L = _abi.lib()
-    with _abi.on_device(dev):
+    with _abi.on_device(dev), _abi.workspace_lock(dev):
         ws = _abi.workspace(dev, L.cbq_quant_int8_group_nd_ws_bytes(outer, Lx, inner, group_size))
         rc = L.cbq_quant_int8_group_nd(_abi.ptr(x), code, outer, Lx, inner, group_size,
                                        float(eps), _abi.ptr(ws), ws.numel(), _abi.ptr(q),

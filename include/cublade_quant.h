@@ -65,7 +65,9 @@ enum { CBQ_OK = 0, CBQ_EINVAL = 1, CBQ_ELAUNCH = 2 };
  * status word (a wait gave up: the call was slow, not wrong). The other
  * entry points leave the control block alone. The rest is per-call scratch. One
  * workspace serves one stream at a time: calls that overlap in time must not
- * share it. */
+ * share it. A call may queue several kernels that pass data through its
+ * workspace: host threads that use one workspace on one stream take turns,
+ * one call at a time (until it returns; it need not have run). */
 #define CBQ_WS_CTRL_BYTES 16384
 
 /* Message of the last failed call on this thread ("" if none). */
