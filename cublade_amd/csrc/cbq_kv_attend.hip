@@ -151,6 +151,18 @@ __device__ __forceinline__ int64_t capacity(const KvAttendArg& a) {
   return c < INT32_MAX - 1024 ? c : INT32_MAX - 1024;
 }
 
+// A sequence's length as the kernels use it; bad: it has keys that no page can hold.
+struct KvLen {
+  int len;
+  bool bad;
+};
+
+__device__ __forceinline__ KvLen len_of(const KvAttendArg& a, const KvSeq& s) {
+  const int64_t cap = capacity(a);
+  const bool bad = s.len > cap;
+  return {static_cast<int>(s.len < 0 ? 0 : bad ? cap : s.len), bad};
+}
+
 __device__ __forceinline__ KeyRange keys_of(const KvAttendArg& a, int len, int n, int i) {
   KeyRange r;
   r.lo = 0;
@@ -164,17 +176,17 @@ __device__ __forceinline__ KeyRange keys_of(const KvAttendArg& a, int len, int n
 }
 
 // Writes 4 outputs of one row: finished ones, or the partial row `prow` of a
-// split of the keys.
+// split of the keys. none: the row sees no key. (Its maximum and sum do not tell:
+// scores that are all -infinity leave both as they began, and their softmax is NaN,
+// as o / l = 0 / 0 is here.)
 __device__ __forceinline__ void put_row(const KvAttendArg& a, int64_t row, int64_t prow, int split,
-                                        int d0, f4 o, float m, float l, bool bad) {
+                                        int d0, f4 o, float m, float l, bool none, bool bad) {
   if (a.splits > 1) {
     const int64_t at = split * a.prows + prow;
     *reinterpret_cast<f4*>(a.po + at * a.d + d0) = o;
     if (d0 == 0) a.pml[at] = bad ? make_float2(0.0f, __builtin_nanf("")) : make_float2(m, l);
     return;
   }
-  // (scores that are all NaN raise no maximum either; their sum is NaN)
-  const bool none = m == kNegInf && l == 0.0f;
   float inv = none ? 0.0f : 1.0f / l;
   if (bad) inv = __builtin_nanf("");
   const float f[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
@@ -301,9 +313,7 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
   if (tl.b < 0) return;
   const int b = tl.b;
   const KvSeq s = tl.s;
-  const int64_t cap = capacity(a);
-  const bool bad = s.len > cap;      // keys that no page can hold
-  const int len = static_cast<int>(s.len < 0 ? 0 : bad ? cap : s.len);
+  const auto [len, bad] = len_of(a, s);
   const int rows = tl.rows, r_first = tl.r_first, n = static_cast<int>(s.n);
   const int r_last = r_first + kRowTile - 1 < rows ? r_first + kRowTile - 1 : rows - 1;
   const int r = r_first + n16;
@@ -516,13 +526,15 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
     f[w] = sml[w][row][0] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(sml[w][row][0] - mm);
     ll += sml[w][row][1] * f[w];
   }
+  const KeyRange seen = keys_of(a, len, n, rr / a.rep);
   const int64_t tok = s.tok0 + rr / a.rep;
   const int64_t orow = tok * a.hq + h * a.rep + rr % a.rep;
   for (int d0 = 4 * (threadIdx.x & 15); d0 < d; d0 += 64) {
     f4 v = {};
 #pragma unroll
     for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f4*>(&so[w][row][d0]) * f[w];
-    put_row(a, orow, static_cast<int64_t>(item * a.hkv + h) * kRowTile + row, split, d0, v, mm, ll, bad);
+    put_row(a, orow, static_cast<int64_t>(item * a.hkv + h) * kRowTile + row, split, d0, v, mm, ll,
+            seen.hi <= seen.lo, bad);
   }
 }
 
@@ -573,9 +585,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_kv_attend_long(c
   const KvTile tl = tile_of(a, item);
   if (tl.b < 0) return;
   const KvSeq s = tl.s;
-  const int64_t cap = capacity(a);
-  const bool bad = s.len > cap;
-  const int len = static_cast<int>(s.len < 0 ? 0 : bad ? cap : s.len);
+  const auto [len, bad] = len_of(a, s);
   const int rows = tl.rows, r_first = tl.r_first, n = static_cast<int>(s.n);
   const int r_last = r_first + kLongTile - 1 < rows ? r_first + kLongTile - 1 : rows - 1;
   const int all_hi = keys_of(a, len, n, r_last / a.rep).hi;
@@ -836,7 +846,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_kv_attend_long(c
       const int d0 = 32 * t + 8 * q + 4 * hf;
       if (EXACT || d0 < d)
         put_row(a, orow, static_cast<int64_t>(item * a.hkv + h) * kLongTile + wave * 32 + n32, split, d0,
-                f4{o[t][4 * q], o[t][4 * q + 1], o[t][4 * q + 2], o[t][4 * q + 3]}, m, sum, bad);
+                f4{o[t][4 * q], o[t][4 * q + 1], o[t][4 * q + 2], o[t][4 * q + 3]}, m, sum,
+                mine.hi <= mine.lo, bad);
     }
 }
 
@@ -899,9 +910,11 @@ __global__ __launch_bounds__(kBlock) void k_kv_attend_join(const KvAttendArg a) 
   }
   const int ti = (tl.r_first + row) / a.rep;
   const int64_t orow = (tl.s.tok0 + ti) * a.hq + h * a.rep + (tl.r_first + row - ti * a.rep);
+  const auto [len, bad] = len_of(a, tl.s);
+  const KeyRange seen = keys_of(a, len, static_cast<int>(tl.s.n), ti);
   KvAttendArg one = a;
   one.splits = 1;
-  if (4 * lane < a.d) put_row(one, orow, 0, 0, d0, acc, m, l, false);
+  if (4 * lane < a.d) put_row(one, orow, 0, 0, d0, acc, m, l, seen.hi <= seen.lo, bad);
 }
 
 // What one call launches: k_kv_attend_rows for the sequences of few rows,

@@ -169,7 +169,7 @@ def attend_kv(
 
     Returns [tokens, q_heads, head_dim] in q's dtype (and the log-sum-exp): fp32
     sums, one final rounding. A query that sees no token gives zeros, and
-    -infinity.
+    -infinity (one whose scores are all -infinity NaN, and -infinity).
     """
     return kv_attend(cache._view, cache.k.device, q, page_table, lengths, cu_q, scale, causal,
                      window, max_length, return_lse)

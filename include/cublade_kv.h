@@ -112,7 +112,8 @@ int cbq_kv_dequant(const cbq_kv_cache* cache, const int32_t* pages, int64_t n, v
  * Query head h reads kv head h / (q_heads / kv_heads). Query i of the n of a
  * sequence of length len has position p = len - n + i and sees the keys j <= p
  * if causal, else all j < len; with window > 0 (causal only) those with
- * j > p - window. A query that sees no key gives o = 0, lse = -infinity.
+ * j > p - window. A query that sees no key gives o = 0, lse = -infinity; one
+ * whose scores are all -infinity gives the NaN of their softmax, lse = -infinity.
  * Probabilities and sums in fp32; probabilities are rounded to fp16 for the
  * product with the codes.
  * out: [tokens, q_heads, head_dim] in dtype, contiguous, 16-byte aligned.
