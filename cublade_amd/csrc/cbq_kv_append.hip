@@ -408,14 +408,14 @@ __device__ __forceinline__ void turn_queries(const KvAppendArg& a, int wave) {
         o1[k] = turned ? f[k] * c[k] - g[k] * sn[k] : f[k];
         o2[k] = turned ? g[k] * c[k] + f[k] * sn[k] : g[k];
       }
-      *reinterpret_cast<uint4*>(out + (h * a.d + d0) * 2) = pack8_out<DT>(o1);
-      *reinterpret_cast<uint4*>(out + (h * a.d + d1) * 2) = pack8_out<DT>(o2);
+      *reinterpret_cast<uint4*>(out + (static_cast<int64_t>(h) * a.d + d0) * 2) = pack8_out<DT>(o1);
+      *reinterpret_cast<uint4*>(out + (static_cast<int64_t>(h) * a.d + d1) * 2) = pack8_out<DT>(o2);
     }
   } else {
     for (int h = h0; h < a.hq; h += hstep) {
       float f[8];
       turned8<DT>(x + h * a.q.hs, 8 * unit, pos, a.rope, f);
-      *reinterpret_cast<uint4*>(out + (h * a.d + 8 * unit) * 2) = pack8_out<DT>(f);
+      *reinterpret_cast<uint4*>(out + (static_cast<int64_t>(h) * a.d + 8 * unit) * 2) = pack8_out<DT>(f);
     }
   }
 }

@@ -58,3 +58,28 @@ def test_rows_of_infinite_scores_are_nan(n, new, store, dt, sign):
     for x in (o, lse):
         assert bool(x[:first, 0].isfinite().all()) and bool(x[first:-1].isfinite().all())
     assert bool((o[-1] == 0).all()) and bool((lse[-1] == -math.inf).all())
+
+
+@pytest.mark.parametrize("style", ["none", "half", "interleaved"])
+def test_queries_past_2_gib_of_a_token(style):
+    """A token's rotated queries of more than 2^31 bytes: the last heads are
+    written where they belong."""
+    from cublade_amd.quantization import QuantizedKVCache, append_kv
+    d, hq = 256, (1 << 22) + 64
+    cache = QuantizedKVCache.empty(1, 1, d, 16)
+    g = _gen(52)
+    q = torch.empty(1, hq, d, dtype=F16, device=DEV)
+    q.view(torch.int16).random_(0, 0x7C00, generator=g)     # finite numbers
+    k = torch.ones(1, 1, d, device=DEV).half()
+    cos, sin = (t[5:6].contiguous() for t in _kv.tables(6, d))
+    positions = torch.zeros(1, dtype=torch.int64, device=DEV)
+    kw = {} if style == "none" else dict(rope=(cos, sin), interleaved=style == "interleaved",
+                                         positions=positions)
+    out = append_kv(cache, k, k, _i32([[0]]), _i32([1]), q=q, **kw)
+    for part in (slice(0, 64), slice(hq // 2, hq // 2 + 64), slice(hq - 128, hq)):
+        want = q[:, part]
+        if kw:
+            want = _kv.rotate_f32(want, positions, cos, sin, style == "interleaved").half()
+        assert torch.equal(out[:, part], want)
+    if style == "none":
+        assert torch.equal(out, q)
