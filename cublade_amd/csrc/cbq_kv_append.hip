@@ -647,6 +647,7 @@ extern "C" int cbq_kv_append(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   if (int rc = kv_check_batch(batch)) return rc;
   CBQ_REQUIRE(dtype == CBQ_F16 || dtype == CBQ_BF16, "kv append: dtype must be fp16 or bf16, got %d",
               dtype);
+  CBQ_REQUIRE(q_heads >= 0, "kv append: q_heads must not be negative, got %d", q_heads);
   const bool has_q = q != nullptr && q->data != nullptr && q_heads > 0;
   KvRopeArg r = {};
   if (rope != nullptr && rope->rot_dim != 0) {
