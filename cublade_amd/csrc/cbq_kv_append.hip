@@ -369,10 +369,12 @@ __device__ __forceinline__ void turn_queries(const KvAppendArg& a, int wave) {
   if (a.m.cu == nullptr) {
     at = static_cast<int64_t>(a.m.lengths[tok]) - 1;
   } else {
-    // The token's sequence, by the tokens that each one brings.
+    // The token's sequence, by the tokens that each one brings. (One in front of the
+    // first sequence's or behind the last's has no position.)
     int rel = 0;
-    const int b = kv_find(a.m, tok - (a.m.cu[0] > 0 ? a.m.cu[0] : 0), rel,
-                          [](const KvSeq& s) { return static_cast<int>(s.n); });
+    const int t0 = a.m.cu[0] > 0 ? a.m.cu[0] : 0;
+    const int b = tok < t0 ? -1 : kv_find(a.m, tok - t0, rel,
+                                          [](const KvSeq& s) { return static_cast<int>(s.n); });
     if (b >= 0) {
       const KvSeq s = kv_seq(a.m, b);
       at = s.len - s.n + rel;

@@ -74,6 +74,7 @@ struct KvAttendArg {
   int window;              // 0: none
   int tile_rows;           // query rows of a workgroup
   int items;               // row tiles of this launch, at most
+  uint32_t tiles;          // workgroups of them; those behind: put_rest
   int row_min, row_max;       // this launch's sequences have row_min .. row_max rows
 };
 
@@ -198,6 +199,28 @@ __device__ __forceinline__ void put_row(const KvAttendArg& a, int64_t row, int64
     a.lse[row] = bad ? __builtin_nanf("") : none ? kNegInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
+// Outputs of the tokens that belong to no sequence, [0, cu[0]) and [cu[batch],
+// tokens): zeros, log-sum-exp -infinity, as of rows that see no key. By the
+// workgroups behind those of the tiles, which find nothing to do in most calls (a
+// padded batch replayed from a graph has such tokens). Drafted tokens take 0.3 us
+// more for it (40.7), prompts no more; a launch of its own took 2 us. (Where each
+// kernel branches to it was chosen by its time: the other way is 0.4 us slower in
+// k_kv_attend_rows and 2 of 78 us in a mixed batch.)
+__device__ __forceinline__ void put_rest(const KvAttendArg& a) {
+  int64_t lo = a.m.cu[0], hi = a.m.cu[a.m.batch];
+  lo = lo < 0 ? 0 : lo > a.m.tokens ? a.m.tokens : lo;
+  hi = hi < lo ? lo : hi > a.m.tokens ? a.m.tokens : hi;
+  const int64_t first = static_cast<int64_t>(blockIdx.x - a.tiles) * blockDim.x + threadIdx.x;
+  const int64_t step = static_cast<int64_t>(gridDim.x - a.tiles) * blockDim.x;
+  const int64_t rest = a.m.tokens - (hi - lo);
+  auto each = [&](int64_t per, auto put) {     // per: elements of a token
+    for (int64_t i = first; i < rest * per; i += step) put(i < lo * per ? i : i + (hi - lo) * per);
+  };
+  each(static_cast<int64_t>(a.hq) * a.d / 8,
+       [&](int64_t i) { reinterpret_cast<uint4*>(a.out)[i] = make_uint4(0, 0, 0, 0); });
+  if (a.lse != nullptr) each(a.hq, [&](int64_t i) { a.lse[i] = kNegInf; });
+}
+
 // One row's queries as fp16 operands, N pieces of 8 dimensions (piece k from
 // dim(k)), and the factor cq of its scores. bf16 queries are scaled to fp16 by a
 // power of two per row (row_max: the maximum over the lanes that share the row);
@@ -309,8 +332,11 @@ __global__ __launch_bounds__(kBlock, DP <= 128 ? 2 : 1) void k_kv_attend_rows(co
   const int rest = blockIdx.x / a.splits;
   const int h = rest % a.hkv;
   const int item = rest / a.hkv;
-  const KvTile tl = tile_of(a, item);
-  if (tl.b < 0) return;
+  const KvTile tl = tile_of(a, item < a.items ? item : INT32_MAX);
+  if (tl.b < 0) {
+    if (item >= a.items) put_rest(a);
+    return;
+  }
   const int b = tl.b;
   const KvSeq s = tl.s;
   const auto [len, bad] = len_of(a, s);
@@ -578,6 +604,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void k_kv_attend_long(c
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n32 = lane & 31, hf = lane >> 5;
 
+  if (blockIdx.x >= a.tiles) return put_rest(a);
   const int h = blockIdx.x % a.hkv;
   const int rest = blockIdx.x / a.hkv;
   const int split = rest % a.splits;
@@ -942,6 +969,8 @@ constexpr int64_t kSharedKeys = 1024;
 // (head size 128); with 4 a batch of mixed lengths takes 113 instead of 126 us (64
 // sequences of 100 to 8000 tokens), one sequence the same.
 constexpr int64_t kRowWgs = 4;
+// Workgroups for the tokens of no sequence, in calls with offsets.
+constexpr int64_t kRestWgs = 16;
 
 int padded_dim(int d) { return (d + 63) / 64 * 64; }
 
@@ -1066,6 +1095,7 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
   hipStream_t st = as_stream(stream);
   // One launch over `items` tiles of `tile` rows, the keys in `splits` ranges (as
   // many as the workspace has room for), and the launch that joins them.
+  int64_t rest_wgs = batch->cu != nullptr ? kRestWgs : 0;     // in the first launch
   auto run = [&](int64_t items, int tile, int splits, int dim, auto kernel) -> int {
     const size_t each = partial_bytes(cache, items, tile);
     splits = std::max(1, static_cast<int>(std::min<size_t>(splits, room / each)));
@@ -1082,9 +1112,11 @@ extern "C" int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batc
     const int64_t blocks = items * a.hkv * splits;
     const bool wide = splits > 8;
     const int64_t joins = items * a.hkv * (wide ? tile : tile / 4);
-    CBQ_REQUIRE(blocks < (int64_t{1} << 31) && joins < (int64_t{1} << 31),
+    CBQ_REQUIRE(blocks < (int64_t{1} << 31) - kRestWgs && joins < (int64_t{1} << 31),
                 "kv attend: too many tokens for one call");
-    const dim3 grid(static_cast<uint32_t>(blocks));
+    a.tiles = static_cast<uint32_t>(blocks);
+    const dim3 grid(static_cast<uint32_t>(blocks + rest_wgs));
+    rest_wgs = 0;
     auto by_dim = [&](auto stc) {
       switch (dim) {
         case 64: kernel(grid, stc, std::integral_constant<int, 64>{}); break;

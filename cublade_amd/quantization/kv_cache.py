@@ -117,8 +117,11 @@ def append_kv(
             multiples of 8 elements, as in a fused projection's output).
         page_table: int32 [batch, max_pages], the page ids of every sequence.
         lengths: int32 [batch], tokens of every sequence with the new ones.
-        cu_new: int32 [batch + 1], where each sequence's new tokens begin among
-            `tokens`, 0 first and `tokens` last; None: one new token each.
+        cu_new: int32 [batch + 1], not decreasing: where each sequence's new
+            tokens begin among `tokens`, and where the last one's end; None:
+            one new token each. Tokens in front of them and behind them (a batch
+            padded to a fixed size) are not appended; their queries are NaN
+            where they would be rotated, unless `positions` are given.
         rope: (cos, sin), float32 [rows, rot_dim / 2]: k and q are rotated by
             the row of the token's position, dimensions i and i + rot_dim / 2
             as a pair (2 i and 2 i + 1 if `interleaved`), dimensions from
@@ -157,7 +160,8 @@ def attend_kv(
         q: [tokens, q_heads, head_dim], fp16 or bf16; q_heads a multiple of
             kv_heads (query head h reads kv head h // (q_heads // kv_heads)).
         page_table, lengths: as given to append_kv; cu_q: as its cu_new. The n
-            queries of a sequence are its last n tokens.
+            queries of a sequence are its last n tokens. A query outside cu_q
+            sees no token.
         scale: of the scores, 1 / sqrt(head_dim) by default.
         causal: a query sees its own token and earlier ones; else all of its
             sequence's.

@@ -51,6 +51,10 @@ typedef struct {
 /* The sequences of a call. lengths[b]: tokens of sequence b with the new ones.
  * cu: [batch + 1] offsets of each sequence's new tokens among the `tokens` new
  * tokens of the call, or null: one new token per sequence (tokens == batch).
+ * They do not decrease. Tokens in front of cu[0] and from cu[batch] on belong to
+ * no sequence (a call padded to a fixed size): they are not appended, their
+ * rotated queries are NaN (as they are, without rotation; turned, with
+ * positions), and their attention is that of a query that sees no key.
  * page_table: [batch, max_pages], rows table_stride elements apart. */
 typedef struct {
   const int32_t* page_table;

@@ -83,3 +83,101 @@ def test_queries_past_2_gib_of_a_token(style):
         assert torch.equal(out[:, part], want)
     if style == "none":
         assert torch.equal(out, q)
+
+
+def _poison(q):
+    """Leaves NaN in the allocator's next free block of q's size and its lse's."""
+    for shape, dt in ((q.shape, q.dtype), (q.shape[:2], torch.float32)):
+        t = torch.full(shape, math.nan, dtype=dt, device=DEV)
+        del t
+
+
+PADDED = [
+    # kv heads, heads of each, d, lens, news, tokens in front and behind, window
+    (2, 4, 64, [40, 90, 7], [1, 3, 0], 0, 5, None),
+    (2, 4, 64, [40, 90, 7], [1, 3, 0], 2, 0, None),
+    (1, 8, 128, [9000], [5], 3, 60, None),
+    (2, 4, 128, [300], [200], 1, 300, None),
+    (1, 2, 80, [400, 50, 9], [300, 1, 1], 7, 70, None),
+    (2, 4, 64, [400, 50, 9], [100, 1, 1], 7, 70, 40),
+    (1, 1, 256, [3, 2], [0, 0], 0, 4, None),
+]
+
+
+@pytest.mark.parametrize("store,dt", [(I8, BF16), (F8, F16)])
+@pytest.mark.parametrize("case", range(len(PADDED)))
+def test_tokens_of_no_sequence_are_zero(case, store, dt):
+    """Tokens in front of the first offset and behind the last (a batch padded
+    to a fixed size): zeros and -infinity, and the others as without them."""
+    from cublade_amd.quantization import attend_kv
+    hkv, rep, d, lens, news, front, behind, window = PADDED[case]
+    g = _gen(60 + case)
+    table, pages = _kv.make_table(lens, 32, g)
+    cache = _kv.random_cache(pages, hkv, d, 32, store, g)
+    t = sum(news)
+    q = torch.randn(front + t + behind, hkv * rep, d, generator=g, device=DEV).to(dt)
+    cu = _cu(news) + front
+    _poison(q)
+    o, lse = attend_kv(q, cache, table, _i32(lens), cu_q=cu, window=window, return_lse=True)
+    own = slice(front, front + t)
+    ref = _kv.attend_ref(q[own], cache, table, lens, news, window=window)
+    _kv.assert_attends((o[own], lse[own]), ref, dt, PADDED[case])
+    rest = torch.ones(q.shape[0], dtype=torch.bool, device=DEV)
+    rest[own] = False
+    assert bool((o[rest] == 0).all()) and bool((lse[rest] == -math.inf).all())
+
+
+def test_appended_queries_of_no_sequence_have_no_position():
+    """Queries in front of the first offset and behind the last: NaN where they
+    would be rotated, whatever stands at the sequences' positions; unless each
+    token's row is given."""
+    from cublade_amd.quantization import append_kv
+    g = _gen(70)
+    lens, news, front, behind = [40, 90], [3, 2], 2, 4
+    table, pages = _kv.make_table(lens, 16, g)
+    cache = _kv.random_cache(pages, 2, 64, 16, I8, g)
+    model = _kv.CacheModel(cache)
+    x = torch.randn(11, 2, 64, generator=g, device=DEV).half()
+    rope = _kv.tables(100, 32)
+    own = slice(front, front + 5)
+    pos = torch.tensor([37, 38, 39, 88, 89], device=DEV)
+    out = append_kv(cache, x, x, table, _i32(lens), cu_new=_cu(news) + front, rope=rope, q=x)
+    turned = _kv.rotate_f32(x[own], pos, *rope, False)
+    assert torch.equal(out[own], turned.half())
+    rest = [0, 1, 7, 8, 9, 10]
+    assert bool(out[rest][..., :32].isnan().all()) and torch.equal(out[rest][..., 32:], x[rest][..., 32:])
+    model.append(turned, x[own], table, lens, news)
+    model.assert_equal(cache)
+    every = torch.arange(11, device=DEV)
+    out = append_kv(cache, x, x, table, _i32(lens), cu_new=_cu(news) + front, rope=rope, q=x,
+                    positions=every)
+    assert torch.equal(out, _kv.rotate_f32(x, every, *rope, False).half())
+
+
+def test_padded_batch_replayed_from_a_graph():
+    """One captured call of a fixed number of tokens, replayed for batches that
+    bring fewer: each replay as the eager call, eager work between them."""
+    from cublade_amd.quantization import attend_kv
+    g = _gen(71)
+    lens = [500, 300, 40]
+    table, pages = _kv.make_table(lens, 16, g)
+    cache = _kv.random_cache(pages, 2, 64, 16, I8, g)
+    q = torch.randn(240, 8, 64, generator=g, device=DEV).bfloat16()
+    n, cu = _i32(lens), _cu([1, 1, 1])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        attend_kv(q, cache, table, n, cu_q=cu, return_lse=True)
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            o, lse = attend_kv(q, cache, table, n, cu_q=cu, return_lse=True)
+        for news in ([1, 1, 1], [200, 30, 10], [0, 0, 0], [1, 100, 1], [1, 1, 1]):
+            cu.copy_(_cu(news))
+            o.fill_(math.nan)
+            lse.fill_(math.nan)
+            graph.replay()
+            s.synchronize()
+            eager = attend_kv(q, cache, table, n, cu_q=cu, return_lse=True)
+            assert torch.equal(o, eager[0]) and torch.equal(lse, eager[1])
+            assert bool((o[sum(news):] == 0).all()) and bool(o[:sum(news)].isfinite().all())
