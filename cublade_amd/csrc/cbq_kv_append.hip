@@ -16,9 +16,10 @@
 //
 // Bound by bytes: the new keys, values and queries in, the queries and codes out.
 // Measured on MI355X, kernel times: 8192 tokens of 32 query and 8 kv heads of 128
-// (185 MB) 36.8 us, 5.0 TB/s, where a copy reaches 5.1; 256 single tokens of 32 and
-// 32 heads of 64 10 us (24 with a workgroup per head); one token 3 us. Reading 128
-// pages of 64 tokens of 8 heads of 128 back (50 MB) 9.8 us, 5.1 TB/s.
+// (185 MB) 36.8 us, 5.0 TB/s, where a copy reaches 5.1, but 64 with interleaved pairs
+// and 126 with a rot_dim that is no multiple of 16 (turned8 for each piece); 256 single
+// tokens of 32 and 32 heads of 64 10 us (24 with a workgroup per head); one token 3 us.
+// Reading 128 pages of 64 tokens of 8 heads of 128 back (50 MB) 9.8 us, 5.1 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -197,7 +198,10 @@ __device__ __forceinline__ PageScale settle(float amax, float s_old, bool begun)
 
 // The first `lo` tokens' codes of a page's head times `lower`, by `n` threads of
 // which this is number `i`; 16 codes at a time: of one token (keys) or 16 tokens of
-// one dimension (values, of which only the first `lo` change).
+// one dimension (values, of which only the first `lo` change). One load behind the
+// other's store, which shows where single tokens make every page grow: 64 tokens of 8
+// heads of 128 at the end of their pages 18 us (64 tokens a page) and 77 us (256)
+// instead of 4.
 template <int ST, bool VALUES>
 __device__ void lower_codes(uint8_t* codes, int lo, int page, int d, float lower, int i, int n) {
   if constexpr (VALUES) {

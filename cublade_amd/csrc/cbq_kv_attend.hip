@@ -10,7 +10,8 @@
 // accumulators are ever multiplied by a scale. Codes are exact in fp16 (INT8
 // up to 127, E4M3 entirely), so both products run on the fp16 matrix cores
 // with fp32 sums and only the queries (bf16 ones are scaled to fp16 by a power
-// of two per row) and the weights are rounded.
+// of two per row) and the weights are rounded: by 2^-11 of each, and below fp16's
+// normal range by 2^-25 of the row's largest. The sum takes them before that.
 //
 // The matrix products compute S^T = K q^T and O^T = V^T w^T. In S^T's result
 // layout a lane holds 4 consecutive rows (keys) of one column (query row) per
@@ -954,16 +955,23 @@ struct KvPlan {
 };
 
 // Sequences of at most this many rows go to k_kv_attend_rows, and all of them
-// where a sequence has at most kFewRows on average: a second launch then costs
-// more than it could save.
+// where a sequence has at most kFewRows on average, which spares drafted tokens a
+// second launch. The mean does not tell of one long sequence among single tokens:
+// 255 of those and a chunk of 512, 64 heads over 8 of 128, 8192 keys, take 1045 us in
+// this one launch, where the two kernels in calls of their own take 643 and 180 (over
+// 2048 keys with 32 heads 228, 166 and 47).
 constexpr int64_t kShortRows = 64;
 constexpr int64_t kFewRows = 32;
 // Where a window leaves every row at most this many keys, and the sequences make at
 // most a tile per CU, k_kv_attend_long takes all rows in one launch: a single token's
-// tile is then no longer than a prompt's. (A batch of 5 prompts and 15 single tokens
-// over 1024 keys 82 instead of 96 us; 1 and 4 of 128 over 256 keys 44 and 54. Beyond,
-// splitting the single tokens' keys is worth more: over 2048 keys beside short
-// prompts 62 and 40 us in one launch and two, with 496 tiles 88 and 80.)
+// tile is then no longer than a prompt's. Measured in one launch and in two, windows
+// of 256 / 1024 / 2048 keys, one prompt for every three single tokens:
+//   20 sequences, prompts of up to 1500, 4 kv heads of 80   37 / 78 / 131, 49 / 91 / 141 us
+//   20, prompts of up to 300, 4 kv heads of 128             40 / 51 / 67,  45 / 56 / 71
+//    5, prompts of up to 1500, 4 kv heads of 128            25 / 50 / 82,  38 / 62 / 94
+//   32, prompts of up to 600, 8 kv heads of 64              28 / 60 / 101, 28 / 51 / 80
+// so what decides is how far the tiles fill the GPU rather than the window: the last,
+// with a tile per CU of single tokens alone, loses from 512 keys on.
 constexpr int64_t kSharedKeys = 1024;
 // Workgroups per CU that the keys of few tiles are split for. 2 fit at once
 // (head size 128); with 4 a batch of mixed lengths takes 113 instead of 126 us (64

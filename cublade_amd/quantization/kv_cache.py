@@ -136,6 +136,7 @@ def append_kv(
     page id is outside the pool, or whose position is outside the table, is
     dropped (attending to such a page gives NaN); one without a row in the
     rotation tables makes its query, and whatever attends to its page, NaN.
+    Neither the cache nor the result carries a gradient.
     """
     return kv_append(cache._view, cache.k.device, k, v, page_table, lengths, cu_new, rope,
                      interleaved, positions, q)
@@ -171,9 +172,19 @@ def attend_kv(
         return_lse: also return the log-sum-exp of the scores, float32
             [tokens, q_heads].
 
-    Returns [tokens, q_heads, head_dim] in q's dtype (and the log-sum-exp): fp32
-    sums, one final rounding. A query that sees no token gives zeros, and
-    -infinity (one whose scores are all -infinity NaN, and -infinity).
+    Returns [tokens, q_heads, head_dim] in q's dtype (and the log-sum-exp). A
+    query that sees no token gives zeros, and -infinity (one whose scores are all
+    -infinity NaN, and -infinity). The result carries no gradient.
+
+    Scores, softmax statistics and sums are fp32, and the codes exact; fewer bits
+    are kept in two places. Probabilities are rounded to fp16 for their product
+    with the values (the sum that divides it takes them before that): 2^-11 of
+    each, and 2^-25 of the largest product of a probability and its page's value
+    scale, so a page's values lose bits where they are far below another page's.
+    bf16 queries are fp16 numbers times a power of two for each row, so elements
+    below 2^-25 of their row's largest vanish. Where value scales that a query
+    sees lie more than 2^100 apart (fp16 values never do; scales below 2^-64
+    count as 2^-64), the pages of the smallest ones may be left out of the sum.
     """
     return kv_attend(cache._view, cache.k.device, q, page_table, lengths, cu_q, scale, causal,
                      window, max_length, return_lse)

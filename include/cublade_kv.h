@@ -107,7 +107,7 @@ int cbq_kv_append(const cbq_kv_cache* cache, const cbq_kv_batch* batch, int dtyp
 
 /* Reads pages back: k_out, v_out [n, kv_heads, page_size, head_dim] in
  * out_dtype (CBQ_F16 / CBQ_BF16), contiguous, 16-byte aligned: T(float(code) *
- * scale). pages: n int32 page ids. */
+ * scale). pages: n int32 page ids. A cache without pages is refused (n > 0). */
 int cbq_kv_dequant(const cbq_kv_cache* cache, const int32_t* pages, int64_t n, void* k_out,
                    void* v_out, int out_dtype, cbq_stream_t stream);
 
@@ -118,8 +118,13 @@ int cbq_kv_dequant(const cbq_kv_cache* cache, const int32_t* pages, int64_t n, v
  * if causal, else all j < len; with window > 0 (causal only) those with
  * j > p - window. A query that sees no key gives o = 0, lse = -infinity; one
  * whose scores are all -infinity gives the NaN of their softmax, lse = -infinity.
- * Probabilities and sums in fp32; probabilities are rounded to fp16 for the
- * product with the codes.
+ * Scores, statistics and sums in fp32. Probabilities are rounded to fp16 for the
+ * product with the codes (not for their sum): 2^-11 of each, and 2^-25 of the
+ * row's largest product of a probability and its page's value scale. bf16 queries
+ * become fp16 under a power of two per row (elements below 2^-25 of the row's
+ * largest vanish). Value scales that a row sees should lie within 2^100 of the
+ * largest (those below 2^-64 count as 2^-64; fp16 values never lie further):
+ * pages with smaller ones may be left out of the sum.
  * out: [tokens, q_heads, head_dim] in dtype, contiguous, 16-byte aligned.
  * lse: [tokens, q_heads] fp32 or null. max_length: an upper bound of lengths
  * that the host knows (0: none); only the split of the work depends on it.
