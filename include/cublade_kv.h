@@ -130,7 +130,9 @@ int cbq_kv_dequant(const cbq_kv_cache* cache, const int32_t* pages, int64_t n, v
  * that the host knows (0: none); only the split of the work depends on it.
  * ws: cbq_kv_attend_ws_bytes(...) bytes, 256-byte aligned (only its part
  * after the control block is used); a smaller one selects fewer splits of the
- * keys (same results within the order of fp32 sums, slower). */
+ * keys (same results within the order of fp32 sums, slower). Partial rows pass
+ * through ws from one kernel of a call to the next: host threads that share a ws
+ * on a stream make their calls one at a time. */
 size_t cbq_kv_attend_ws_bytes(const cbq_kv_cache* cache, const cbq_kv_batch* batch,
                               int32_t q_heads, int64_t max_length);
 int cbq_kv_attend(const cbq_kv_cache* cache, const cbq_kv_batch* batch, int dtype,
