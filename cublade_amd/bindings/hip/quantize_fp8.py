@@ -41,7 +41,7 @@ def quantize_per_tensor_fp8(
         watch = watch_exchange(dev)
         rc = L.cbq_quant_fp8_tensor(_abi.ptr(x), code, n, float(eps), _abi.ptr(ws), ws.numel(),
                                     _abi.ptr(q), _abi.ptr(scale), _abi.stream_handle(dev))
-    _abi.check(rc, "quantize_per_tensor_fp8")
-    if watch:
-        check_exchange(dev, "quantize_per_tensor_fp8")
+        _abi.check(rc, "quantize_per_tensor_fp8")
+        if watch:
+            check_exchange(dev, "quantize_per_tensor_fp8")
     return q, scale

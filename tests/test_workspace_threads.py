@@ -119,3 +119,20 @@ def test_two_threads_on_one_stream():
     for i in range(2):
         assert len(got[i]) == 200
         assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+def test_the_watched_status_is_read_under_the_lock():
+    """With CUBLADE_CHECK_EXCHANGE=1 a call clears its workspace's status word,
+    runs, and reads the word: another thread's call in between would clear what
+    this one has to report."""
+    found = 0
+    for path in sorted(BINDINGS.glob("quantize_*.py")):
+        tree = ast.parse(path.read_text())
+        held = [n for node in ast.walk(tree) if isinstance(node, ast.With)
+                and any(_attribute_calls(i.context_expr, "workspace_lock") for i in node.items)
+                for s in node.body for n in ast.walk(s)]
+        for call in [n for n in ast.walk(tree) if isinstance(n, ast.Call) and isinstance(n.func, ast.Name)
+                     and n.func.id in ("watch_exchange", "check_exchange")]:
+            assert call in held, f"{path.name}:{call.lineno}"
+            found += 1
+    assert found == 4
