@@ -28,6 +28,9 @@ SOURCES = [
     CSRC / "cbq_gemm.hip",
     CSRC / "cbq_kv_append.hip",
     CSRC / "cbq_kv_attend.hip",
+    CSRC / "cbq_w8a8.hip",
+    CSRC / "cbq_w8a8_few.hip",
+    CSRC / "cbq_norm.hip",
 ]
 
 WS_CTRL_BYTES = 16384
@@ -44,7 +47,7 @@ _P, _I64, _I32, _F, _SZ = (ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes
                            ctypes.c_size_t)
 
 # name -> (restype, argtypes); must match include/cublade_quant.h (KV_SIGNATURES:
-# include/cublade_kv.h).
+# include/cublade_kv.h, W8A8_SIGNATURES: include/cublade_w8a8.h).
 SIGNATURES = {
     "cbq_last_error": (ctypes.c_char_p, []),
     "cbq_abi_version": (_I32, []),
@@ -110,6 +113,36 @@ KV_SIGNATURES = {
     "cbq_kv_attend": (_I32, [_P, _P, _I32, _P, _I32, _F, _I32, _I64, _I64, _P, _SZ, _P, _P, _P]),
 }
 
+# include/cublade_w8a8.h: INT8 x INT8 products, and the norms around a block.
+ACT_CODE = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
+
+
+class I8Rows(ctypes.Structure):
+    _fields_ = [("data", _P), ("stride", _I64), ("scale", _P), ("scale_stride", _I64)]
+
+
+NORM_CODE = {"rms": 0, "layer": 1}
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = [("tokens", _I64), ("hidden", _I64), ("x", _P), ("x_stride", _I64), ("residual", _P),
+                ("residual_stride", _I64), ("gate", _P), ("gate_token_stride", _I64),
+                ("gate_channel_stride", _I64), ("post_weight", _P), ("post_bias", _P),
+                ("weight", _P), ("bias", _P), ("h", _P), ("out", _P), ("scale", _P),
+                ("x_dtype", ctypes.c_int32), ("residual_dtype", ctypes.c_int32),
+                ("param_dtype", ctypes.c_int32), ("gate_dtype", ctypes.c_int32),
+                ("out_dtype", ctypes.c_int32), ("kind", ctypes.c_int32), ("post", ctypes.c_int32),
+                ("eps", _F), ("alpha", _F)]
+
+
+W8A8_SIGNATURES = {
+    "cbq_w8a8_ws_bytes": (_SZ, [_I64, _I64, _I64, _I32]),
+    "cbq_w8a8_linear": (_I32, [_P, _P, _P, _I32, _I64, _I64, _I64, _P, _I32, _P, _SZ, _P]),
+    "cbq_w8a8_gated": (_I32, [_P, _P, _P, _P, _P, _I32, _I32, _I64, _I64, _I64, _P, _I32, _P, _SZ,
+                              _P]),
+    "cbq_norm": (_I32, [_P, _P]),
+}
+
 _lib = None
 _lib_lock = threading.Lock()
 
@@ -128,7 +161,7 @@ def lib() -> ctypes.CDLL:
                     raise RuntimeError(
                         f"cublade: {LIB_NAME} has ABI version {ver}, these bindings need major "
                         f"version {ABI_MAJOR} (rebuild the library)")
-                for name, (res, args) in {**SIGNATURES, **KV_SIGNATURES}.items():
+                for name, (res, args) in {**SIGNATURES, **KV_SIGNATURES, **W8A8_SIGNATURES}.items():
                     fn = getattr(L, name)
                     fn.restype = res
                     fn.argtypes = args

@@ -1,0 +1,122 @@
+"""Products of INT8 activations and INT8 weights on the HIP C ABI
+(include/cublade_w8a8.h). No counterpart in the reference."""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from ... import _abi
+
+_MAX_STRIDE = 1 << 22      # bytes between rows that the kernels take
+
+
+def _rows(codes: torch.Tensor, scale: torch.Tensor, dev: torch.device, k: int | None, name: str):
+    """(I8Rows, the tensors it points to): codes as they are where the kernels
+    can read their rows, else a contiguous copy."""
+    if codes.dtype != torch.int8 or codes.dim() != 2 or (k is not None and codes.size(1) != k):
+        raise RuntimeError(f"{name} must be int8 [rows, {'columns' if k is None else k}], got "
+                           f"{tuple(codes.shape)} {codes.dtype}")
+    if codes.device != dev or scale.device != dev:
+        raise RuntimeError(f"{name} and its scales must be on {dev}, got {codes.device} and "
+                           f"{scale.device}")
+    if scale.dtype != torch.float32:
+        raise RuntimeError(f"{name} must have torch.float32 scales, got {scale.dtype}")
+    rows, cols = codes.shape
+    step = 1
+    if scale.dim() == 0:
+        step = 0
+    elif scale.dim() != 1 or scale.numel() != rows:
+        raise RuntimeError(f"{name} must have one scale for each of its {rows} rows, or a 0-d one "
+                           f"for all, got {tuple(scale.shape)}")
+    elif not scale.is_contiguous():
+        scale = scale.contiguous()
+    stride, es = codes.stride()
+    if es != 1 or stride < cols or stride > _MAX_STRIDE or (
+            cols % 16 == 0 and (stride % 16 or codes.data_ptr() % 16)):
+        codes = codes.clone(memory_format=torch.contiguous_format)
+        stride = cols
+    return _abi.I8Rows(codes.data_ptr(), stride, scale.data_ptr(), step), codes, scale
+
+
+def _bias(b: torch.Tensor | None, n: int, dev: torch.device, name: str):
+    if b is None:
+        return None
+    if b.device != dev or b.dtype not in _abi.DTYPE_CODE or b.dim() != 1 or b.numel() != n:
+        raise RuntimeError(f"{name} must be [{n}] in float32, float16 or bfloat16 on {dev}, got "
+                           f"{tuple(b.shape)} {b.dtype} on {b.device}")
+    return b.detach().contiguous()
+
+
+def _out_code(dtype: torch.dtype) -> int:
+    code = _abi.DTYPE_CODE.get(dtype)
+    if code is None:
+        raise RuntimeError(f"out_dtype must be float32, float16 or bfloat16, got {dtype}")
+    return code
+
+
+def _check_cuda(x: torch.Tensor, what: str) -> None:
+    if not x.is_cuda:
+        raise RuntimeError(f"{what}: x must be on CUDA, got {x.device}")
+
+
+def w8a8_linear(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                bias: torch.Tensor | None, out_dtype: torch.dtype) -> torch.Tensor:
+    """y[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] + bias[n]; see
+    quantization.w8a8.linear_w8a8."""
+    _check_cuda(x, "w8a8_linear")
+    dev = x.device
+    cx, x, x_scale = _rows(x, x_scale, dev, None, "x")
+    m, k = x.shape
+    cw, w, w_scale = _rows(w, w_scale, dev, k, "weight")
+    n = w.size(0)
+    b = _bias(bias, n, dev, "bias")
+    code = _out_code(out_dtype)
+    y = torch.empty((m, n), dtype=out_dtype, device=dev)
+    if m == 0 or n == 0:
+        return y
+    L = _abi.lib()
+    with _abi.on_device(dev), _abi.workspace_lock(dev):
+        ws = _abi.workspace(dev, L.cbq_w8a8_ws_bytes(m, n, k, 1))
+        rc = L.cbq_w8a8_linear(ctypes.byref(cx), ctypes.byref(cw), _abi.ptr(b),
+                               0 if b is None else _abi.DTYPE_CODE[b.dtype], m, n, k, y.data_ptr(),
+                               code, ws.data_ptr(), ws.numel(), _abi.stream_handle(dev))
+    _abi.check(rc, "w8a8_linear")
+    return y
+
+
+def w8a8_gated(x: torch.Tensor, x_scale: torch.Tensor, gate: torch.Tensor,
+               gate_scale: torch.Tensor, up: torch.Tensor, up_scale: torch.Tensor,
+               activation: str, gate_bias: torch.Tensor | None, up_bias: torch.Tensor | None,
+               out_dtype: torch.dtype) -> torch.Tensor:
+    """act(x . gate^T + gate_bias) (x . up^T + up_bias); see
+    quantization.w8a8.gated_w8a8."""
+    _check_cuda(x, "w8a8_gated")
+    act = _abi.ACT_CODE.get(activation)
+    if act is None:
+        raise RuntimeError(f"activation must be one of {sorted(_abi.ACT_CODE)}, got {activation!r}")
+    dev = x.device
+    cx, x, x_scale = _rows(x, x_scale, dev, None, "x")
+    m, k = x.shape
+    cg, gate, gate_scale = _rows(gate, gate_scale, dev, k, "gate")
+    cu, up, up_scale = _rows(up, up_scale, dev, k, "up")
+    n = gate.size(0)
+    if up.size(0) != n:
+        raise RuntimeError(f"gate and up must have equally many rows, got {n} and {up.size(0)}")
+    gb, ub = _bias(gate_bias, n, dev, "gate_bias"), _bias(up_bias, n, dev, "up_bias")
+    if gb is not None and ub is not None and gb.dtype != ub.dtype:
+        raise RuntimeError(f"gate_bias and up_bias must have one dtype, got {gb.dtype} and {ub.dtype}")
+    code = _out_code(out_dtype)
+    y = torch.empty((m, n), dtype=out_dtype, device=dev)
+    if m == 0 or n == 0:
+        return y
+    some = gb if gb is not None else ub
+    L = _abi.lib()
+    with _abi.on_device(dev), _abi.workspace_lock(dev):
+        ws = _abi.workspace(dev, L.cbq_w8a8_ws_bytes(m, n, k, 2))
+        rc = L.cbq_w8a8_gated(ctypes.byref(cx), ctypes.byref(cg), ctypes.byref(cu), _abi.ptr(gb),
+                              _abi.ptr(ub), 0 if some is None else _abi.DTYPE_CODE[some.dtype], act,
+                              m, n, k, y.data_ptr(), code, ws.data_ptr(), ws.numel(),
+                              _abi.stream_handle(dev))
+    _abi.check(rc, "w8a8_gated")
+    return y

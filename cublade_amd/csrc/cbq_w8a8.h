@@ -1,0 +1,102 @@
+// cbq_w8a8.h - what the kernels of the INT8 x INT8 products share: their
+// arguments, the activations, and the step from an integer sum to an output.
+#pragma once
+
+#include "cbq_device.h"
+#include "cbq_host.h"
+#include "cublade_w8a8.h"
+
+namespace cbq {
+
+typedef int i4v __attribute__((ext_vector_type(4)));
+typedef int i16x __attribute__((ext_vector_type(16)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+
+// Activation of the gate; kNoAct: a single product (linear).
+enum : int { kNoAct = -1 };
+
+struct W8Args {
+  const uint8_t* x;        // [M] rows of K codes, ldx bytes apart
+  const uint8_t* w[2];     // [N] rows of K codes (gated: the gate's, the up projection's)
+  int64_t ldx, ldw[2];
+  const float* sx;         // scales: sx[m sx_step], sw[p][n sw_step[p]]
+  const float* sw[2];
+  int64_t sx_step, sw_step[2];
+  const void* bias[2];     // [N] in bias_dt, or null
+  int bias_dt;
+  int act;
+  void* y;                 // [M, N] in out_dt
+  int out_dt;
+  int vec;                 // y's rows may be stored 16 bytes at a time
+  int M, N, K;
+  int tiles_m, tiles_n;
+  int splits, split_steps; // K in ranges of split_steps 64-byte steps
+  int* part;               // sums of the ranges: [splits][projections][M][ldp]
+  int64_t ldp;
+};
+
+// act(g) in fp32. The sigmoids take the hardware's 2^x and reciprocal (1 ulp
+// each); the argument's rounding costs |g| 2^-24 of e^-g. act is uniform.
+__device__ __forceinline__ float sigmoid_of(float z) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));
+}
+
+template <int ACT>
+__device__ __forceinline__ float activate(float g) {
+  if constexpr (ACT == CBQ_ACT_SILU) return g * sigmoid_of(g);
+  // 1/2 (1 + tanh(u)) = sigmoid(2 u)
+  else if constexpr (ACT == CBQ_ACT_GELU_TANH)
+    return g * sigmoid_of(g * (1.59576912f + 0.0713548163f * (g * g)));
+  else if constexpr (ACT == CBQ_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.707106781f));
+  else if constexpr (ACT == CBQ_ACT_RELU) return g < 0.0f ? 0.0f : g;
+  else return g;
+}
+
+__device__ __forceinline__ float ld_any(const void* p, int dt, int64_t i) {
+  return dt == kF32 ? ld1<kF32>(p, i) : dt == kF16 ? ld1<kF16>(p, i) : ld1<kBF16>(p, i);
+}
+
+// An integer sum with its scales and bias.
+__device__ __forceinline__ float scaled(int sum, float sx, float sw, float b) {
+  return static_cast<float>(sum) * sx * sw + b;
+}
+
+__device__ __forceinline__ void st_any(void* y, int dt, int64_t i, float v) {
+  if (dt == kF32) static_cast<float*>(y)[i] = v;
+  else if (dt == kF16) static_cast<uint16_t*>(y)[i] = out1<kF16>(v);
+  else static_cast<uint16_t*>(y)[i] = out1<kBF16>(v);
+}
+
+// Four neighbouring outputs y[m, n .. n + 3] (n % 4 == 0).
+__device__ __forceinline__ void st_quad(const W8Args& a, int64_t m, int n, f4v v) {
+  const int64_t i = m * a.N + n;
+  if (a.vec && n + 3 < a.N) {
+    if (a.out_dt == kF32) *reinterpret_cast<f4v*>(static_cast<float*>(a.y) + i) = v;
+    else
+      *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.y) + i) =
+          a.out_dt == kF16 ? u32x2{pack2_out<kF16>(v.x, v.y), pack2_out<kF16>(v.z, v.w)}
+                           : u32x2{pack2_out<kBF16>(v.x, v.y), pack2_out<kBF16>(v.z, v.w)};
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (n + q < a.N) st_any(a.y, a.out_dt, i + q, v[q]);
+  }
+}
+
+// Calls f with the activation as a constant.
+template <typename F>
+inline void with_act(int act, F&& f) {
+  switch (act) {
+    case CBQ_ACT_SILU: f(std::integral_constant<int, CBQ_ACT_SILU>{}); break;
+    case CBQ_ACT_GELU: f(std::integral_constant<int, CBQ_ACT_GELU>{}); break;
+    case CBQ_ACT_GELU_TANH: f(std::integral_constant<int, CBQ_ACT_GELU_TANH>{}); break;
+    case CBQ_ACT_RELU: f(std::integral_constant<int, CBQ_ACT_RELU>{}); break;
+    default: f(std::integral_constant<int, kNoAct>{}); break;
+  }
+}
+
+// cbq_w8a8_few.hip: M <= kFewRows, any K and alignment; returns after queueing.
+constexpr int kFewRows = 64;
+void launch_w8a8_few(const W8Args& a, hipStream_t s);
+
+}  // namespace cbq

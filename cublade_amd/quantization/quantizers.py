@@ -171,7 +171,9 @@ def _init_registry():
     """Filled lazily (the layer module imports this one)."""
     if not QUANT_LAYER_REGISTRY:
         from .linear import cuBladeW8A16LinearLayer
+        from .w8a8 import cuBladeW8A8LinearLayer
         QUANT_LAYER_REGISTRY["w8a16"] = cuBladeW8A16LinearLayer
+        QUANT_LAYER_REGISTRY["w8a8"] = cuBladeW8A8LinearLayer
 
 
 def quantize_model(
@@ -185,10 +187,11 @@ def quantize_model(
     """Replace the model's nn.Linear layers with quantized layers
     (reference: quantizers.py:152-224).
 
-    quant_type: "w8a16" (INT8 per-output-channel weights, 16-bit activations).
+    quant_type: "w8a16" (INT8 per-output-channel weights, 16-bit activations) or
+    "w8a8" (the activations in INT8 too, one scale for each token).
     target_modules / exclude_modules: substring filters on dotted names.
     inplace=False quantizes a deep copy. quant_kwargs go to the layer
-    (handle_outliers, outlier_threshold). Returns the (possibly copied) model.
+    ("w8a16": handle_outliers, outlier_threshold, outlier_mode). Returns the (possibly copied) model.
     """
     _init_registry()
     if quant_type not in QUANT_LAYER_REGISTRY:

@@ -1,0 +1,123 @@
+"""linear_w8a8 and gated_w8a8 against plain forms in 64 bits (tests/_w8a8.py)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests import _w8a8 as P
+
+pytestmark = pytest.mark.gpu
+
+DT = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+# rows, output channels, columns: single tokens, both sides of every limit between
+# kernels (16, 32, 64 rows), columns that fill no block, no step, no 16 bytes
+SHAPES = [(1, 1, 1), (1, 4096, 512), (2, 40, 15), (3, 17, 33), (15, 4100, 272), (16, 9000, 144),
+          (17, 100, 1000), (33, 513, 128), (64, 129, 2064), (64, 8200, 130), (65, 128, 64), (65, 1, 16),
+          (65, 7, 17), (100, 300, 48), (127, 255, 4096), (128, 256, 272), (257, 511, 1040),
+          (300, 1001, 1403), (70, 130, 9), (1000, 520, 640), (2100, 2050, 80), (260, 4096, 11008)]
+
+
+def _case(m, n, k, seed, bias, xmode, dtype):
+    x, sx = P.codes(m, k, seed)
+    w, sw = P.codes(n, k, seed + 1)
+    if xmode == "tensor":
+        sx = sx[0].clone()
+    b = torch.randn(n, generator=torch.Generator().manual_seed(seed + 2)).to(dtype).cuda() if bias else None
+    return x, sx, w, sw, b
+
+
+@pytest.mark.parametrize("i,shape", list(enumerate(SHAPES)))
+def test_linear_to_the_last_bit(i, shape):
+    from cublade_amd.quantization import linear_w8a8
+    dtype = list(DT.values())[i % 3]
+    x, sx, w, sw, b = _case(*shape, 10 * i, i % 2 == 0, "tensor" if i % 4 == 3 else "token", dtype)
+    y = linear_w8a8(P.qt(x, sx, dtype), P.qt(w, sw), b)
+    assert y.dtype == dtype and y.shape == shape[:2]
+    want = P.linear(x, sx, w, sw, b, dtype)
+    assert torch.equal(y.cpu(), want), (y.cpu().float() - want.float()).abs().max()
+
+
+@pytest.mark.parametrize("act", P.ACTS)
+@pytest.mark.parametrize("shape", [(1, 1, 1), (1, 4100, 528), (5, 33, 17), (16, 9000, 144), (20, 300, 1000),
+                                   (64, 70, 130), (65, 128, 64), (90, 129, 33), (128, 64, 4096),
+                                   (333, 700, 1400), (1030, 1500, 96)])
+def test_gated(shape, act):
+    from cublade_amd.quantization import gated_w8a8
+    m, n, k = shape
+    i = P.ACTS.index(act) + m
+    dtype = list(DT.values())[i % 3]
+    x, sx, g, sg, gb = _case(m, n, k, i, i % 2 == 0, "token", dtype)
+    _, _, u, su, ub = _case(1, n, k, i + 7, i % 4 < 2, "token", dtype)
+    sx, sg, su = sx * 40 / k ** 0.5, sg / 4, su / 4
+    y = gated_w8a8(P.qt(x, sx, dtype), P.qt(g, sg), P.qt(u, su), activation=act, gate_bias=gb, up_bias=ub)
+    assert y.dtype == dtype and y.shape == (m, n)
+    want, bound = P.gated(x, sx, (g, sg, gb), (u, su, ub), act, dtype)
+    err = (y.cpu().double() - want).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("m", [2, 40, 65, 300])
+def test_sums_of_the_largest_codes(m):
+    """The longest rows of the largest codes, -128 among them: 2^14 K < 2^31."""
+    from cublade_amd.quantization import linear_w8a8
+    k, n = 131071, 40
+    x = torch.full((m, k), -128, dtype=torch.int8, device="cuda")
+    w = torch.full((n, k), -128, dtype=torch.int8, device="cuda")
+    w[1::2] = 127
+    one = torch.ones((), device="cuda")
+    y = linear_w8a8(P.qt(x, one), P.qt(w, one), out_dtype=torch.float32)
+    assert torch.equal(y.cpu()[0, :2], torch.tensor([k * 16384.0, -k * 16256.0]))
+    assert bool((y == y[0]).all()) and bool((y[:, ::2] == y[0, 0]).all())
+
+
+def test_a_token_does_not_depend_on_its_batch():
+    """The same row alone, among few, among many and where K is split: equal bits."""
+    from cublade_amd.quantization import gated_w8a8, linear_w8a8
+    n, k = 1000, 4096
+    x, sx = P.codes(700, k, 1)
+    (w, sw), (u, su) = P.codes(n, k, 2), P.codes(n, k, 3)
+    sx = sx / 50
+    for f in (lambda r: linear_w8a8(P.qt(x[r], sx[r]), P.qt(w, sw)),
+              lambda r: gated_w8a8(P.qt(x[r], sx[r]), P.qt(w, sw), P.qt(u, su))):
+        whole = f(slice(0, 700))
+        for r in (slice(0, 1), slice(3, 20), slice(100, 164), slice(200, 330)):
+            assert torch.equal(f(r), whole[r])
+
+
+def test_strided_rows_and_offsets():
+    """Codes as columns of a larger tensor, with and without alignment, and scales
+    with strides."""
+    from cublade_amd.quantization import linear_w8a8
+    big, _ = P.codes(200, 640, 5)
+    wide, _ = P.codes(96, 512, 6)
+    s = torch.rand(400, device="cuda")[::2] * 0.01
+    for m in (3, 64, 200):
+        for off, k in ((0, 512), (16, 256), (5, 256), (7, 77), (3, 512)):
+            x, w = big[:m, off:off + k], wide[:, :k]
+            y = linear_w8a8(P.qt(x, s[:m]), P.qt(w, s[:96]))
+            want = P.linear(x, s[:m], w, s[:96], None, torch.float16)
+            assert torch.equal(y.cpu(), want), (m, off, k)
+
+
+def test_empty_sizes():
+    from cublade_amd.quantization import gated_w8a8, linear_w8a8
+    for m, n, k in ((0, 8, 16), (4, 0, 16), (4, 8, 0), (80, 8, 0)):
+        (x, sx), (w, sw) = P.codes(m, k, 1), P.codes(n, k, 2)
+        b = torch.arange(n, dtype=torch.float32, device="cuda") + 0.5
+        y = linear_w8a8(P.qt(x, sx), P.qt(w, sw), b)
+        assert y.shape == (m, n) and torch.equal(y, b.half().expand(m, n))
+        y = gated_w8a8(P.qt(x, sx), P.qt(w, sw), P.qt(w, sw), activation="relu", gate_bias=b, up_bias=b)
+        assert torch.equal(y, (b * b).half().expand(m, n))
+
+
+def test_scales_that_are_not_finite():
+    """A NaN scale (a token whose norm was not finite) and an infinite one reach
+    their own row or column only."""
+    from cublade_amd.quantization import linear_w8a8
+    for m in (5, 70):
+        (x, sx), (w, sw) = P.codes(m, 128, 1), P.codes(30, 128, 2)
+        sx[2], sw[4] = float("nan"), float("inf")
+        y = linear_w8a8(P.qt(x, sx), P.qt(w, sw)).cpu()
+        want = P.linear(x, sx, w, sw, None, torch.float16)
+        assert torch.equal(y.isnan(), want.isnan())
+        assert torch.equal(y.nan_to_num(1.0), want.nan_to_num(1.0))
