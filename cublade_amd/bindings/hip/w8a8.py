@@ -12,31 +12,31 @@ _MAX_STRIDE = 1 << 22      # bytes between rows that the kernels take
 
 
 def _rows(codes: torch.Tensor, scale: torch.Tensor, dev: torch.device, k: int | None, name: str):
-    """(I8Rows, the tensors it points to): codes as they are where the kernels
-    can read their rows, else a contiguous copy."""
-    if codes.dtype != torch.int8 or codes.dim() != 2 or (k is not None and codes.size(1) != k):
+    """(I8Rows, rows, columns, the tensors it points to): codes as they are where
+    the kernels can read their rows, else a contiguous copy."""
+    shape = codes.shape
+    if codes.dtype is not torch.int8 or len(shape) != 2 or (k is not None and shape[1] != k):
         raise RuntimeError(f"{name} must be int8 [rows, {'columns' if k is None else k}], got "
-                           f"{tuple(codes.shape)} {codes.dtype}")
+                           f"{tuple(shape)} {codes.dtype}")
     if codes.device != dev or scale.device != dev:
         raise RuntimeError(f"{name} and its scales must be on {dev}, got {codes.device} and "
                            f"{scale.device}")
-    if scale.dtype != torch.float32:
+    if scale.dtype is not torch.float32:
         raise RuntimeError(f"{name} must have torch.float32 scales, got {scale.dtype}")
-    rows, cols = codes.shape
-    step = 1
-    if scale.dim() == 0:
-        step = 0
-    elif scale.dim() != 1 or scale.numel() != rows:
-        raise RuntimeError(f"{name} must have one scale for each of its {rows} rows, or a 0-d one "
-                           f"for all, got {tuple(scale.shape)}")
-    elif not scale.is_contiguous():
-        scale = scale.contiguous()
+    rows, cols = shape
+    step = scale.dim()
+    if step:
+        if step != 1 or scale.numel() != rows:
+            raise RuntimeError(f"{name} must have one scale for each of its {rows} rows, or a 0-d "
+                               f"one for all, got {tuple(scale.shape)}")
+        if not scale.is_contiguous():
+            scale = scale.contiguous()
     stride, es = codes.stride()
-    if es != 1 or stride < cols or stride > _MAX_STRIDE or (
-            cols % 16 == 0 and (stride % 16 or codes.data_ptr() % 16)):
+    p = codes.data_ptr()
+    if es != 1 or stride < cols or stride > _MAX_STRIDE or (cols % 16 == 0 and (stride % 16 or p % 16)):
         codes = codes.clone(memory_format=torch.contiguous_format)
-        stride = cols
-    return _abi.I8Rows(codes.data_ptr(), stride, scale.data_ptr(), step), codes, scale
+        stride, p = cols, codes.data_ptr()
+    return _abi.I8Rows(p, stride, scale.data_ptr(), step), rows, cols, (codes, scale)
 
 
 def _bias(b: torch.Tensor | None, n: int, dev: torch.device, name: str):
@@ -60,28 +60,35 @@ def _check_cuda(x: torch.Tensor, what: str) -> None:
         raise RuntimeError(f"{what}: x must be on CUDA, got {x.device}")
 
 
+def _run(call, args, dev: torch.device, size, what: str) -> None:
+    with _abi.on_device(dev):
+        need = _abi.lib().cbq_w8a8_ws_bytes(*size)
+        if need <= _abi.WS_CTRL_BYTES:      # one launch that passes nothing on
+            rc = call(*args, None, 0, _abi.stream_handle(dev))
+        else:
+            with _abi.workspace_lock(dev):
+                ws = _abi.workspace(dev, need)
+                rc = call(*args, ws.data_ptr(), ws.numel(), _abi.stream_handle(dev))
+    _abi.check(rc, what)
+
+
 def w8a8_linear(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
                 bias: torch.Tensor | None, out_dtype: torch.dtype) -> torch.Tensor:
     """y[m, n] = x_scale[m] w_scale[n] sum_k x[m, k] w[n, k] + bias[n]; see
     quantization.w8a8.linear_w8a8."""
     _check_cuda(x, "w8a8_linear")
     dev = x.device
-    cx, x, x_scale = _rows(x, x_scale, dev, None, "x")
-    m, k = x.shape
-    cw, w, w_scale = _rows(w, w_scale, dev, k, "weight")
-    n = w.size(0)
+    cx, m, k, keep_x = _rows(x, x_scale, dev, None, "x")
+    cw, n, _, keep_w = _rows(w, w_scale, dev, k, "weight")
     b = _bias(bias, n, dev, "bias")
     code = _out_code(out_dtype)
-    y = torch.empty((m, n), dtype=out_dtype, device=dev)
+    y = x.new_empty((m, n), dtype=out_dtype)
     if m == 0 or n == 0:
         return y
-    L = _abi.lib()
-    with _abi.on_device(dev), _abi.workspace_lock(dev):
-        ws = _abi.workspace(dev, L.cbq_w8a8_ws_bytes(m, n, k, 1))
-        rc = L.cbq_w8a8_linear(ctypes.byref(cx), ctypes.byref(cw), _abi.ptr(b),
-                               0 if b is None else _abi.DTYPE_CODE[b.dtype], m, n, k, y.data_ptr(),
-                               code, ws.data_ptr(), ws.numel(), _abi.stream_handle(dev))
-    _abi.check(rc, "w8a8_linear")
+    call = _abi.lib().cbq_w8a8_linear
+    args = (ctypes.byref(cx), ctypes.byref(cw), _abi.ptr(b),
+            0 if b is None else _abi.DTYPE_CODE[b.dtype], m, n, k, y.data_ptr(), code)
+    _run(call, args, dev, (m, n, k, 1), "w8a8_linear")
     return y
 
 
@@ -96,27 +103,21 @@ def w8a8_gated(x: torch.Tensor, x_scale: torch.Tensor, gate: torch.Tensor,
     if act is None:
         raise RuntimeError(f"activation must be one of {sorted(_abi.ACT_CODE)}, got {activation!r}")
     dev = x.device
-    cx, x, x_scale = _rows(x, x_scale, dev, None, "x")
-    m, k = x.shape
-    cg, gate, gate_scale = _rows(gate, gate_scale, dev, k, "gate")
-    cu, up, up_scale = _rows(up, up_scale, dev, k, "up")
-    n = gate.size(0)
-    if up.size(0) != n:
-        raise RuntimeError(f"gate and up must have equally many rows, got {n} and {up.size(0)}")
+    cx, m, k, keep_x = _rows(x, x_scale, dev, None, "x")
+    cg, n, _, keep_gate = _rows(gate, gate_scale, dev, k, "gate")
+    cu, n_up, _, keep_up = _rows(up, up_scale, dev, k, "up")
+    if n_up != n:
+        raise RuntimeError(f"gate and up must have equally many rows, got {n} and {n_up}")
     gb, ub = _bias(gate_bias, n, dev, "gate_bias"), _bias(up_bias, n, dev, "up_bias")
     if gb is not None and ub is not None and gb.dtype != ub.dtype:
         raise RuntimeError(f"gate_bias and up_bias must have one dtype, got {gb.dtype} and {ub.dtype}")
     code = _out_code(out_dtype)
-    y = torch.empty((m, n), dtype=out_dtype, device=dev)
+    y = x.new_empty((m, n), dtype=out_dtype)
     if m == 0 or n == 0:
         return y
     some = gb if gb is not None else ub
-    L = _abi.lib()
-    with _abi.on_device(dev), _abi.workspace_lock(dev):
-        ws = _abi.workspace(dev, L.cbq_w8a8_ws_bytes(m, n, k, 2))
-        rc = L.cbq_w8a8_gated(ctypes.byref(cx), ctypes.byref(cg), ctypes.byref(cu), _abi.ptr(gb),
-                              _abi.ptr(ub), 0 if some is None else _abi.DTYPE_CODE[some.dtype], act,
-                              m, n, k, y.data_ptr(), code, ws.data_ptr(), ws.numel(),
-                              _abi.stream_handle(dev))
-    _abi.check(rc, "w8a8_gated")
+    call = _abi.lib().cbq_w8a8_gated
+    args = (ctypes.byref(cx), ctypes.byref(cg), ctypes.byref(cu), _abi.ptr(gb), _abi.ptr(ub),
+            0 if some is None else _abi.DTYPE_CODE[some.dtype], act, m, n, k, y.data_ptr(), code)
+    _run(call, args, dev, (m, n, k, 2), "w8a8_gated")
     return y

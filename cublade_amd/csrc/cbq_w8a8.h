@@ -36,7 +36,7 @@ struct W8Args {
 };
 
 // act(g) in fp32. The sigmoids take the hardware's 2^x and reciprocal (1 ulp
-// each); the argument's rounding costs |g| 2^-24 of e^-g. act is uniform.
+// each); the argument's rounding costs |g| 2^-24 of e^-g. 
 __device__ __forceinline__ float sigmoid_of(float z) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504f));
 }
@@ -52,8 +52,36 @@ __device__ __forceinline__ float activate(float g) {
   else return g;
 }
 
+// The same for an activation known at run time (the same for all threads).
+__device__ __forceinline__ float activate(int act, float g) {
+  switch (act) {
+    case CBQ_ACT_SILU: return activate<CBQ_ACT_SILU>(g);
+    case CBQ_ACT_GELU: return activate<CBQ_ACT_GELU>(g);
+    case CBQ_ACT_GELU_TANH: return activate<CBQ_ACT_GELU_TANH>(g);
+    default: return activate<CBQ_ACT_RELU>(g);
+  }
+}
+
 __device__ __forceinline__ float ld_any(const void* p, int dt, int64_t i) {
   return dt == kF32 ? ld1<kF32>(p, i) : dt == kF16 ? ld1<kF16>(p, i) : ld1<kBF16>(p, i);
+}
+
+// 16 bytes of a row of K >= 16 codes at min(k, K - 16), at any address.
+__device__ __forceinline__ u32x4 ld_codes(const uint8_t* row, int k, int K) {
+  typedef u32x4 __attribute__((aligned(1))) u32x4_any;
+  return *reinterpret_cast<const u32x4_any*>(row + min(k, K - 16));
+}
+
+// The codes k .. k + 15 of what ld_codes loaded for them, with zeros from K on.
+__device__ __forceinline__ u32x4 from_k(u32x4 v, int k, int K) {
+  if (const int d = k - min(k, K - 16)) {   // the row's last chunk: moved down
+    if (d & 8) v = u32x4{v.z, v.w, 0u, 0u};
+    if (d & 4) v = u32x4{v.y, v.z, v.w, 0u};
+    v = u32x4{__builtin_amdgcn_alignbyte(v.y, v.x, d & 3), __builtin_amdgcn_alignbyte(v.z, v.y, d & 3),
+              __builtin_amdgcn_alignbyte(v.w, v.z, d & 3), __builtin_amdgcn_alignbyte(0u, v.w, d & 3)};
+    if (d >= 16) v = u32x4{0u, 0u, 0u, 0u};
+  }
+  return v;
 }
 
 // An integer sum with its scales and bias.
@@ -95,8 +123,8 @@ inline void with_act(int act, F&& f) {
   }
 }
 
-// cbq_w8a8_few.hip: M <= kFewRows, any K and alignment; returns after queueing.
-constexpr int kFewRows = 64;
+// cbq_w8a8_few.hip: M <= kFewRows, K >= 16, any alignment; returns after queueing.
+constexpr int kFewRows = 128;
 void launch_w8a8_few(const W8Args& a, hipStream_t s);
 
 }  // namespace cbq

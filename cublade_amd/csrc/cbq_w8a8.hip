@@ -7,23 +7,29 @@
 //
 // Sums are int32 and exact (K <= 131071). M <= 64: cbq_w8a8_few.hip.
 //
-// k_w8_tile<T, ACT, SPLIT>: T x T tiles (gated: T x T / 2 outputs, T / 2 columns of
-// each projection side by side, so that a lane holds g and u of the same outputs) of
-// v_mfma_i32_32x32x32_i8, 4 waves of T / 2 x T / 2. k-steps of 64 bytes; four LDS
-// stages filled by LDS DMA, three k-steps in flight, one barrier per k-step between
-// its two halves, so that the fragment reads of the next half overlap the products
-// of this one.
+// k_w8_tile<J, I, NS, ACT, SPLIT, ANY>: tiles of 64 J tokens x 64 I weight rows (gated:
+// 32 I columns of each projection side by side, so that a lane holds g and u of the
+// same outputs) of v_mfma_i32_32x32x32_i8, 4 waves of 32 J x 32 I. k-steps of 128 bytes,
+// a cache line of every row (steps of 64 asked the L2 for each line twice); NS LDS
+// stages filled by LDS DMA; one barrier per k-step, in front of its last quarter.
 //
-// LDS layout of a stage: T rows of x, then T weight rows, 64 bytes each; 16-byte
-// chunk c of row r at c ^ ((r >> 2) & 3). In half s of a k-step the lanes of half h
-// (lane / 32) take chunk 2 h + s of both operands.
+// LDS layout of a stage: the tile's rows of x, then its weight rows, 128 bytes each;
+// 16-byte chunk c of row r at c ^ (r & 7). In quarter s of a k-step the lanes of half h
+// (lane / 32) take chunk 2 s + h of both operands.
 //
 // A = weight rows, B = activation rows: lane l holds the outputs of token m = l % 32
 // and n = 8 (v / 4) + 4 (l / 32) + v % 4. Outputs leave through LDS, 32 tokens at a
 // time per wave, and are stored 16 bytes per lane along a row.
 //
+// ANY: rows that are no multiples of 16 bytes, which the DMA does not take. They pass
+// through registers, loaded a k-step ahead: 1.0 us a k-step of 128 x 128 instead of 0.5
+// (loads from the multiple of 4 in front, shifted by the vector unit: 1.7). From 1024
+// tokens on, copies in rows that the DMA takes cost less (k_w8_pad).
+//
 // K is cut into ranges where few tiles would leave CUs idle: each range writes its
 // sums to the workspace and k_w8_join adds them (integers: exact in any order).
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "cbq_lds_dma.h"
@@ -32,18 +38,16 @@
 namespace cbq {
 namespace {
 
-constexpr int kW8NS = 4;   // LDS stages
-
-template <int T> struct W8Geom {
+template <int J, int I, int NS> struct W8Geom {
   static constexpr int kWaves = 4;
   static constexpr int kThreads = 64 * kWaves;
-  static constexpr int kHalf = T * 64;                  // bytes of one operand per stage
-  static constexpr int kSB = 2 * kHalf;
-  static constexpr int kL = kHalf / (kThreads * 16);    // DMA instructions per operand
-  static constexpr int kWT = T / 2;                     // edge of a wave's tile
-  static constexpr int kJ = kWT / 32;                   // 32 x 32 tiles along its edges
-  static constexpr int kPitch = kWT * 4 + 16;           // row of outputs in LDS, bytes
-  static_assert(kWaves * 32 * kPitch <= kW8NS * kSB, "the outputs fit in the stages");
+  static constexpr int kTM = 64 * J, kTN = 64 * I;      // rows of x, weight rows
+  static constexpr int kX = kTM * 128;                  // bytes of x per stage
+  static constexpr int kSB = (kTM + kTN) * 128;
+  static constexpr int kLX = 2 * J, kLW = 2 * I;        // loads per thread and stage
+  static constexpr int kPitch = 128 * I + 16;           // row of outputs in LDS, bytes
+  static_assert(kWaves * 32 * kPitch <= NS * kSB, "the outputs fit in the stages");
+  static_assert((NS - 1) * (kLX + kLW) <= 63, "loads in flight are counted in 6 bits");
 };
 
 // Workgroup -> (tile m, tile n): XCD b % 8 takes a contiguous run of tiles, in
@@ -60,15 +64,18 @@ __device__ __forceinline__ void w8_tile(int b, const W8Args& a, int& tm, int& tn
   tn = r / gsize;
 }
 
-template <int T, int ACT, bool SPLIT>
-__global__ __launch_bounds__(W8Geom<T>::kThreads) void k_w8_tile(W8Args a) {
-  typedef W8Geom<T> G;
+template <int J, int I, int NS, int ACT, bool SPLIT, bool ANY>
+__global__ __launch_bounds__(256) void k_w8_tile(W8Args a) {
+  typedef W8Geom<J, I, NS> G;
   constexpr bool GATED = ACT != kNoAct;
-  constexpr int J = G::kJ, L = G::kL, WT = G::kWT, NW = G::kWaves;
-  constexpr int TN = GATED ? T / 2 : T;                 // output columns of a tile
-  constexpr int WN = GATED ? WT / 2 : WT;               // and of a wave
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[kW8NS * G::kSB];
-  __shared__ __attribute__((aligned(16))) float s_x[T], s_w[T], s_b[T];
+  static_assert(!GATED || I % 2 == 0, "pairs of tiles");
+  static_assert(!ANY || NS == 2, "two stages");
+  constexpr int LX = G::kLX, LT = G::kLX + G::kLW, NW = G::kWaves;
+  constexpr int WM = 32 * J, WR = 32 * I;               // a wave's tokens, weight rows
+  constexpr int WN = GATED ? WR / 2 : WR;               // and output columns
+  constexpr int IO = GATED && !SPLIT ? I / 2 : I;       // 32-column tiles it puts out
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[NS * G::kSB];
+  __shared__ __attribute__((aligned(16))) float s_x[G::kTM], s_w[G::kTN], s_b[G::kTN];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -78,21 +85,20 @@ __global__ __launch_bounds__(W8Geom<T>::kThreads) void k_w8_tile(W8Args a) {
   const int split = SPLIT ? blockIdx.x / tiles : 0;
   int tm, tn;
   w8_tile(SPLIT ? blockIdx.x % tiles : blockIdx.x, a, tm, tn);
-  const int m0 = tm * T, n0 = tn * TN;
-  const int steps = a.K >> 6;                           // whole k-steps of all of K
-  const int kb = split * a.split_steps;                 // first one of this range
+  const int m0 = tm * G::kTM, n0 = tn * 2 * WN;
+  const int steps = (a.K + 127) >> 7;
+  const int kb = split * a.split_steps;                 // first k-step of this range
   const int nk = SPLIT ? min(a.split_steps, steps - kb) : steps;
-  const bool tail = (a.K & 63) && (!SPLIT || split == a.splits - 1);
   const uint32_t sbase = __builtin_amdgcn_readfirstlane(lds_addr(smem));
 
-  // Weight row `r` of the tile: its projection, and its column from n0 on.
-  // Gated: a wave's rows are WN of the gate, then the same WN of the up projection.
-  auto proj_of = [&](int r) { return GATED ? (r % WT) / WN : 0; };
-  auto col_of = [&](int r) { return GATED ? r / WT * WN + r % WN : r; };
+  // Weight row r of the tile: its projection, and its column from n0 on. Gated: a
+  // wave's rows are WN of the gate, then the same WN of the up projection.
+  auto proj_of = [&](int r) { return GATED ? (r % WR) / WN : 0; };
+  auto col_of = [&](int r) { return GATED ? r / WR * WN + r % WN : r; };
 
   if constexpr (!SPLIT) {   // scales and biases of the tile's rows and columns
-    for (int r = tid; r < T; r += G::kThreads) {
-      s_x[r] = a.sx[min(m0 + r, a.M - 1) * a.sx_step];
+    for (int r = tid; r < G::kTM; r += 256) s_x[r] = a.sx[min(m0 + r, a.M - 1) * a.sx_step];
+    for (int r = tid; r < G::kTN; r += 256) {
       const int p = proj_of(r);
       const int64_t n = min(n0 + col_of(r), a.N - 1);
       s_w[r] = p ? a.sw[1][n * a.sw_step[1]] : a.sw[0][n * a.sw_step[0]];
@@ -101,142 +107,162 @@ __global__ __launch_bounds__(W8Geom<T>::kThreads) void k_w8_tile(W8Args a) {
     }
   }
 
-  // DMA instruction u of an operand fills rows (u NW + wave) 16 + lane / 4, chunk
-  // slot lane % 4. Rows past M or N are the last row's; their products are not stored.
-  const uint8_t* xbase = a.x + m0 * a.ldx;
-  uint32_t xo[L], wo[L];
-  const uint8_t* wbase[L];
+  // Load u of a stage: rows (u NW + wave) 8 + lane / 8 (of x, then of the weight), the
+  // chunk that belongs at slot lane % 8. Rows past M or N are the last row's; their
+  // products are not stored. Chunks past K are the last one's (ANY: see there); x counts
+  // as zero there.
+  const int lrow = lane >> 3;
+  const int lk = ((lane & 7) ^ lrow) << 4;
+  uint32_t off[LT];                                     // of the row, from its base
+  const uint8_t* base[LT];
 #pragma unroll
-  for (int u = 0; u < L; ++u) {
-    const int row = (u * NW + wave) * 16 + (lane >> 2);
-    const uint32_t c = static_cast<uint32_t>((lane & 3) ^ ((row >> 2) & 3)) << 4;
-    const int p = __builtin_amdgcn_readfirstlane(proj_of(row));
-    xo[u] = static_cast<uint32_t>(min(row, a.M - 1 - m0)) * static_cast<uint32_t>(a.ldx) + c;
-    wo[u] = static_cast<uint32_t>(min(col_of(row), a.N - 1 - n0)) *
-                static_cast<uint32_t>(p ? a.ldw[1] : a.ldw[0]) + c;
-    wbase[u] = p ? a.w[1] + n0 * a.ldw[1] : a.w[0] + n0 * a.ldw[0];
+  for (int u = 0; u < LT; ++u) {
+    if (u < LX) {
+      const int r = (u * NW + wave) * 8 + lrow;
+      off[u] = static_cast<uint32_t>(min(r, a.M - 1 - m0)) * static_cast<uint32_t>(a.ldx);
+      base[u] = a.x + m0 * a.ldx;
+    } else {
+      const int r = ((u - LX) * NW + wave) * 8 + lrow;
+      const int p = __builtin_amdgcn_readfirstlane(proj_of(r));
+      off[u] = static_cast<uint32_t>(min(col_of(r), a.N - 1 - n0)) *
+               static_cast<uint32_t>(p ? a.ldw[1] : a.ldw[0]);
+      base[u] = p ? a.w[1] + n0 * a.ldw[1] : a.w[0] + n0 * a.ldw[0];
+    }
   }
-  auto issue_one = [&](int t, int stage, int u) {
-    const uint32_t dst = sbase + stage * G::kSB + wave * 1024;
-    if (u < L)
-      lds_dma16(xo[u], uniform_ptr(xbase + static_cast<int64_t>(kb + t) * 64), dst + u * NW * 1024);
-    else
-      lds_dma16(wo[u - L], uniform_ptr(wbase[u - L] + static_cast<int64_t>(kb + t) * 64),
-                dst + G::kHalf + (u - L) * NW * 1024);
+  auto issue_one = [&](int t, int u) {                  // t: k-step of this range
+    const int k = min((kb + t) * 128 + lk, a.K - 16);
+    if constexpr (!ANY)
+      lds_dma16(off[u] + static_cast<uint32_t>(k), uniform_ptr(base[u]),
+                sbase + (t % NS) * G::kSB + (u < LX ? 0 : G::kX) + ((u < LX ? u : u - LX) * NW + wave) * 1024);
+  };
+  u32x4 held[ANY ? LT : 1];                             // ANY: a tile's loads on their way to LDS
+  auto hold_one = [&](int t, int u) { held[u] = ld_codes(base[u] + off[u], (kb + t) * 128 + lk, a.K); };
+  auto land = [&](int t, int u) {
+    u32x4 v = held[u];
+    if ((kb + t) * 128 + 128 > a.K) v = from_k(v, (kb + t) * 128 + lk, a.K);
+    *reinterpret_cast<u32x4*>(smem + (t % NS) * G::kSB + (u < LX ? 0 : G::kX) +
+                              ((u < LX ? u : u - LX) * NW + wave) * 1024 + lane * 16) = v;
   };
 
-  uint32_t xr[2], wr[2];   // fragment read offsets of half s
+  const uint32_t xr = (wm * WM + r32) * 128, wr = G::kX + (wn * WR + r32) * 128;
+  uint32_t slot[4];
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const uint32_t slot = static_cast<uint32_t>((2 * h + s) ^ ((r32 >> 2) & 3)) << 4;
-    xr[s] = (wm * WT + r32) * 64 + slot;
-    wr[s] = G::kHalf + (wn * WT + r32) * 64 + slot;
-  }
-  i16x acc[J][J];          // [token tile][weight tile]
+  for (int s = 0; s < 4; ++s) slot[s] = static_cast<uint32_t>((2 * s + h) ^ (r32 & 7)) << 4;
+  i16x acc[J][I];          // [token tile][weight tile]
 #pragma unroll
   for (int j = 0; j < J; ++j)
 #pragma unroll
-    for (int i = 0; i < J; ++i) acc[j][i] = i16x{};
-  struct Frags { i4v x[J], w[J]; };
-  auto read_one = [&](int stage, int s, Frags& f, int r) {
-    const uint8_t* st = smem + stage * G::kSB;
-    if (r < J) f.w[r] = *reinterpret_cast<const i4v*>(st + wr[s] + r * 2048);
-    else f.x[r - J] = *reinterpret_cast<const i4v*>(st + xr[s] + (r - J) * 2048);
+    for (int i = 0; i < I; ++i) acc[j][i] = i16x{};
+  struct Frags { i4v x[J], w[I]; };
+  auto read_one = [&](int t, int s, Frags& f, int r) {  // fragment r of quarter s
+    const uint8_t* st = smem + (t % NS) * G::kSB;
+    if (r < I) f.w[r] = *reinterpret_cast<const i4v*>(st + wr + slot[s] + r * 4096);
+    else f.x[r - I] = *reinterpret_cast<const i4v*>(st + xr + slot[s] + (r - I) * 4096);
   };
-  auto mma_one = [&](const Frags& f, int q) {
-    acc[q / J][q % J] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[q % J], f.x[q / J],
-                                                              acc[q / J][q % J], 0, 0, 0);
+  // The products of one quarter, with n pieces of other work spread between them.
+  auto quarter = [&](const Frags& f, auto n, auto&& work) {
+#pragma unroll
+    for (int q = 0; q < J * I; ++q) {
+      acc[q / I][q % I] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[q % I], f.x[q / I], acc[q / I][q % I],
+                                                                0, 0, 0);
+#pragma unroll
+      for (int e = decltype(n)::value * q / (J * I); e < decltype(n)::value * (q + 1) / (J * I); ++e) work(e);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
+  constexpr std::integral_constant<int, J + I> kReads{};
+  constexpr std::integral_constant<int, J + I + LT> kAll{};
 
-  // Step t: f0 holds the fragments of tile t's first half. Its products run with the
-  // reads of the second half into f1 between them; then the wait for tile t + 1 and
-  // the barrier (every wave is past its reads of tile t - 1, whose stage tile t + 3
-  // takes); then the second half's products, between them the DMA of tile t + 3 and
-  // the reads of tile t + 1's first half.
+  // Step t: the products of a quarter run with the reads of the next one between them.
+  // In front of the last quarter every fragment of tile t is read and, past the wait
+  // and the barrier, tile t + 1 is there: its stage is read from and tile t + NS takes
+  // tile t's. more: there is a tile t + NS; all: wait for every load in flight.
   Frags f0, f1;
-  auto step = [&](int t, auto dma, auto all) {
-#pragma unroll
-    for (int q = 0; q < J * J; ++q) {
-      mma_one(f0, q);
-#pragma unroll
-      for (int r = 2 * J * q / (J * J); r < 2 * J * (q + 1) / (J * J); ++r)
-        read_one(t % kW8NS, 1, f1, r);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if constexpr (decltype(all)::value) dma_wait_barrier<0>();
-    else dma_wait_barrier<2 * L>();
+  auto step = [&](int t, auto more, auto all) {
+    quarter(f0, kReads, [&](int e) { read_one(t, 1, f1, e); });
+    quarter(f1, kReads, [&](int e) { read_one(t, 2, f0, e); });
+    quarter(f0, kReads, [&](int e) { read_one(t, 3, f1, e); });
+    dma_wait_barrier<decltype(all)::value ? 0 : (NS - 2) * LT>();
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int q = 0; q < J * J; ++q) {
-      mma_one(f1, q);
-#pragma unroll
-      for (int r = 2 * J * q / (J * J); r < 2 * J * (q + 1) / (J * J); ++r)
-        read_one((t + 1) % kW8NS, 0, f0, r);
-      if constexpr (decltype(dma)::value) {
-#pragma unroll
-        for (int u = 2 * L * q / (J * J); u < 2 * L * (q + 1) / (J * J); ++u)
-          issue_one(t + kW8NS - 1, (t + kW8NS - 1) % kW8NS, u);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    if constexpr (decltype(more)::value)
+      quarter(f1, kAll, [&](int e) {
+        if (e < J + I) read_one(t + 1, 0, f0, e);
+        else issue_one(t + NS, e - J - I);
+      });
+    else quarter(f1, kReads, [&](int e) { read_one(t + 1, 0, f0, e); });
+  };
+  // ANY: tile t + 1 lands during the third quarter, and its registers are loaded again
+  // (past the end with some chunk that is not used).
+  auto step_any = [&](int t) {
+    quarter(f0, kReads, [&](int e) { read_one(t, 1, f1, e); });
+    quarter(f1, kReads, [&](int e) { read_one(t, 2, f0, e); });
+    quarter(f0, kAll, [&](int e) {
+      if (e < J + I) read_one(t, 3, f1, e);
+      else land(t + 1, e - J - I);
+    });
+    __syncthreads();
+    quarter(f1, kAll, [&](int e) {
+      if (e < J + I) read_one(t + 1, 0, f0, e);
+      else hold_one(t + 2, e - J - I);
+    });
   };
   using yes = std::true_type;
   using no = std::false_type;
+  if constexpr (ANY) {
 #pragma unroll
-  for (int t = 0; t < kW8NS - 1; ++t)
-    if (t < nk) {
+    for (int u = 0; u < LT; ++u) hold_one(0, u);
 #pragma unroll
-      for (int u = 0; u < 2 * L; ++u) issue_one(t, t, u);
-    }
-  if (nk > 0) {
-    if (nk > 2) dma_wait_barrier<4 * L>();
-    else if (nk > 1) dma_wait_barrier<2 * L>();
-    else dma_wait_barrier<0>();
+    for (int u = 0; u < LT; ++u) land(0, u);
 #pragma unroll
-    for (int r = 0; r < 2 * J; ++r) read_one(0, 0, f0, r);
-    int t = 0;
-    for (; t + kW8NS - 1 < nk; ++t) step(t, yes{}, no{});
-    if (t + 2 < nk) step(t++, no{}, no{});
-    if (t + 1 < nk) step(t++, no{}, yes{});
+    for (int u = 0; u < LT; ++u) hold_one(1, u);
+    __syncthreads();
+  } else {
 #pragma unroll
-    for (int r = 0; r < 2 * J; ++r) read_one((nk - 1) % kW8NS, 1, f1, r);
+    for (int t = 0; t < NS; ++t)
+      if (t < nk) {
 #pragma unroll
-    for (int q = 0; q < J * J; ++q) mma_one(f0, q);
-#pragma unroll
-    for (int q = 0; q < J * J; ++q) mma_one(f1, q);
-  }
-  const int mw = m0 + wm * WT;
-  if (tail) {   // the last K % 64 columns (a multiple of 16), straight from memory
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int k = steps * 64 + (2 * h + s) * 16;
-      const bool in = k < a.K;
-      const int kc = in ? k : 0;
-#pragma unroll
-      for (int i = 0; i < J; ++i) {
-        const int r = wn * WT + 32 * i + r32, p = proj_of(wn * WT + 32 * i);
-        const int64_t n = min(n0 + col_of(r), a.N - 1);
-        f0.w[i] = *reinterpret_cast<const i4v*>((p ? a.w[1] : a.w[0]) +
-                                                n * (p ? a.ldw[1] : a.ldw[0]) + kc);
-        f0.x[i] = *reinterpret_cast<const i4v*>(a.x + min(mw + 32 * i + r32, a.M - 1) * a.ldx + kc);
-        if (!in) f0.x[i] = i4v{0, 0, 0, 0};
+        for (int u = 0; u < LT; ++u) issue_one(t, u);
       }
+    if (nk >= NS) dma_wait_barrier<(NS - 1) * LT>();
+    else dma_wait_barrier<0>();
+  }
 #pragma unroll
-      for (int q = 0; q < J * J; ++q) mma_one(f0, q);
+  for (int r = 0; r < J + I; ++r) read_one(0, 0, f0, r);
+  int t = 0;
+  if constexpr (ANY) {
+    for (; t + 1 < nk; ++t) step_any(t);
+  } else {
+    for (; t + NS < nk; ++t) step(t, yes{}, no{});
+    for (; t + 1 < nk; ++t) step(t, no{}, yes{});
+  }
+  // The last tile. Where K ends inside it, x is zero from there on.
+  auto cut = [&](Frags& f, int s) {
+    if (!ANY && (kb + t) * 128 + (2 * s + h) * 16 >= a.K) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) f.x[j] = i4v{0, 0, 0, 0};
     }
+  };
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    Frags& now = s & 1 ? f1 : f0;
+    Frags& next = s & 1 ? f0 : f1;
+    cut(now, s);
+    quarter(now, kReads, [&](int e) {
+      if (s < 3) read_one(t, s + 1, next, e);
+    });
   }
 
   // Outputs: 32 tokens at a time through the wave's own part of LDS.
   __syncthreads();
   uint8_t* const out = smem + wave * 32 * G::kPitch;
-  const int nw = n0 + wn * WN;                          // the wave's first column
+  const int mw = m0 + wm * WM, nw = n0 + wn * WN;       // the wave's first token and column
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int mj = mw + 32 * j;
-    const float sx = SPLIT ? 0.0f : s_x[wm * WT + 32 * j + r32];
+    const float sx = SPLIT ? 0.0f : s_x[wm * WM + 32 * j + r32];
     wave_lds_fence();                                   // the last rows are read
 #pragma unroll
-    for (int i = 0; i < (GATED && !SPLIT ? J / 2 : J); ++i)
+    for (int i = 0; i < IO; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int c = 32 * i + 8 * q + 4 * h;           // the wave's column of 4 outputs
@@ -245,17 +271,17 @@ __global__ __launch_bounds__(W8Geom<T>::kThreads) void k_w8_tile(W8Args a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) bits[e] = acc[j][i][4 * q + e];
         } else {
-          const f4v w0 = *reinterpret_cast<const f4v*>(s_w + wn * WT + c);
-          const f4v b0 = *reinterpret_cast<const f4v*>(s_b + wn * WT + c);
+          const f4v w0 = *reinterpret_cast<const f4v*>(s_w + wn * WR + c);
+          const f4v b0 = *reinterpret_cast<const f4v*>(s_b + wn * WR + c);
           f4v v;
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] = scaled(acc[j][i][4 * q + e], sx, w0[e], b0[e]);
           if constexpr (GATED) {
-            const f4v w1 = *reinterpret_cast<const f4v*>(s_w + wn * WT + WN + c);
-            const f4v b1 = *reinterpret_cast<const f4v*>(s_b + wn * WT + WN + c);
+            const f4v w1 = *reinterpret_cast<const f4v*>(s_w + wn * WR + WN + c);
+            const f4v b1 = *reinterpret_cast<const f4v*>(s_b + wn * WR + WN + c);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              v[e] = activate<ACT>(v[e]) * scaled(acc[j][i + J / 2][4 * q + e], sx, w1[e], b1[e]);
+              v[e] = activate<ACT>(v[e]) * scaled(acc[j][i + I / 2][4 * q + e], sx, w1[e], b1[e]);
           }
           bits = __builtin_bit_cast(i4v, v);
         }
@@ -263,10 +289,10 @@ __global__ __launch_bounds__(W8Geom<T>::kThreads) void k_w8_tile(W8Args a) {
       }
     wave_lds_fence();                                   // written before it is read
     if constexpr (SPLIT) {
-      // rows of T / 2 sums: gated, WN of each projection
+      // rows of WR sums: gated, WN of each projection
 #pragma unroll
-      for (int r = 0; r < 32 * WT / 256; ++r) {
-        const int e = (r * 64 + lane) * 4, row = e / WT, c = e % WT;
+      for (int r = 0; r < 32 * WR / 256; ++r) {
+        const int e = (r * 64 + lane) * 4, row = e / WR, c = e % WR;
         const int p = GATED ? c / WN : 0;
         if (mj + row < a.M) {
           int* dst = a.part + ((static_cast<int64_t>(split) * (GATED ? 2 : 1) + p) * a.M + mj + row) * a.ldp;
@@ -323,9 +349,16 @@ __global__ __launch_bounds__(kBlock) void k_w8_join(W8Args a) {
 #pragma unroll
   for (int p = 0; p < P; ++p) {
     const int* src = a.part + (p * static_cast<int64_t>(a.M) + m) * a.ldp + n;
+    const int64_t plane = static_cast<int64_t>(P) * a.M * a.ldp;
     i4v s = {0, 0, 0, 0};
-    for (int r = 0; r < a.splits; ++r)
-      s += *reinterpret_cast<const i4v*>(src + static_cast<int64_t>(r) * P * a.M * a.ldp);
+    for (int r = 0; r < a.splits; r += 4) {   // 4 loads under way at a time
+      i4v v4[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v4[e] = *reinterpret_cast<const i4v*>(src + min(r + e, a.splits - 1) * plane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (r + e < a.splits) s += v4[e];
+    }
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const int nc = min(n + c, a.N - 1);
@@ -340,42 +373,43 @@ __global__ __launch_bounds__(kBlock) void k_w8_join(W8Args a) {
   st_quad(a, m, n, v[0]);
 }
 
-// K = 0: the sums are empty.
+// K < 16 (0: the sums are empty): one output per thread, code by code.
 template <int ACT>
-__global__ __launch_bounds__(kBlock) void k_w8_empty(W8Args a) {
+__global__ __launch_bounds__(kBlock) void k_w8_short(W8Args a) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
   if (i >= static_cast<int64_t>(a.M) * a.N) return;
   const int64_t m = i / a.N, n = i - m * a.N;
   const float sx = a.sx[m * a.sx_step];
   auto one = [&](int p) {
-    return scaled(0, sx, a.sw[p][n * a.sw_step[p]], a.bias[p] ? ld_any(a.bias[p], a.bias_dt, n) : 0.0f);
+    int sum = 0;
+    for (int k = 0; k < a.K; ++k)
+      sum += static_cast<int8_t>(a.x[m * a.ldx + k]) * static_cast<int8_t>(a.w[p][n * a.ldw[p] + k]);
+    return scaled(sum, sx, a.sw[p][n * a.sw_step[p]], a.bias[p] ? ld_any(a.bias[p], a.bias_dt, n) : 0.0f);
   };
   float v = one(0);
   if constexpr (ACT != kNoAct) v = activate<ACT>(v) * one(1);
   st_any(a.y, a.out_dt, i, v);
 }
 
-// Rows of K codes, ld bytes apart, as rows of kp bytes (a multiple of 64) with
-// zeros behind them. One thread per 16 bytes of the result.
-__global__ __launch_bounds__(kBlock) void k_w8_pad(const uint8_t* __restrict__ src, int64_t ld,
-                                                   int64_t rows, int K, int64_t kp,
-                                                   uint8_t* __restrict__ dst) {
-  typedef u32x4 __attribute__((aligned(1))) u32x4_any;
-  const int64_t cpr = kp >> 4;
+// Copies of x's rows and the weights' in rows of kp bytes (a multiple of 16), with
+// zeros behind K: one launch for all, a thread per 16 bytes of the result.
+struct W8Pad {
+  const uint8_t* src[3];
+  int64_t ld[3], first[4];   // first thread of each operand's copy, and the end
+  uint8_t* dst;              // the copies, one behind the other
+  int kp, K;
+};
+
+__global__ __launch_bounds__(kBlock) void k_w8_pad(W8Pad a) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
-  if (i >= rows * cpr) return;
-  const int64_t r = i / cpr;
-  const int k = static_cast<int>(i - r * cpr) * 16;
-  const uint8_t* p = src + r * ld + k;
-  u32x4 v = {0u, 0u, 0u, 0u};
-  if (k + 16 <= K) {
-    v = *reinterpret_cast<const u32x4_any*>(p);
-  } else {
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-    for (int j = 0; k + j < K; ++j) w[j >> 2] |= static_cast<uint32_t>(p[j]) << (8 * (j & 3));
-    v = u32x4{w[0], w[1], w[2], w[3]};
-  }
-  *reinterpret_cast<u32x4*>(dst + i * 16) = v;
+  if (i >= a.first[3]) return;
+  const int o = i >= a.first[2] ? 2 : i >= a.first[1] ? 1 : 0;
+  const int cpr = a.kp >> 4;
+  const int64_t c = i - (o == 2 ? a.first[2] : o ? a.first[1] : 0), r = c / cpr;
+  const int k = static_cast<int>(c - r * cpr) * 16;
+  const uint8_t* row = (o == 2 ? a.src[2] : o ? a.src[1] : a.src[0]) +
+                       r * (o == 2 ? a.ld[2] : o ? a.ld[1] : a.ld[0]);
+  *reinterpret_cast<u32x4*>(a.dst + i * 16) = from_k(ld_codes(row, k, a.K), k, a.K);
 }
 
 // ---------------------------------------------------------------------------
@@ -383,76 +417,115 @@ __global__ __launch_bounds__(kBlock) void k_w8_pad(const uint8_t* __restrict__ s
 // ---------------------------------------------------------------------------
 size_t align256(size_t v) { return (v + 255) & ~static_cast<size_t>(255); }
 
+// The tiles: 256 x 256, 192 x 256 and 128 x 128, the last with four stages or, two
+// workgroups per CU, with two.
+enum { kT256, kT192, kT128, kT128x2, kTiles };
+constexpr int kTileJ[] = {4, 3, 2, 2}, kTileI[] = {4, 4, 2, 2};
+
 struct W8Plan {
   int tile, splits, split_steps;
-  int64_t ldp;               // columns of a plane of sums, a multiple of the tile's
-  int64_t kp;                // K padded to whole steps
-  size_t x_off, w_off[2], part_off, bytes;
+  bool pad;                  // x and the weights are copied to rows of kp bytes first
+  int64_t kp, ldp;           // ldp: columns of a plane of sums, a multiple of the tile's
+  size_t part_off, bytes;
 };
 
-// Tile and ranges of K: the pair with the lowest modelled time.
-void w8_choose(int64_t M, int64_t N, int64_t nk, int proj, int& tile, int& splits) {
-  const int64_t cus = device_cus();
-  tile = 256;
-  splits = 1;
-  int64_t best = -1;
-  for (int t : {256, 128}) {
-    const int64_t tiles = cdiv(M, t) * cdiv(N, t / proj);
-    const int64_t step = t == 256 ? 70 : 35;
-    const int64_t max_wg = t == 256 ? cus : 2 * cus;
-    for (int64_t sp = 1; sp <= 16; ++sp) {
-      if (sp > 1 && (tiles * sp > max_wg || nk / sp < 4)) break;
-      int64_t cost = step * cdiv(nk, sp) * cdiv(tiles * sp, cus);
-      if (sp > 1) cost += 9 * cdiv(sp * M * N * proj * 4, 262144) + 400;
-      if (best < 0 || cost < best) {
-        best = cost;
-        tile = t;
-        splits = static_cast<int>(sp);
+// Modelled time in us of `tiles` tiles of steps_all k-steps, cut into sp ranges, for out
+// sums (of both projections). A k-step takes longer the more CUs are busy (clock and
+// bandwidth), a round adds the first loads and the outputs, ranges add a launch and
+// their sums' traffic. Fitted to timings on MI355X (M = 130 .. 4096, N = 1024 .. 28672,
+// K = 1024 .. 11008, one and two projections, 1 to 8 ranges): 9800 with aligned rows, of
+// which it is 7% off rms, and what it picks is 0.8% slower on average than the best;
+// 5700 without alignment, 7% and 1.5%.
+struct W8Model { double step[kTiles], busy[kTiles], round[kTiles], two, call, join, sum; };
+constexpr W8Model kAligned = {{1.13, 0.88, 0.35, 0.48}, {0.49, 0.39, 0.17, 0.215}, {7.4, 6.3, 3.3, 2.7},
+                              1.07, 3.0, 3.3, 1e-6};
+constexpr W8Model kUnaligned = {{2.12, 0, 0, 0.85}, {0.41, 0, 0, 0.40}, {6.9, 0, 0, 1.1}, 2.0, 6.3, 3.0, 0.86e-6};
+
+double w8_time(const W8Model& f, int tile, int64_t tiles, int64_t steps_all, int64_t out, int64_t sp, double cus) {
+  const double wgs = static_cast<double>(tiles * sp), steps = static_cast<double>(cdiv(steps_all, sp));
+  double t = f.call;
+  auto once = [&](double n) { return steps * (f.step[tile] + f.busy[tile] * std::min(1.0, n / cus)) + f.round[tile]; };
+  if (tile != kT128x2) {
+    t += std::ceil(wgs / cus) * once(wgs);
+  } else {   // two: a step of both workgroups of a CU
+    const double full = std::floor(wgs / (2 * cus)), rem = wgs - full * 2 * cus;
+    t += full * (steps * f.two + f.round[tile]);
+    if (rem > cus) t += once(cus) + steps * (f.two - f.step[tile] - f.busy[tile]) * (rem - cus) / cus;
+    else if (rem > 0) t += once(rem);
+  }
+  return sp > 1 ? t + f.join + f.sum * static_cast<double>(sp * out) : t;
+}
+
+// any: rows that the DMA does not take. room: bytes of workspace, or all that is wanted.
+W8Plan w8_plan(int64_t M, int64_t N, int64_t K, int proj, bool any, size_t room = ~static_cast<size_t>(0)) {
+  const int cus = device_cus();
+  const int64_t steps = cdiv(K, 128);
+  W8Plan p = {};
+  p.kp = cdiv(K, 16) * 16;
+  p.part_off = CBQ_WS_CTRL_BYTES;
+  // The copies read and write M K + N K bytes at 4 TB/s and take a launch; the tiles win
+  // that back from about 640 tokens on.
+  const size_t copies = align256(static_cast<size_t>(M + proj * N) * p.kp);
+  p.pad = any && M >= 640 && p.part_off + copies <= room;
+  if (p.pad) p.part_off += copies;
+  any = any && !p.pad;
+  double best = -1;
+  for (int tile = 0; tile < kTiles; ++tile) {
+    if (any && (tile == kT192 || tile == kT128)) continue;
+    const int64_t tiles = cdiv(M, 64 * kTileJ[tile]) * cdiv(N, 64 * kTileI[tile] / proj);
+    const int tn = 64 * kTileI[tile] / proj;
+    const int64_t ldp = cdiv(N, tn) * tn;
+    for (int64_t sp = 1; sp <= 8; ++sp) {
+      const size_t bytes = p.part_off + (sp > 1 ? align256(static_cast<size_t>(sp * proj * M * ldp) * 4) : 0);
+      if (sp > 1 && (tiles * sp > (tile == kT128x2 ? 2 : 1) * cus || steps / sp < 3 || bytes > room)) break;
+      const double t = w8_time(any ? kUnaligned : kAligned, tile, tiles, steps, proj * M * N, sp, cus);
+      if (best < 0 || t < best) {
+        best = t;
+        p.tile = tile;
+        p.splits = static_cast<int>(sp);
+        p.ldp = ldp;
+        p.bytes = bytes;
       }
     }
   }
-}
-
-// pad: x and the weights are copied to padded rows.
-W8Plan w8_plan(int64_t M, int64_t N, int64_t K, int proj, bool pad) {
-  W8Plan p;
-  p.kp = cdiv(K, 64) * 64;
-  size_t off = CBQ_WS_CTRL_BYTES;
-  p.x_off = p.w_off[0] = p.w_off[1] = off;
-  if (pad) {
-    off = align256(off + static_cast<size_t>(M) * p.kp);
-    for (int i = 0; i < proj; ++i) {
-      p.w_off[i] = off;
-      off = align256(off + static_cast<size_t>(N) * p.kp);
-    }
-  }
-  const int64_t steps = pad ? p.kp / 64 : K / 64;
-  w8_choose(M, N, steps, proj, p.tile, p.splits);
-  p.split_steps = static_cast<int>(steps);
-  if (p.splits > 1) {
-    p.split_steps = static_cast<int>(cdiv(steps, p.splits));
-    p.splits = static_cast<int>(cdiv(steps, p.split_steps));   // no empty ranges
-  }
-  p.ldp = cdiv(N, p.tile / proj) * (p.tile / proj);
-  p.part_off = off;
-  if (p.splits > 1) off = align256(off + static_cast<size_t>(p.splits) * proj * M * p.ldp * 4);
-  p.bytes = off;
+  p.split_steps = static_cast<int>(cdiv(steps, p.splits));
+  p.splits = static_cast<int>(cdiv(steps, p.split_steps));   // no empty ranges
   return p;
 }
 
+// cbq_w8a8_few.hip takes up to 64 rows, and up to 128 where x, which all of its
+// workgroups read, is small: at M = 128 (us, there / here) N = K = 4096 11 / 17, N =
+// 4096, K = 8192 20 / 19, N = 11008, K = 4096 20 / 20, N = 28672, K = 8192 78 / 72.
+bool few_rows(int64_t M, int64_t N, int64_t K) {
+  return M <= 64 || (M <= kFewRows && N <= 16 * device_cus() && K <= 6144);
+}
+
+template <int J, int I, int NS, int ACT>
+void launch_tile(const W8Args& a, bool any, hipStream_t s) {
+  const unsigned grid = static_cast<unsigned>(a.tiles_m) * a.tiles_n * a.splits;
+  constexpr int RAW = ACT == kNoAct ? kNoAct : CBQ_ACT_RELU;   // sums do not depend on it
+  if constexpr (NS == 2 && J != 3) {
+    if (any) {
+      if (a.splits > 1) k_w8_tile<J, I, 2, RAW, true, true><<<grid, 256, 0, s>>>(a);
+      else k_w8_tile<J, I, 2, ACT, false, true><<<grid, 256, 0, s>>>(a);
+      return;
+    }
+  }
+  if (a.splits > 1) k_w8_tile<J, I, NS, RAW, true, false><<<grid, 256, 0, s>>>(a);
+  else k_w8_tile<J, I, NS, ACT, false, false><<<grid, 256, 0, s>>>(a);
+}
+
 template <int ACT>
-void launch_tiles(const W8Args& a, int tile, hipStream_t s) {
-  const unsigned tiles = static_cast<unsigned>(a.tiles_m) * a.tiles_n;
-  constexpr int RAW = ACT == kNoAct ? kNoAct : CBQ_ACT_RELU;   // the sums do not depend on it
+void launch_tiles(const W8Args& a, int tile, bool any, hipStream_t s) {
+  switch (tile) {
+    case kT256: launch_tile<4, 4, 2, ACT>(a, any, s); break;
+    case kT192: launch_tile<3, 4, 2, ACT>(a, false, s); break;
+    case kT128x2: launch_tile<2, 2, 2, ACT>(a, any, s); break;
+    default: launch_tile<2, 2, 4, ACT>(a, false, s); break;
+  }
   if (a.splits > 1) {
-    if (tile == 256) k_w8_tile<256, RAW, true><<<tiles * a.splits, W8Geom<256>::kThreads, 0, s>>>(a);
-    else k_w8_tile<128, RAW, true><<<tiles * a.splits, W8Geom<128>::kThreads, 0, s>>>(a);
     const int64_t quads = static_cast<int64_t>(a.M) * ((a.N + 3) / 4);
     k_w8_join<ACT><<<static_cast<unsigned>(cdiv(quads, kBlock)), kBlock, 0, s>>>(a);
-  } else if (tile == 256) {
-    k_w8_tile<256, ACT, false><<<tiles, W8Geom<256>::kThreads, 0, s>>>(a);
-  } else {
-    k_w8_tile<128, ACT, false><<<tiles, W8Geom<128>::kThreads, 0, s>>>(a);
   }
 }
 
@@ -495,14 +568,14 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
   a.ldx = x->stride;
   a.sx = x->scale;
   a.sx_step = x->scale_stride;
-  bool pad = K % 16 || !even16(*x);
+  bool any = K % 16 || !even16(*x);
   for (int p = 0; p < proj; ++p) {
     a.w[p] = reinterpret_cast<const uint8_t*>(w[p]->data);
     a.ldw[p] = w[p]->stride;
     a.sw[p] = w[p]->scale;
     a.sw_step[p] = w[p]->scale_stride;
     a.bias[p] = bias[p];
-    pad = pad || !even16(*w[p]);
+    any = any || !even16(*w[p]);
   }
   a.bias_dt = bias_dtype;
   a.act = act;
@@ -514,47 +587,43 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
   a.K = static_cast<int>(K);
   a.splits = 1;
   hipStream_t s = as_stream(stream);
-  if (K == 0) {
+  if (K < 16) {
     CBQ_REQUIRE(cdiv(M * N, kBlock) < (1LL << 31), "%s: too many outputs", what);
     with_act(act, [&](auto c) {
-      k_w8_empty<decltype(c)::value><<<static_cast<unsigned>(cdiv(M * N, kBlock)), kBlock, 0, s>>>(a);
+      k_w8_short<decltype(c)::value><<<static_cast<unsigned>(cdiv(M * N, kBlock)), kBlock, 0, s>>>(a);
     });
     return launch_status(what);
   }
-  if (M <= kFewRows) {
+  if (few_rows(M, N, K)) {
     launch_w8a8_few(a, s);
     return launch_status(what);
   }
-  W8Plan p = w8_plan(M, N, K, proj, pad);
-  const bool ws_ok = ws && aligned(ws, 256) && ws_bytes >= p.bytes;
-  CBQ_REQUIRE(ws_ok || !pad, "%s: K, strides and addresses that are no multiples of 16 need a workspace of "
-              "%zu bytes, 256-byte aligned", what, p.bytes);
-  if (!ws_ok && p.splits > 1) {
-    p.splits = 1;
-    p.split_steps = static_cast<int>(K / 64);
-  }
-  a.tiles_m = static_cast<int>(cdiv(M, p.tile));
-  a.tiles_n = static_cast<int>(cdiv(N, p.tile / proj));
-  CBQ_REQUIRE(static_cast<int64_t>(a.tiles_m) * a.tiles_n * p.splits < (1LL << 31) &&
-                  cdiv(M * cdiv(N, 4), kBlock) < (1LL << 31), "%s: too many tiles", what);
+  const W8Plan p = w8_plan(M, N, K, proj, any, ws && aligned(ws, 256) ? ws_bytes : 0);
+  const int64_t tiles_m = cdiv(M, 64 * kTileJ[p.tile]), tiles_n = cdiv(N, 64 * kTileI[p.tile] / proj);
+  CBQ_REQUIRE(tiles_m * tiles_n * p.splits < (1LL << 31), "%s: too many tiles", what);
+  a.tiles_m = static_cast<int>(tiles_m);
+  a.tiles_n = static_cast<int>(tiles_n);
   a.splits = p.splits;
   a.split_steps = p.split_steps;
-  uint8_t* base = static_cast<uint8_t*>(ws);
-  if (pad) {
-    auto copy = [&](const uint8_t*& src, int64_t& ld, int64_t rows, size_t off) {
-      const int64_t n = rows * (p.kp / 16);
-      k_w8_pad<<<static_cast<unsigned>(cdiv(n, kBlock)), kBlock, 0, s>>>(src, ld, rows, a.K, p.kp, base + off);
-      src = base + off;
-      ld = p.kp;
-    };
-    CBQ_REQUIRE(cdiv((M > N ? M : N) * (p.kp / 16), kBlock) < (1LL << 31), "%s: too many rows", what);
-    copy(a.x, a.ldx, M, p.x_off);
-    for (int i = 0; i < proj; ++i) copy(a.w[i], a.ldw[i], N, p.w_off[i]);
-    a.K = static_cast<int>(p.kp);
-  }
-  a.part = reinterpret_cast<int*>(base + p.part_off);
   a.ldp = p.ldp;
-  with_act(act, [&](auto c) { launch_tiles<decltype(c)::value>(a, p.tile, s); });
+  uint8_t* const w0 = static_cast<uint8_t*>(ws);
+  if (p.pad) {
+    W8Pad c = {{a.x, a.w[0], a.w[1]}, {a.ldx, a.ldw[0], a.ldw[1]}, {}, w0 + CBQ_WS_CTRL_BYTES,
+               static_cast<int>(p.kp), a.K};
+    const int64_t rows[3] = {M, N, proj == 2 ? N : 0};
+    for (int o = 0; o < 3; ++o) c.first[o + 1] = c.first[o] + rows[o] * (p.kp / 16);
+    const int64_t grid = cdiv(c.first[3], kBlock);
+    CBQ_REQUIRE(grid < (1LL << 31), "%s: too many rows", what);
+    k_w8_pad<<<static_cast<unsigned>(grid), kBlock, 0, s>>>(c);
+    a.x = c.dst;
+    a.w[0] = c.dst + c.first[1] * 16;
+    a.w[1] = c.dst + c.first[2] * 16;
+    a.ldx = a.ldw[0] = a.ldw[1] = p.kp;
+    a.K = static_cast<int>(p.kp);   // zeros behind K
+    any = false;
+  }
+  if (p.splits > 1) a.part = reinterpret_cast<int*>(w0 + p.part_off);
+  with_act(act, [&](auto c) { launch_tiles<decltype(c)::value>(a, p.tile, any, s); });
   return launch_status(what);
 }
 
@@ -564,7 +633,7 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
 using namespace cbq;
 
 extern "C" size_t cbq_w8a8_ws_bytes(int64_t M, int64_t N, int64_t K, int projections) {
-  if (M <= kFewRows || N <= 0 || K <= 0 || K > 131071 || projections < 1 || projections > 2)
+  if (M <= 0 || N <= 0 || K < 16 || K > 131071 || projections < 1 || projections > 2 || few_rows(M, N, K))
     return CBQ_WS_CTRL_BYTES;
   return w8_plan(M, N, K, projections, K % 16 != 0).bytes;
 }

@@ -31,17 +31,18 @@ typedef struct {
 enum { CBQ_ACT_SILU = 0, CBQ_ACT_GELU = 1, CBQ_ACT_GELU_TANH = 2, CBQ_ACT_RELU = 3 };
 
 /* y[m, n] = sx[m] sw[n] (sum_k x[m, k] w[n, k]) + bias[n]
- * x: M rows, w: N rows, of K codes; K <= 131071, so that the int32 sums are
+ * x: M rows, w: N rows, of K codes (strides up to 2^22); K <= 131071, so that the int32 sums are
  * exact for any codes. y: [M, N] in out_dtype, contiguous. bias (or null): [N]
  * in bias_dtype. The sum becomes fp32 (rounded once past 2^24), the rest is
  * fp32 with each product and sum rounded, then one rounding to out_dtype.
  *
  * ws: cbq_w8a8_ws_bytes(M, N, K, 1) bytes, 256-byte aligned, of which the
- * control block is not used. Less is allowed where K and both strides are
- * multiples of 16 and the codes 16-byte aligned, or M <= 64: K is then split
- * less (same results, slower). Codes pass through ws from one kernel of a call
- * to the next: host threads that share a ws on a stream make their calls one
- * at a time. */
+ * control block is not used. With less, or none, K is not cut into ranges, and
+ * rows that are no multiples of 16 bytes are not copied to such (same results,
+ * slower). Sums and copies pass through ws from one kernel of a call to the next:
+ * host threads that share a ws on a stream make their calls one at a time.
+ * Codes may have any alignment; x and w, their strides and K in multiples of 16
+ * bytes are faster. */
 size_t cbq_w8a8_ws_bytes(int64_t M, int64_t N, int64_t K, int projections);
 int cbq_w8a8_linear(const cbq_i8_rows* x, const cbq_i8_rows* w, const void* bias, int bias_dtype,
                     int64_t M, int64_t N, int64_t K, void* y, int out_dtype, void* ws,

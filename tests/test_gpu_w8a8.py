@@ -13,8 +13,9 @@ DT = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
 # kernels (16, 32, 64 rows), columns that fill no block, no step, no 16 bytes
 SHAPES = [(1, 1, 1), (1, 4096, 512), (2, 40, 15), (3, 17, 33), (15, 4100, 272), (16, 9000, 144),
           (17, 100, 1000), (33, 513, 128), (64, 129, 2064), (64, 8200, 130), (65, 128, 64), (65, 1, 16),
-          (65, 7, 17), (100, 300, 48), (127, 255, 4096), (128, 256, 272), (257, 511, 1040),
-          (300, 1001, 1403), (70, 130, 9), (1000, 520, 640), (2100, 2050, 80), (260, 4096, 11008)]
+          (65, 7, 17), (129, 40, 7), (90, 5000, 784), (128, 11008, 400), (120, 9000, 1001), (129, 70, 33),
+          (129, 300, 48), (100, 300, 48), (127, 255, 4096), (128, 256, 272), (257, 511, 1040),
+          (300, 1001, 1403), (70, 130, 9), (1000, 520, 640), (2100, 2050, 80), (700, 300, 1001), (640, 1000, 35), (1100, 4100, 531), (260, 4096, 11008)]
 
 
 def _case(m, n, k, seed, bias, xmode, dtype):
@@ -39,8 +40,9 @@ def test_linear_to_the_last_bit(i, shape):
 
 @pytest.mark.parametrize("act", P.ACTS)
 @pytest.mark.parametrize("shape", [(1, 1, 1), (1, 4100, 528), (5, 33, 17), (16, 9000, 144), (20, 300, 1000),
-                                   (64, 70, 130), (65, 128, 64), (90, 129, 33), (128, 64, 4096),
-                                   (333, 700, 1400), (1030, 1500, 96)])
+                                   (64, 70, 130), (65, 128, 64), (90, 129, 33), (128, 64, 4096), (128, 4200, 528), (40, 9000, 777), (33, 13000, 272), (10, 20000, 130),
+                                   (129, 129, 33), (140, 64, 4096),
+                                   (333, 700, 1400), (700, 300, 1001), (650, 1300, 39), (1030, 1500, 96)])
 def test_gated(shape, act):
     from cublade_amd.quantization import gated_w8a8
     m, n, k = shape
@@ -80,7 +82,7 @@ def test_a_token_does_not_depend_on_its_batch():
     for f in (lambda r: linear_w8a8(P.qt(x[r], sx[r]), P.qt(w, sw)),
               lambda r: gated_w8a8(P.qt(x[r], sx[r]), P.qt(w, sw), P.qt(u, su))):
         whole = f(slice(0, 700))
-        for r in (slice(0, 1), slice(3, 20), slice(100, 164), slice(200, 330)):
+        for r in (slice(0, 1), slice(3, 20), slice(100, 164), slice(30, 150), slice(200, 330)):
             assert torch.equal(f(r), whole[r])
 
 
@@ -88,15 +90,37 @@ def test_strided_rows_and_offsets():
     """Codes as columns of a larger tensor, with and without alignment, and scales
     with strides."""
     from cublade_amd.quantization import linear_w8a8
-    big, _ = P.codes(200, 640, 5)
+    big, _ = P.codes(800, 640, 5)
     wide, _ = P.codes(96, 512, 6)
-    s = torch.rand(400, device="cuda")[::2] * 0.01
-    for m in (3, 64, 200):
+    s = torch.rand(1600, device="cuda")[::2] * 0.01
+    for m in (3, 64, 128, 200, 800):
         for off, k in ((0, 512), (16, 256), (5, 256), (7, 77), (3, 512)):
             x, w = big[:m, off:off + k], wide[:, :k]
             y = linear_w8a8(P.qt(x, s[:m]), P.qt(w, s[:96]))
             want = P.linear(x, s[:m], w, s[:96], None, torch.float16)
             assert torch.equal(y.cpu(), want), (m, off, k)
+
+
+def test_less_workspace_gives_the_same():
+    """Without a workspace K is not cut and unaligned rows are not copied."""
+    import ctypes
+    from cublade_amd import _abi
+    L = _abi.lib()
+    for m, n, k in ((200, 512, 8192), (900, 300, 1403), (700, 260, 11003)):
+        (x, sx), (w, sw) = P.codes(m, k, 1), P.codes(n, k, 2)
+        need = L.cbq_w8a8_ws_bytes(m, n, k, 1)
+        assert need > _abi.WS_CTRL_BYTES
+        rows = [_abi.I8Rows(q.data_ptr(), k, s.data_ptr(), 1) for q, s in ((x, sx), (w, sw))]
+        got = []
+        for nbytes in (0, _abi.WS_CTRL_BYTES, need - 1, need):
+            y = torch.empty(m, n, device="cuda")
+            ws = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device="cuda")
+            assert L.cbq_w8a8_linear(ctypes.byref(rows[0]), ctypes.byref(rows[1]), None, 0, m, n, k,
+                                     y.data_ptr(), 0, ws.data_ptr() if nbytes else None, nbytes,
+                                     _abi.stream_handle(y.device)) == 0
+            got.append(y.cpu())
+        want = P.linear(x, sx, w, sw, None, torch.float32)
+        assert all(torch.equal(y, want) for y in got)
 
 
 def test_empty_sizes():

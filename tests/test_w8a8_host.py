@@ -39,11 +39,11 @@ def test_c_entries_refuse_bad_arguments():
     def rows(data=4096, stride=64, scale=4096, step=1):
         return by(_abi.I8Rows(data, stride, scale, step))
 
-    def linear(x=None, w=None, bias=None, bdt=0, m=100, n=8, k=64, y=4096, out=1, ws=None, nb=0):
+    def linear(x=None, w=None, bias=None, bdt=0, m=200, n=8, k=64, y=4096, out=1, ws=None, nb=0):
         return L.cbq_w8a8_linear(x or rows(), w or rows(), bias, bdt, m, n, k, y, out, ws, nb, None)
 
     def gated(gate=None, up=None, act=0, **kw):
-        a = dict(m=100, n=8, k=64, out=1)
+        a = dict(m=200, n=8, k=64, out=1)
         a.update(kw)
         return L.cbq_w8a8_gated(rows(), gate or rows(), up or rows(), None, None, 0, act, a["m"],
                                 a["n"], a["k"], 4096, a["out"], None, 0, None)
@@ -60,10 +60,6 @@ def test_c_entries_refuse_bad_arguments():
     _refused(linear(x=rows(step=2)), "scale_stride")
     _refused(linear(y=None), "y is null")
     _refused(linear(y=4097), "aligned")
-    # more than 64 rows that are not 16-byte aligned pass through the workspace
-    for bad in (dict(k=60), dict(x=rows(data=4100)), dict(w=rows(stride=72))):
-        _refused(linear(**bad), "workspace")
-        _refused(linear(ws=4096, nb=16384, **bad), "workspace")
     _refused(gated(act=4), "activation")
     _refused(gated(act=-1), "activation")
     _refused(gated(up=rows(scale=None)), "up has a null")
@@ -124,12 +120,17 @@ def test_norms_on_the_host():
 def test_workspace_sizes():
     _abi, L = _L()
     C = _abi.WS_CTRL_BYTES
-    assert L.cbq_w8a8_ws_bytes(64, 11008, 4096, 1) == C          # few rows: none
+    assert L.cbq_w8a8_ws_bytes(64, 11008, 4096, 1) == C           # few rows: none
+    assert L.cbq_w8a8_ws_bytes(128, 4096, 4096, 2) == C
     assert L.cbq_w8a8_ws_bytes(4096, 28672, 8192, 1) == C        # tiles enough for every CU
-    assert L.cbq_w8a8_ws_bytes(0, 8, 8, 1) == C and L.cbq_w8a8_ws_bytes(100, 8, 0, 2) == C
-    # rows of 1403 codes are copied to rows of 1408
-    assert L.cbq_w8a8_ws_bytes(4096, 8192, 1403, 1) >= C + 1408 * (4096 + 8192)
-    assert L.cbq_w8a8_ws_bytes(4096, 8192, 1403, 2) >= C + 1408 * (4096 + 2 * 8192)
+    assert L.cbq_w8a8_ws_bytes(0, 8, 8, 1) == C and L.cbq_w8a8_ws_bytes(1000, 8, 0, 2) == C
+    # many tokens with rows of 1403 codes: copies in rows of 1408
+    for p in (1, 2):
+        assert L.cbq_w8a8_ws_bytes(4096, 8192, 1403, p) == C + 1408 * (4096 + p * 8192)
+    # few tiles of long rows: planes of int32 sums, for each projection
+    one, two = (L.cbq_w8a8_ws_bytes(200, 1024, 11008, p) - C for p in (1, 2))
+    assert one % (200 * 1024 * 4) == 0 and two % (2 * 200 * 1024 * 4) == 0
+    assert 2 <= one // (200 * 1024 * 4) <= 8 and 2 <= two // (2 * 200 * 1024 * 4) <= 8
 
 
 def test_quantized_operands_are_checked():
