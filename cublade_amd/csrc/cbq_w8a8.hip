@@ -22,9 +22,9 @@
 // time per wave, and are stored 16 bytes per lane along a row.
 //
 // ANY: rows that are no multiples of 16 bytes, which the DMA does not take. They pass
-// through registers, loaded a k-step ahead: 1.0 us a k-step of 128 x 128 instead of 0.5
-// (loads from the multiple of 4 in front, shifted by the vector unit: 1.7). From 1024
-// tokens on, copies in rows that the DMA takes cost less (k_w8_pad).
+// through registers, loaded a k-step ahead: a k-step of 128 x 128 takes 0.9 us where rows
+// are whole words and 1.2 where not, instead of 0.6 (loads from the multiple of 4 in
+// front, shifted by the vector unit: 1.7). Many tokens: k_w8_pad.
 //
 // K is cut into ranges where few tiles would leave CUs idle: each range writes its
 // sums to the workspace and k_w8_join adds them (integers: exact in any order).
@@ -433,13 +433,15 @@ struct W8Plan {
 // sums (of both projections). A k-step takes longer the more CUs are busy (clock and
 // bandwidth), a round adds the first loads and the outputs, ranges add a launch and
 // their sums' traffic. Fitted to timings on MI355X (M = 130 .. 4096, N = 1024 .. 28672,
-// K = 1024 .. 11008, one and two projections, 1 to 8 ranges): 9800 with aligned rows, of
-// which it is 7% off rms, and what it picks is 0.8% slower on average than the best;
-// 5700 without alignment, 7% and 1.5%.
+// K = 1024 .. 11008, one and two projections, 1 to 8 ranges of K): 9800 with aligned rows
+// (7% off rms; what it picks is 0.8% slower on average than the best), 5700 each with
+// rows of whole words and with others (8% and 7%; 1.6% and 1.5%).
 struct W8Model { double step[kTiles], busy[kTiles], round[kTiles], two, call, join, sum; };
-constexpr W8Model kAligned = {{1.13, 0.88, 0.35, 0.48}, {0.49, 0.39, 0.17, 0.215}, {7.4, 6.3, 3.3, 2.7},
-                              1.07, 3.0, 3.3, 1e-6};
-constexpr W8Model kUnaligned = {{2.12, 0, 0, 0.85}, {0.41, 0, 0, 0.40}, {6.9, 0, 0, 1.1}, 2.0, 6.3, 3.0, 0.86e-6};
+enum { kRows16, kRows4, kRows1 };   // what rows and their strides are multiples of
+constexpr W8Model kModels[] = {
+    {{1.13, 0.88, 0.35, 0.48}, {0.49, 0.39, 0.17, 0.215}, {7.4, 6.3, 3.3, 2.7}, 1.07, 3.0, 3.3, 1e-6},
+    {{1.69, 0, 0, 0.62}, {0.51, 0, 0, 0.29}, {7.0, 0, 0, 2.6}, 1.46, 3.9, 3.0, 1e-6},
+    {{2.12, 0, 0, 0.85}, {0.41, 0, 0, 0.40}, {6.9, 0, 0, 1.1}, 2.0, 6.3, 3.0, 0.86e-6}};
 
 double w8_time(const W8Model& f, int tile, int64_t tiles, int64_t steps_all, int64_t out, int64_t sp, double cus) {
   const double wgs = static_cast<double>(tiles * sp), steps = static_cast<double>(cdiv(steps_all, sp));
@@ -456,29 +458,31 @@ double w8_time(const W8Model& f, int tile, int64_t tiles, int64_t steps_all, int
   return sp > 1 ? t + f.join + f.sum * static_cast<double>(sp * out) : t;
 }
 
-// any: rows that the DMA does not take. room: bytes of workspace, or all that is wanted.
-W8Plan w8_plan(int64_t M, int64_t N, int64_t K, int proj, bool any, size_t room = ~static_cast<size_t>(0)) {
+// room: bytes of workspace, or all that is wanted.
+W8Plan w8_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, size_t room = ~static_cast<size_t>(0)) {
   const int cus = device_cus();
   const int64_t steps = cdiv(K, 128);
   W8Plan p = {};
   p.kp = cdiv(K, 16) * 16;
   p.part_off = CBQ_WS_CTRL_BYTES;
-  // The copies read and write M K + N K bytes at 4 TB/s and take a launch; the tiles win
-  // that back from about 640 tokens on.
+  // Copies read and write M K + N K bytes at 4 TB/s and take a launch. Where rows are no
+  // whole words the tiles win that back from about 640 tokens on, else hardly ever.
   const size_t copies = align256(static_cast<size_t>(M + proj * N) * p.kp);
-  p.pad = any && M >= 640 && p.part_off + copies <= room;
-  if (p.pad) p.part_off += copies;
-  any = any && !p.pad;
+  p.pad = rows == kRows1 && M >= 640 && p.part_off + copies <= room;
+  if (p.pad) {
+    p.part_off += copies;
+    rows = kRows16;
+  }
   double best = -1;
   for (int tile = 0; tile < kTiles; ++tile) {
-    if (any && (tile == kT192 || tile == kT128)) continue;
+    if (rows != kRows16 && (tile == kT192 || tile == kT128)) continue;
     const int64_t tiles = cdiv(M, 64 * kTileJ[tile]) * cdiv(N, 64 * kTileI[tile] / proj);
     const int tn = 64 * kTileI[tile] / proj;
     const int64_t ldp = cdiv(N, tn) * tn;
     for (int64_t sp = 1; sp <= 8; ++sp) {
       const size_t bytes = p.part_off + (sp > 1 ? align256(static_cast<size_t>(sp * proj * M * ldp) * 4) : 0);
       if (sp > 1 && (tiles * sp > (tile == kT128x2 ? 2 : 1) * cus || steps / sp < 3 || bytes > room)) break;
-      const double t = w8_time(any ? kUnaligned : kAligned, tile, tiles, steps, proj * M * N, sp, cus);
+      const double t = w8_time(kModels[rows], tile, tiles, steps, proj * M * N, sp, cus);
       if (best < 0 || t < best) {
         best = t;
         p.tile = tile;
@@ -541,7 +545,11 @@ int check_rows(const char* what, const char* name, const cbq_i8_rows* r, int64_t
   return CBQ_OK;
 }
 
-bool even16(const cbq_i8_rows& r) { return r.stride % 16 == 0 && aligned(r.data, 16); }
+// What rows of K codes are multiples of.
+int rows_of(const cbq_i8_rows& r, int64_t K) {
+  const uint64_t all = reinterpret_cast<uintptr_t>(r.data) | static_cast<uint64_t>(r.stride) | static_cast<uint64_t>(K);
+  return all % 16 == 0 ? kRows16 : all % 4 == 0 ? kRows4 : kRows1;
+}
 
 int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)[2], int proj,
            const void* const (&bias)[2], int bias_dtype, int act, int64_t M, int64_t N, int64_t K,
@@ -568,14 +576,14 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
   a.ldx = x->stride;
   a.sx = x->scale;
   a.sx_step = x->scale_stride;
-  bool any = K % 16 || !even16(*x);
+  int rows = rows_of(*x, K);
   for (int p = 0; p < proj; ++p) {
     a.w[p] = reinterpret_cast<const uint8_t*>(w[p]->data);
     a.ldw[p] = w[p]->stride;
     a.sw[p] = w[p]->scale;
     a.sw_step[p] = w[p]->scale_stride;
     a.bias[p] = bias[p];
-    any = any || !even16(*w[p]);
+    rows = std::max(rows, rows_of(*w[p], K));
   }
   a.bias_dt = bias_dtype;
   a.act = act;
@@ -598,7 +606,7 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
     launch_w8a8_few(a, s);
     return launch_status(what);
   }
-  const W8Plan p = w8_plan(M, N, K, proj, any, ws && aligned(ws, 256) ? ws_bytes : 0);
+  const W8Plan p = w8_plan(M, N, K, proj, rows, ws && aligned(ws, 256) ? ws_bytes : 0);
   const int64_t tiles_m = cdiv(M, 64 * kTileJ[p.tile]), tiles_n = cdiv(N, 64 * kTileI[p.tile] / proj);
   CBQ_REQUIRE(tiles_m * tiles_n * p.splits < (1LL << 31), "%s: too many tiles", what);
   a.tiles_m = static_cast<int>(tiles_m);
@@ -610,8 +618,8 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
   if (p.pad) {
     W8Pad c = {{a.x, a.w[0], a.w[1]}, {a.ldx, a.ldw[0], a.ldw[1]}, {}, w0 + CBQ_WS_CTRL_BYTES,
                static_cast<int>(p.kp), a.K};
-    const int64_t rows[3] = {M, N, proj == 2 ? N : 0};
-    for (int o = 0; o < 3; ++o) c.first[o + 1] = c.first[o] + rows[o] * (p.kp / 16);
+    const int64_t count[3] = {M, N, proj == 2 ? N : 0};
+    for (int o = 0; o < 3; ++o) c.first[o + 1] = c.first[o] + count[o] * (p.kp / 16);
     const int64_t grid = cdiv(c.first[3], kBlock);
     CBQ_REQUIRE(grid < (1LL << 31), "%s: too many rows", what);
     k_w8_pad<<<static_cast<unsigned>(grid), kBlock, 0, s>>>(c);
@@ -620,10 +628,10 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
     a.w[1] = c.dst + c.first[2] * 16;
     a.ldx = a.ldw[0] = a.ldw[1] = p.kp;
     a.K = static_cast<int>(p.kp);   // zeros behind K
-    any = false;
+    rows = kRows16;
   }
   if (p.splits > 1) a.part = reinterpret_cast<int*>(w0 + p.part_off);
-  with_act(act, [&](auto c) { launch_tiles<decltype(c)::value>(a, p.tile, any, s); });
+  with_act(act, [&](auto c) { launch_tiles<decltype(c)::value>(a, p.tile, rows != kRows16, s); });
   return launch_status(what);
 }
 
@@ -635,7 +643,7 @@ using namespace cbq;
 extern "C" size_t cbq_w8a8_ws_bytes(int64_t M, int64_t N, int64_t K, int projections) {
   if (M <= 0 || N <= 0 || K < 16 || K > 131071 || projections < 1 || projections > 2 || few_rows(M, N, K))
     return CBQ_WS_CTRL_BYTES;
-  return w8_plan(M, N, K, projections, K % 16 != 0).bytes;
+  return w8_plan(M, N, K, projections, K % 16 == 0 ? kRows16 : K % 4 == 0 ? kRows4 : kRows1).bytes;
 }
 
 extern "C" int cbq_w8a8_linear(const cbq_i8_rows* x, const cbq_i8_rows* w, const void* bias,
