@@ -31,8 +31,7 @@ struct W8Args {
   int M, N, K;
   int tiles_m, tiles_n;
   int splits, split_steps; // K in ranges of split_steps 64-byte steps
-  int* part;               // sums of the ranges: [splits][projections][M][ldp]
-  int64_t ldp;
+  int* part;               // sums of the ranges: [splits][tiles], as the tiles' registers hold them
 };
 
 // act(g) in fp32. The sigmoids take the hardware's 2^x and reciprocal (1 ulp

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void k_w8_tile(W8Args a) {
   constexpr int LX = G::kLX, LT = G::kLX + G::kLW, NW = G::kWaves;
   constexpr int WM = 32 * J, WR = 32 * I;               // a wave's tokens, weight rows
   constexpr int WN = GATED ? WR / 2 : WR;               // and output columns
-  constexpr int IO = GATED && !SPLIT ? I / 2 : I;       // 32-column tiles it puts out
+  constexpr int IO = GATED ? I / 2 : I;                 // 32-column tiles it puts out
   __shared__ __attribute__((aligned(1024))) uint8_t smem[NS * G::kSB];
   __shared__ __attribute__((aligned(16))) float s_x[G::kTM], s_w[G::kTN], s_b[G::kTN];
 
@@ -252,6 +252,22 @@ __global__ __launch_bounds__(256) void k_w8_tile(W8Args a) {
     });
   }
 
+  // A range's sums go to the workspace as they lie in registers, 1 KiB per store.
+  if constexpr (SPLIT) {
+    i4v* dst = reinterpret_cast<i4v*>(a.part) +
+               ((static_cast<int64_t>(split) * tiles + tm * a.tiles_n + tn) * NW + wave) * (J * I * 256) + lane;
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          __builtin_nontemporal_store(
+              i4v{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]},
+              dst + ((j * I + i) * 4 + q) * 64);
+    return;
+  }
+
   // Outputs: 32 tokens at a time through the wave's own part of LDS.
   __syncthreads();
   uint8_t* const out = smem + wave * 32 * G::kPitch;
@@ -259,48 +275,29 @@ __global__ __launch_bounds__(256) void k_w8_tile(W8Args a) {
 #pragma unroll
   for (int j = 0; j < J; ++j) {
     const int mj = mw + 32 * j;
-    const float sx = SPLIT ? 0.0f : s_x[wm * WM + 32 * j + r32];
+    const float sx = s_x[wm * WM + 32 * j + r32];
     wave_lds_fence();                                   // the last rows are read
 #pragma unroll
     for (int i = 0; i < IO; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int c = 32 * i + 8 * q + 4 * h;           // the wave's column of 4 outputs
-        i4v bits;
-        if constexpr (SPLIT) {
+        const f4v w0 = *reinterpret_cast<const f4v*>(s_w + wn * WR + c);
+        const f4v b0 = *reinterpret_cast<const f4v*>(s_b + wn * WR + c);
+        f4v v;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) bits[e] = acc[j][i][4 * q + e];
-        } else {
-          const f4v w0 = *reinterpret_cast<const f4v*>(s_w + wn * WR + c);
-          const f4v b0 = *reinterpret_cast<const f4v*>(s_b + wn * WR + c);
-          f4v v;
+        for (int e = 0; e < 4; ++e) v[e] = scaled(acc[j][i][4 * q + e], sx, w0[e], b0[e]);
+        if constexpr (GATED) {
+          const f4v w1 = *reinterpret_cast<const f4v*>(s_w + wn * WR + WN + c);
+          const f4v b1 = *reinterpret_cast<const f4v*>(s_b + wn * WR + WN + c);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = scaled(acc[j][i][4 * q + e], sx, w0[e], b0[e]);
-          if constexpr (GATED) {
-            const f4v w1 = *reinterpret_cast<const f4v*>(s_w + wn * WR + WN + c);
-            const f4v b1 = *reinterpret_cast<const f4v*>(s_b + wn * WR + WN + c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              v[e] = activate<ACT>(v[e]) * scaled(acc[j][i + I / 2][4 * q + e], sx, w1[e], b1[e]);
-          }
-          bits = __builtin_bit_cast(i4v, v);
+          for (int e = 0; e < 4; ++e)
+            v[e] = activate<ACT>(v[e]) * scaled(acc[j][i + I / 2][4 * q + e], sx, w1[e], b1[e]);
         }
-        *reinterpret_cast<i4v*>(out + r32 * G::kPitch + c * 4) = bits;
+        *reinterpret_cast<f4v*>(out + r32 * G::kPitch + c * 4) = v;
       }
     wave_lds_fence();                                   // written before it is read
-    if constexpr (SPLIT) {
-      // rows of WR sums: gated, WN of each projection
-#pragma unroll
-      for (int r = 0; r < 32 * WR / 256; ++r) {
-        const int e = (r * 64 + lane) * 4, row = e / WR, c = e % WR;
-        const int p = GATED ? c / WN : 0;
-        if (mj + row < a.M) {
-          int* dst = a.part + ((static_cast<int64_t>(split) * (GATED ? 2 : 1) + p) * a.M + mj + row) * a.ldp;
-          *reinterpret_cast<i4v*>(dst + nw + c % WN) =
-              *reinterpret_cast<const i4v*>(out + row * G::kPitch + c * 4);
-        }
-      }
-    } else if (a.vec && a.out_dt != kF32) {
+    if (a.vec && a.out_dt != kF32) {
 #pragma unroll
       for (int r = 0; r < 32 * WN / 512; ++r) {
         const int e = (r * 64 + lane) * 8, row = e / WN, c = e % WN;
@@ -335,42 +332,51 @@ __global__ __launch_bounds__(256) void k_w8_tile(W8Args a) {
   }
 }
 
-// Adds the ranges' sums and finishes the outputs, four neighbouring ones per thread.
-template <int ACT>
+// Adds the ranges' sums and finishes the outputs. A workgroup has one block of 32 x 32
+// outputs as k_w8_tile<J, I> left it; a thread has 4 neighbouring ones, 8 threads a
+// token's 32, so that loads and stores both go in pieces of 64 bytes or more.
+template <int J, int I, int ACT>
 __global__ __launch_bounds__(kBlock) void k_w8_join(W8Args a) {
-  constexpr int P = ACT != kNoAct ? 2 : 1;
-  const int64_t quads = (a.N + 3) / 4;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
-  if (i >= quads * a.M) return;
-  const int64_t m = i / quads;
-  const int n = static_cast<int>(i - m * quads) * 4;
+  constexpr bool GATED = ACT != kNoAct;
+  constexpr int IO = GATED ? I / 2 : I;
+  int b = blockIdx.x;
+  const int i = b % IO;
+  b /= IO;
+  const int j = b % J;
+  b /= J;
+  const int wave = b & 3, tile = b >> 2, tm = tile / a.tiles_n, tn = tile - tm * a.tiles_n;
+  const int row = threadIdx.x >> 3, q = (threadIdx.x & 7) >> 1, h = threadIdx.x & 1;
+  const int64_t m = static_cast<int64_t>(tm) * 64 * J + (wave & 1) * 32 * J + 32 * j + row;
+  const int64_t n = static_cast<int64_t>(tn) * 64 * IO + (wave >> 1) * 32 * IO + 32 * i + 8 * q + 4 * h;
+  if (m >= a.M || n >= a.N) return;
+  const int64_t plane = static_cast<int64_t>(a.tiles_m) * a.tiles_n * (4 * J * I * 256);
+  const i4v* src = reinterpret_cast<const i4v*>(a.part) +
+                   (static_cast<int64_t>(tile) * 4 + wave) * (J * I * 256) + (j * I + i) * 256 + q * 64 + h * 32 + row;
   const float sx = a.sx[m * a.sx_step];
-  f4v v[P];
+  f4v v[2];
 #pragma unroll
-  for (int p = 0; p < P; ++p) {
-    const int* src = a.part + (p * static_cast<int64_t>(a.M) + m) * a.ldp + n;
-    const int64_t plane = static_cast<int64_t>(P) * a.M * a.ldp;
+  for (int p = 0; p < (GATED ? 2 : 1); ++p) {
     i4v s = {0, 0, 0, 0};
     for (int r = 0; r < a.splits; r += 4) {   // 4 loads under way at a time
       i4v v4[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v4[e] = *reinterpret_cast<const i4v*>(src + min(r + e, a.splits - 1) * plane);
+      for (int e = 0; e < 4; ++e) v4[e] = src[min(r + e, a.splits - 1) * plane + p * (I / 2 * 256)];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (r + e < a.splits) s += v4[e];
     }
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const int nc = min(n + c, a.N - 1);
+      const int64_t nc = n + c < a.N ? n + c : a.N - 1;
       v[p][c] = scaled(s[c], sx, a.sw[p][nc * a.sw_step[p]],
                        a.bias[p] ? ld_any(a.bias[p], a.bias_dt, nc) : 0.0f);
     }
   }
-  if constexpr (P == 2) {
+  if constexpr (GATED) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) v[0][c] = activate<ACT>(v[0][c]) * v[P - 1][c];
+    for (int c = 0; c < 4; ++c) v[0][c] = activate<ACT>(v[0][c]) * v[1][c];
   }
-  st_quad(a, m, n, v[0]);
+  st_quad(a, m, static_cast<int>(n), v[0]);
 }
 
 // K < 16 (0: the sums are empty): one output per thread, code by code.
@@ -425,7 +431,7 @@ constexpr int kTileJ[] = {4, 3, 2, 2}, kTileI[] = {4, 4, 2, 2};
 struct W8Plan {
   int tile, splits, split_steps;
   bool pad;                  // x and the weights are copied to rows of kp bytes first
-  int64_t kp, ldp;           // ldp: columns of a plane of sums, a multiple of the tile's
+  int64_t kp;
   size_t part_off, bytes;
 };
 
@@ -477,17 +483,15 @@ W8Plan w8_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, size_t room 
   for (int tile = 0; tile < kTiles; ++tile) {
     if (rows != kRows16 && (tile == kT192 || tile == kT128)) continue;
     const int64_t tiles = cdiv(M, 64 * kTileJ[tile]) * cdiv(N, 64 * kTileI[tile] / proj);
-    const int tn = 64 * kTileI[tile] / proj;
-    const int64_t ldp = cdiv(N, tn) * tn;
+    const size_t plane = static_cast<size_t>(tiles) * kTileJ[tile] * kTileI[tile] * 16384;   // bytes of sums
     for (int64_t sp = 1; sp <= 8; ++sp) {
-      const size_t bytes = p.part_off + (sp > 1 ? align256(static_cast<size_t>(sp * proj * M * ldp) * 4) : 0);
+      const size_t bytes = p.part_off + (sp > 1 ? sp * plane : 0);
       if (sp > 1 && (tiles * sp > (tile == kT128x2 ? 2 : 1) * cus || steps / sp < 3 || bytes > room)) break;
       const double t = w8_time(kModels[rows], tile, tiles, steps, proj * M * N, sp, cus);
       if (best < 0 || t < best) {
         best = t;
         p.tile = tile;
         p.splits = static_cast<int>(sp);
-        p.ldp = ldp;
         p.bytes = bytes;
       }
     }
@@ -506,17 +510,20 @@ bool few_rows(int64_t M, int64_t N, int64_t K) {
 
 template <int J, int I, int NS, int ACT>
 void launch_tile(const W8Args& a, bool any, hipStream_t s) {
-  const unsigned grid = static_cast<unsigned>(a.tiles_m) * a.tiles_n * a.splits;
+  const unsigned tiles = static_cast<unsigned>(a.tiles_m) * a.tiles_n, grid = tiles * a.splits;
   constexpr int RAW = ACT == kNoAct ? kNoAct : CBQ_ACT_RELU;   // sums do not depend on it
-  if constexpr (NS == 2 && J != 3) {
-    if (any) {
-      if (a.splits > 1) k_w8_tile<J, I, 2, RAW, true, true><<<grid, 256, 0, s>>>(a);
+  const bool split = a.splits > 1;
+  if (any) {
+    if constexpr (NS == 2 && J != 3) {
+      if (split) k_w8_tile<J, I, 2, RAW, true, true><<<grid, 256, 0, s>>>(a);
       else k_w8_tile<J, I, 2, ACT, false, true><<<grid, 256, 0, s>>>(a);
-      return;
     }
+  } else if (split) {
+    k_w8_tile<J, I, NS, RAW, true, false><<<grid, 256, 0, s>>>(a);
+  } else {
+    k_w8_tile<J, I, NS, ACT, false, false><<<grid, 256, 0, s>>>(a);
   }
-  if (a.splits > 1) k_w8_tile<J, I, NS, RAW, true, false><<<grid, 256, 0, s>>>(a);
-  else k_w8_tile<J, I, NS, ACT, false, false><<<grid, 256, 0, s>>>(a);
+  if (split) k_w8_join<J, I, ACT><<<tiles * 4 * J * (ACT == kNoAct ? I : I / 2), kBlock, 0, s>>>(a);
 }
 
 template <int ACT>
@@ -526,10 +533,6 @@ void launch_tiles(const W8Args& a, int tile, bool any, hipStream_t s) {
     case kT192: launch_tile<3, 4, 2, ACT>(a, false, s); break;
     case kT128x2: launch_tile<2, 2, 2, ACT>(a, any, s); break;
     default: launch_tile<2, 2, 4, ACT>(a, false, s); break;
-  }
-  if (a.splits > 1) {
-    const int64_t quads = static_cast<int64_t>(a.M) * ((a.N + 3) / 4);
-    k_w8_join<ACT><<<static_cast<unsigned>(cdiv(quads, kBlock)), kBlock, 0, s>>>(a);
   }
 }
 
@@ -613,7 +616,6 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
   a.tiles_n = static_cast<int>(tiles_n);
   a.splits = p.splits;
   a.split_steps = p.split_steps;
-  a.ldp = p.ldp;
   uint8_t* const w0 = static_cast<uint8_t*>(ws);
   if (p.pad) {
     W8Pad c = {{a.x, a.w[0], a.w[1]}, {a.ldx, a.ldw[0], a.ldw[1]}, {}, w0 + CBQ_WS_CTRL_BYTES,

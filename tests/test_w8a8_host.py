@@ -127,10 +127,10 @@ def test_workspace_sizes():
     # many tokens with rows of 1403 codes: copies in rows of 1408
     for p in (1, 2):
         assert L.cbq_w8a8_ws_bytes(4096, 8192, 1403, p) == C + 1408 * (4096 + p * 8192)
-    # few tiles of long rows: planes of int32 sums, for each projection
-    one, two = (L.cbq_w8a8_ws_bytes(200, 1024, 11008, p) - C for p in (1, 2))
-    assert one % (200 * 1024 * 4) == 0 and two % (2 * 200 * 1024 * 4) == 0
-    assert 2 <= one // (200 * 1024 * 4) <= 8 and 2 <= two // (2 * 200 * 1024 * 4) <= 8
+    # few tiles of long rows: planes of int32 sums (here of whole tiles), for each projection
+    one, two = (L.cbq_w8a8_ws_bytes(256, 1024, 11008, p) - C for p in (1, 2))
+    assert one % (256 * 1024 * 4) == 0 and two % (2 * 256 * 1024 * 4) == 0
+    assert 2 <= one // (256 * 1024 * 4) <= 8 and 2 <= two // (2 * 256 * 1024 * 4) <= 8
 
 
 def test_quantized_operands_are_checked():
