@@ -154,16 +154,22 @@ def test_rows_of_zeros_and_of_one_value():
 
 
 def test_views_are_read_in_place():
-    """Rows that are slices of wider ones, odd offsets, one row with a stride of its
-    own, transposed input."""
+    """Rows that are slices of wider ones, odd offsets (which another kernel takes, with
+    the sums in another order), one row with a stride of its own, transposed input."""
     from cublade_amd.quantization import norm_tensor, residual_norm
     big = _rand(30, 1500, seed=7, dtype=F16).cuda()
-    for x in (big[:, 3:1003], big[::2, 100:612], big[4:5, 1:78], big[:, :64].t(), big[3], big.view(5, 6, 1500)[:, 2]):
-        a, b = norm_tensor(x), norm_tensor(x.clone(memory_format=torch.contiguous_format))
-        assert torch.equal(a.data, b.data) and torch.equal(a.scale, b.scale)
+    for x in (big[:, 3:1003], big[::2, 100:612], big[4:5, 1:78], big[:, :64].t(), big[3],
+              big.view(5, 6, 1500)[:, 2], big[:, 1:65], big[:, 2:1026]):
+        rows = x.cpu().reshape(-1, x.shape[-1])
+        zero = torch.zeros(rows.shape, dtype=torch.float64)
+        a = norm_tensor(x)
+        P.check_codes(a.data, a.scale, *P.norm(rows.double(), zero, "rms", 1e-6, None, None))
         h, n = residual_norm(x, x, gate=x)
-        hc, nc = residual_norm(*[x.clone(memory_format=torch.contiguous_format)] * 2, gate=x.clone())
-        assert torch.equal(h, hc) and torch.equal(n.data, nc.data) and h.shape == x.shape
+        want, bound = P.residual(rows, rows, "rms", 1e-6, False, None, None, rows, 1.0, F16)
+        assert h.shape == x.shape
+        stored = h.cpu().double().reshape(rows.shape)
+        assert bool(((stored - want).abs() <= bound).all())
+        P.check_codes(n.data, n.scale, *P.norm(stored, zero, "rms", 1e-6, None, None))
 
 
 def test_empty_and_refusals_on_the_gpu():

@@ -106,6 +106,15 @@ def test_norm_entry_refuses_bad_arguments():
     assert norm(tokens=0, x=None) == 0 and norm(hidden=0, x=None) == 0
 
 
+def test_norm_arguments_as_bytes():
+    """The binding packs cbq_norm_args itself: the same bytes as the structure's."""
+    from cublade_amd import _abi
+    from cublade_amd.bindings.hip.norm import _ARGS
+    assert _ARGS.size == ctypes.sizeof(_abi.NormArgs)
+    values = [*range(1, 24), 0.5, -2.0]
+    assert _ARGS.pack(*values) == bytes(_abi.NormArgs(*values))
+
+
 def test_norms_on_the_host():
     from cublade_amd.quantization import norm_tensor, residual_norm
     x = torch.zeros(4, 64)
