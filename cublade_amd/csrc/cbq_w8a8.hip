@@ -268,68 +268,84 @@ __global__ __launch_bounds__(256) void k_w8_tile(W8Args a) {
     return;
   }
 
-  // Outputs: 32 tokens at a time through the wave's own part of LDS.
+  // Outputs: the sums of 32 tokens at a time go through the wave's own part of LDS as
+  // they are (straight from the accumulation registers, which the vector unit cannot
+  // read) and are finished on the other side, where a lane keeps its columns, and with
+  // them their scales, for all rows.
   __syncthreads();
   uint8_t* const out = smem + wave * 32 * G::kPitch;
   const int mw = m0 + wm * WM, nw = n0 + wn * WN;       // the wave's first token and column
+  const float* const cols = s_w + wn * WR;              // gated: the up projection's WN further
+  const float* const bias = s_b + wn * WR;
+  auto finish = [&](int sum, int sum2, float sx, float w0, float b0, float w1, float b1) {
+    const float v = scaled(sum, sx, w0, b0);
+    return GATED ? activate<ACT>(v) * scaled(sum2, sx, w1, b1) : v;
+  };
+  // C columns per lane and row: st(row, column, values). ROLL keeps the rows in a loop.
+  auto put = [&](auto per_lane, auto roll, auto&& st) {
+    constexpr int C = decltype(per_lane)::value, LR = WN / C, RL = 64 / LR;   // lanes of a row, rows at a time
+    constexpr int kUnroll = decltype(roll)::value ? 1 : 32 / RL;
+    const int c = lane % LR * C;
+    float w0[C], b0[C], w1[C], b1[C];
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int mj = mw + 32 * j;
-    const float sx = s_x[wm * WM + 32 * j + r32];
-    wave_lds_fence();                                   // the last rows are read
+    for (int e = 0; e < C; ++e) {
+      w0[e] = cols[c + e];
+      b0[e] = bias[c + e];
+      w1[e] = GATED ? cols[WN + c + e] : 0.0f;
+      b1[e] = GATED ? bias[WN + c + e] : 0.0f;
+    }
 #pragma unroll
-    for (int i = 0; i < IO; ++i)
+    for (int j = 0; j < J; ++j) {
+      wave_lds_fence();                                 // the last rows are read
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = 32 * i + 8 * q + 4 * h;           // the wave's column of 4 outputs
-        const f4v w0 = *reinterpret_cast<const f4v*>(s_w + wn * WR + c);
-        const f4v b0 = *reinterpret_cast<const f4v*>(s_b + wn * WR + c);
-        f4v v;
+      for (int i = 0; i < I; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = scaled(acc[j][i][4 * q + e], sx, w0[e], b0[e]);
-        if constexpr (GATED) {
-          const f4v w1 = *reinterpret_cast<const f4v*>(s_w + wn * WR + WN + c);
-          const f4v b1 = *reinterpret_cast<const f4v*>(s_b + wn * WR + WN + c);
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<i4v*>(out + r32 * G::kPitch + (32 * i + 8 * q + 4 * h) * 4) =
+              i4v{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+      wave_lds_fence();                                 // written before it is read
+#pragma unroll kUnroll
+      for (int r = 0; r < 32 / RL; ++r) {
+        const int row = r * RL + lane / LR;
+        const uint8_t* src = out + row * G::kPitch + c * 4;
+        const float sx = s_x[wm * WM + 32 * j + row];
+        float v[C];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[e] = activate<ACT>(v[e]) * scaled(acc[j][i + I / 2][4 * q + e], sx, w1[e], b1[e]);
+        for (int e = 0; e < C; e += 4) {
+          const i4v g = *reinterpret_cast<const i4v*>(src + e * 4);
+          i4v u = {0, 0, 0, 0};
+          if constexpr (GATED) u = *reinterpret_cast<const i4v*>(src + WN * 4 + e * 4);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[e + k] = finish(g[k], u[k], sx, w0[e + k], b0[e + k], w1[e + k], b1[e + k]);
         }
-        *reinterpret_cast<f4v*>(out + r32 * G::kPitch + c * 4) = v;
-      }
-    wave_lds_fence();                                   // written before it is read
-    if (a.vec && a.out_dt != kF32) {
-#pragma unroll
-      for (int r = 0; r < 32 * WN / 512; ++r) {
-        const int e = (r * 64 + lane) * 8, row = e / WN, c = e % WN;
-        const f4v lo = *reinterpret_cast<const f4v*>(out + row * G::kPitch + c * 4);
-        const f4v hi = *reinterpret_cast<const f4v*>(out + row * G::kPitch + c * 4 + 16);
-        const u32x4 o = a.out_dt == kF16
-            ? u32x4{pack2_out<kF16>(lo.x, lo.y), pack2_out<kF16>(lo.z, lo.w),
-                    pack2_out<kF16>(hi.x, hi.y), pack2_out<kF16>(hi.z, hi.w)}
-            : u32x4{pack2_out<kBF16>(lo.x, lo.y), pack2_out<kBF16>(lo.z, lo.w),
-                    pack2_out<kBF16>(hi.x, hi.y), pack2_out<kBF16>(hi.z, hi.w)};
-        if (mj + row < a.M && nw + c < a.N)
-          *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.y) +
-                                    static_cast<int64_t>(mj + row) * a.N + nw + c) = o;
-      }
-    } else if (a.vec) {
-#pragma unroll
-      for (int r = 0; r < 32 * WN / 256; ++r) {
-        const int e = (r * 64 + lane) * 4, row = e / WN, c = e % WN;
-        const f4v v = *reinterpret_cast<const f4v*>(out + row * G::kPitch + c * 4);
-        if (mj + row < a.M && nw + c < a.N)
-          *reinterpret_cast<f4v*>(static_cast<float*>(a.y) + static_cast<int64_t>(mj + row) * a.N +
-                                  nw + c) = v;
-      }
-    } else {
-      for (int r = 0; r < 32 * WN / 64; ++r) {
-        const int e = r * 64 + lane, row = e / WN, c = e % WN;
-        const float v = *reinterpret_cast<const float*>(out + row * G::kPitch + c * 4);
-        if (mj + row < a.M && nw + c < a.N)
-          st_any(a.y, a.out_dt, static_cast<int64_t>(mj + row) * a.N + nw + c, v);
+        if (mw + 32 * j + row < a.M) st(mw + 32 * j + row, nw + c, v);
       }
     }
-  }
+  };
+  auto put16 = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    put(std::integral_constant<int, 8>{}, std::false_type{}, [&](int m, int n, const float (&v)[8]) {
+      if (n < a.N)
+        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(a.y) + static_cast<int64_t>(m) * a.N + n) =
+            u32x4{pack2_out<DT>(v[0], v[1]), pack2_out<DT>(v[2], v[3]), pack2_out<DT>(v[4], v[5]),
+                  pack2_out<DT>(v[6], v[7])};
+    });
+  };
+  if (a.vec && a.out_dt == kF16) put16(std::integral_constant<int, kF16>{});
+  else if (a.vec && a.out_dt == kBF16) put16(std::integral_constant<int, kBF16>{});
+  else if (a.vec)
+    put(std::integral_constant<int, 4>{}, std::false_type{}, [&](int m, int n, const float (&v)[4]) {
+      if (n < a.N)
+        *reinterpret_cast<f4v*>(static_cast<float*>(a.y) + static_cast<int64_t>(m) * a.N + n) =
+            f4v{v[0], v[1], v[2], v[3]};
+    });
+  else
+    put(std::integral_constant<int, 4>{}, std::true_type{}, [&](int m, int n, const float (&v)[4]) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < a.N) st_any(a.y, a.out_dt, static_cast<int64_t>(m) * a.N + n + e, v[e]);
+    });
 }
 
 // Adds the ranges' sums and finishes the outputs. A workgroup has one block of 32 x 32
