@@ -122,8 +122,14 @@ inline void with_act(int act, F&& f) {
   }
 }
 
-// cbq_w8a8_few.hip: M <= kFewRows, K >= 16, any alignment; returns after queueing.
-constexpr int kFewRows = 128;
-void launch_w8a8_few(const W8Args& a, hipStream_t s);
+// What rows of codes and their strides are multiples of.
+enum { kRows16, kRows4, kRows1 };
+
+// cbq_w8a8_few.hip: few rows of x, or few outputs; K >= 16. The shape for these sizes and
+// its modelled time; any: rows that are no multiples of 16 bytes. Returns after queueing.
+constexpr int kFewRows = 2048;
+struct FewPlan { int shape; double us; };
+FewPlan few_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, int cus);
+void launch_w8a8_few(const W8Args& a, int shape, bool any, hipStream_t s);
 
 }  // namespace cbq

@@ -5,7 +5,7 @@
 //   y[m, n] = sx[m] sw[n] sum_k x[m, k] w[n, k] + bias[n]
 //   y[m, n] = act(g) u,  g and u as above with the gate's and the up rows
 //
-// Sums are int32 and exact (K <= 131071). M <= 64: cbq_w8a8_few.hip.
+// Sums are int32 and exact (K <= 131071). M <= 64, and small products: cbq_w8a8_few.hip.
 //
 // k_w8_tile<J, I, NS, ACT, SPLIT, ANY>: tiles of 64 J tokens x 64 I weight rows (gated:
 // 32 I columns of each projection side by side, so that a lane holds g and u of the
@@ -445,6 +445,7 @@ enum { kT256, kT192, kT128, kT128x2, kTiles };
 constexpr int kTileJ[] = {4, 3, 2, 2}, kTileI[] = {4, 4, 2, 2};
 
 struct W8Plan {
+  int few;                   // shape of cbq_w8a8_few.hip, or -1
   int tile, splits, split_steps;
   bool pad;                  // x and the weights are copied to rows of kp bytes first
   int64_t kp;
@@ -459,7 +460,6 @@ struct W8Plan {
 // (7% off rms; what it picks is 0.8% slower on average than the best), 5700 each with
 // rows of whole words and with others (8% and 7%; 1.6% and 1.5%).
 struct W8Model { double step[kTiles], busy[kTiles], round[kTiles], two, call, join, sum; };
-enum { kRows16, kRows4, kRows1 };   // what rows and their strides are multiples of
 constexpr W8Model kModels[] = {
     {{1.13, 0.88, 0.35, 0.48}, {0.49, 0.39, 0.17, 0.215}, {7.4, 6.3, 3.3, 2.7}, 1.07, 3.0, 3.3, 1e-6},
     {{1.69, 0, 0, 0.62}, {0.51, 0, 0, 0.29}, {7.0, 0, 0, 2.6}, 1.46, 3.9, 3.0, 1e-6},
@@ -485,6 +485,10 @@ W8Plan w8_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, size_t room 
   const int cus = device_cus();
   const int64_t steps = cdiv(K, 128);
   W8Plan p = {};
+  p.bytes = CBQ_WS_CTRL_BYTES;
+  const FewPlan few = M <= kFewRows ? few_plan(M, N, K, proj, rows, cus) : FewPlan{-1, 0.0};
+  p.few = few.shape;
+  if (M <= 64) return p;     // 64 x 11008 x 4096, gated: 24 us, by tiles 22; mostly a third of the tiles' time
   p.kp = cdiv(K, 16) * 16;
   p.part_off = CBQ_WS_CTRL_BYTES;
   // Copies read and write M K + N K bytes at 4 TB/s and take a launch. Where rows are no
@@ -512,16 +516,18 @@ W8Plan w8_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, size_t room 
       }
     }
   }
+  if (p.few >= 0) {
+    if (p.pad) best += 3.0 + static_cast<double>(copies) * 0.5e-6;
+    if (few.us <= best) {
+      p.pad = false;
+      p.bytes = CBQ_WS_CTRL_BYTES;
+      return p;
+    }
+    p.few = -1;
+  }
   p.split_steps = static_cast<int>(cdiv(steps, p.splits));
   p.splits = static_cast<int>(cdiv(steps, p.split_steps));   // no empty ranges
   return p;
-}
-
-// cbq_w8a8_few.hip takes up to 64 rows, and up to 128 where x, which all of its
-// workgroups read, is small: at M = 128 (us, there / here) N = K = 4096 11 / 17, N =
-// 4096, K = 8192 20 / 19, N = 11008, K = 4096 20 / 20, N = 28672, K = 8192 78 / 72.
-bool few_rows(int64_t M, int64_t N, int64_t K) {
-  return M <= 64 || (M <= kFewRows && N <= 16 * device_cus() && K <= 6144);
 }
 
 template <int J, int I, int NS, int ACT>
@@ -621,11 +627,11 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
     });
     return launch_status(what);
   }
-  if (few_rows(M, N, K)) {
-    launch_w8a8_few(a, s);
+  const W8Plan p = w8_plan(M, N, K, proj, rows, ws && aligned(ws, 256) ? ws_bytes : 0);
+  if (p.few >= 0) {
+    launch_w8a8_few(a, p.few, rows != kRows16, s);
     return launch_status(what);
   }
-  const W8Plan p = w8_plan(M, N, K, proj, rows, ws && aligned(ws, 256) ? ws_bytes : 0);
   const int64_t tiles_m = cdiv(M, 64 * kTileJ[p.tile]), tiles_n = cdiv(N, 64 * kTileI[p.tile] / proj);
   CBQ_REQUIRE(tiles_m * tiles_n * p.splits < (1LL << 31), "%s: too many tiles", what);
   a.tiles_m = static_cast<int>(tiles_m);
@@ -659,7 +665,7 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
 using namespace cbq;
 
 extern "C" size_t cbq_w8a8_ws_bytes(int64_t M, int64_t N, int64_t K, int projections) {
-  if (M <= 0 || N <= 0 || K < 16 || K > 131071 || projections < 1 || projections > 2 || few_rows(M, N, K))
+  if (M <= 0 || N <= 0 || K < 16 || K > 131071 || projections < 1 || projections > 2)
     return CBQ_WS_CTRL_BYTES;
   return w8_plan(M, N, K, projections, K % 16 == 0 ? kRows16 : K % 4 == 0 ? kRows4 : kRows1).bytes;
 }

@@ -1,11 +1,11 @@
-// cbq_w8a8_few.hip - products of few rows of INT8 activations with INT8 weights
-// (M <= 128): what counts is the stream of the weight, and then that of x.
+// cbq_w8a8_few.hip - products of few rows of INT8 activations with INT8 weights, and
+// small products: too few outputs for the tiles of cbq_w8a8.hip to fill the chip.
 //
 //   y[m, n] = sx[m] sw[n] sum_k x[m, k] w[n, k] + bias[n]     or act(g) u of two
 //
-// k_w8_few<RT, MT, W, D, GATED, ANY>: a workgroup of W waves owns RT tiles of 16
+// k_w8_few<RT, MT, W, D, GATED, ANY, ONE>: a workgroup of W waves owns RT tiles of 16
 // weight rows (gated: RT / 2 of the gate's and the same of the up projection's) and
-// all MT tiles of 16 rows of x. Wave w takes the blocks w, w + W, ... of 128 bytes of
+// MT tiles of 16 rows of x. Wave w takes the blocks w, w + W, ... of 128 bytes of
 // k of all of them, so the waves share nothing until their sums meet. A unit (block,
 // tile) is two loads of 8 rows x 128 bytes by LDS DMA: 8 lanes in a row fetch one
 // cache line, while the matrix operand's own order (16 rows x 64 bytes, neighbouring
@@ -15,8 +15,13 @@
 // v_mfma_i32_16x16x64_i8: A = weight rows, B = rows of x, so a lane ends with 4
 // neighbouring outputs of one token.
 //
-// Bound: memory for 16 rows or less (N = 28672, K = 8192, M = 1: 39 us = 6.0 TB/s; M =
-// 16, N = 11008, K = 4096: 9.9 us in a graph), then the reads of x by every workgroup.
+// Bound: memory for 16 rows or less (N = 28672, K = 8192, M = 1: 45 us = 5.3 TB/s; M =
+// 16, N = 11008, K = 4096: 9.7 us), then the reads of x by every workgroup, and for small
+// products the chain of loads, sums and stores. Blocks of 16 or 32 rows of x, each with
+// workgroups of its own, beat workgroups with all rows there, since more waves load (us,
+// M = 64 / 128, N = K = 4096: 7.3 / 11.3 -> 6.8 / 8.2), and beat the tiles, whose 256
+// threads own 128 x 128 outputs or more (M = 333, N = 1001, K = 1403: 12 -> 7.4; M = 256,
+// N = K = 4096: 17 -> 11).
 // Measured against loads in the operand's order through registers (us, M = 16 / 32 /
 // 64 / 128, N = K = 4096): 6.6 / 8.8 / 12.8 / 20.7 -> 5.8 / 5.9 / 7.3 / 11.3.
 //
@@ -24,6 +29,7 @@
 // not count; rows past M and N repeat the last one and are not stored. ANY: rows that
 // are no multiples of 16 bytes, which the DMA does not take: through registers, one
 // block ahead.
+#include <algorithm>
 #include <type_traits>
 
 #include "cbq_lds_dma.h"
@@ -37,7 +43,7 @@ __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-template <int RT, int MT, int W, int D, bool GATED, bool ANY>
+template <int RT, int MT, int W, int D, bool GATED, bool ANY, bool ONE>
 __global__ __launch_bounds__(64 * W) void k_w8_few(W8Args a) {
   constexpr int CT = GATED ? RT / 2 : RT;           // tiles of 16 output columns
   static_assert(!GATED || RT % 2 == 0, "pairs of tiles");
@@ -50,7 +56,18 @@ __global__ __launch_bounds__(64 * W) void k_w8_few(W8Args a) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16 * CT;
+  // Workgroups of the same weight rows run on one XCD (b % 8), one after the other, so
+  // that its L2 reads them once (M = 64, N = 11008, K = 4096, 16 rows of x each: 23 us
+  // -> 16). The grid is a whole number of rounds over the XCDs. ONE: one block of rows of
+  // x and no such order, which would cost single tokens 0.3 us.
+  int n0 = blockIdx.x, m0 = 0;
+  if constexpr (!ONE) {
+    const int turn = n0 >> 3;
+    m0 = turn % a.tiles_m * 16 * MT;
+    n0 = turn / a.tiles_m * 8 + (n0 & 7);
+    if (n0 * 16 * CT >= a.N) return;
+  }
+  n0 *= 16 * CT;
   uint8_t* const mine = ring + wave * (D * U * 2048);
   const uint32_t mine_lds = __builtin_amdgcn_readfirstlane(lds_addr(mine));
   const int nblk = (a.K + 127) / 128;
@@ -70,11 +87,11 @@ __global__ __launch_bounds__(64 * W) void k_w8_few(W8Args a) {
         off[u][h] = static_cast<uint32_t>(min(t * 16 + h * 8 + lrow, a.N - 1 - n0)) *
                     static_cast<uint32_t>(a.ldw[p]);
       } else {
-        off[u][h] = static_cast<uint32_t>(min((u - RT) * 16 + h * 8 + lrow, a.M - 1)) *
+        off[u][h] = static_cast<uint32_t>(min((u - RT) * 16 + h * 8 + lrow, a.M - 1 - m0)) *
                     static_cast<uint32_t>(a.ldx);
       }
     }
-  const uint8_t* base[3] = {a.w[0] + n0 * a.ldw[0], GATED ? a.w[1] + n0 * a.ldw[1] : nullptr, a.x};
+  const uint8_t* base[3] = {a.w[0] + n0 * a.ldw[0], GATED ? a.w[1] + n0 * a.ldw[1] : nullptr, a.x + m0 * a.ldx};
   auto base_of = [&](int u) { return u >= RT ? base[2] : GATED && (u & 1) ? base[1] : base[0]; };
   u32x4 held[ANY ? U : 1][2];                       // ANY: loads on their way to LDS
   auto fetch = [&](int i, int slot) {
@@ -172,7 +189,7 @@ __global__ __launch_bounds__(64 * W) void k_w8_few(W8Args a) {
   };
   for (int q = wave; q < CT * MT; q += W) {
     const int t = q / MT, j = q % MT;
-    const int m = j * 16 + row, n = n0 + t * 16 + g * 4;
+    const int m = m0 + j * 16 + row, n = n0 + t * 16 + g * 4;
     if (m >= a.M || n >= a.N) continue;
     const float sx = a.sx[m * a.sx_step];
     f4v v[2];
@@ -194,55 +211,97 @@ __global__ __launch_bounds__(64 * W) void k_w8_few(W8Args a) {
   }
 }
 
+// The shapes a workgroup comes in (6 tiles of weight rows: gated only).
+struct FewShape { int rt, mt, waves, depth; };
+constexpr FewShape kShapes[] = {{1, 1, 8, 2}, {2, 1, 8, 1}, {3, 1, 8, 1}, {4, 1, 4, 1}, {6, 1, 8, 1},
+                                {1, 2, 8, 1}, {2, 2, 8, 1}, {3, 2, 8, 1}, {4, 2, 4, 1},
+                                {2, 4, 8, 1}, {3, 4, 8, 1}, {4, 4, 4, 1}, {4, 4, 8, 1}};
+constexpr int kNumShapes = sizeof(kShapes) / sizeof(kShapes[0]);
+
+// Modelled time in us of a shape: a call, a round of as many workgroups as fit the CUs
+// (counted on the fullest XCD), a wave's blocks in it (step; more for each further
+// workgroup of the CU), and the weights' megabytes (far: those past 90). Fitted to
+// timings on MI355X (M = 1 .. 1024, N = 200 .. 32000, K = 200 .. 14336, one and two
+// projections): 2400 with aligned rows, 1200 each with rows of whole words and with
+// others. A time is 10% off rms; what the model picks is 1% slower on average than the
+// fastest of the shapes.
+struct FewModel { double call, round, step, more, mb, far; };
+constexpr FewModel kFewModels[][kNumShapes] = {
+    {{1.65, 0.819, 0.216, 0.258, 0.0832, 0.0742}, {1.89, 0.778, 0.316, 0.352, 0.105, 0.0611},
+     {1.88, 0.749, 0.417, 0.541, 0.0982, 0.0825}, {1.43, 1.45, 0.399, 0.229, 0.103, 0.0713},
+     {1.19, 1.87, 0.934, 0, 0.0995, 0.0668}, {2.09, 0.578, 0.381, 0.47, 0.0586, 0.113},
+     {1.8, 1.19, 0.515, 0.626, 0.0746, 0.0801}, {1.34, 1.47, 0.704, 0, 0.0696, 0.129},
+     {1.5, 2.01, 0.539, 0.319, 0.0821, 0.0991}, {1.37, 1.83, 0.861, 0, 0.0677, 0.121},
+     {1.23, 2.42, 1.01, 0, 0.072, 0.113}, {1.35, 3.95, 0.671, 0.487, 0.0812, 0.0862},
+     {1.34, 2.62, 1.16, 0, 0.0876, 0.0897}},
+    {{2.17, 0.422, 0.299, 0.377, 0.0786, 0.141}, {2.08, 0.778, 0.448, 0.563, 0.101, 0.0812},
+     {1.72, 1.13, 0.587, 0.711, 0.106, 0.101}, {2.3, 0.995, 0.51, 0.536, 0.0936, 0.0888},
+     {1.19, 2.01, 1.48, 0, 0.114, 0.0646}, {2.2, 0.501, 0.576, 0.587, 0.0722, 0.244},
+     {1.81, 1.23, 0.802, 0.724, 0.0813, 0.128}, {1.27, 1.85, 0.996, 0, 0.0976, 0.182},
+     {1.76, 2.2, 0.691, 0.553, 0.0888, 0.113}, {1.27, 2.19, 1.23, 0, 0.0897, 0.14},
+     {1.18, 2.86, 1.46, 0, 0.101, 0.18}, {1.59, 4.31, 0.995, 0.809, 0.0763, 0.119},
+     {1.22, 3.08, 1.77, 0, 0.105, 0.0888}},
+    {{2.37, 0, 0.709, 0.661, 0.0326, 0.146}, {2.11, 0.498, 1.02, 0.9, 0.0594, 0.111},
+     {1.77, 0.663, 1.36, 1.17, 0.0619, 0.116}, {2.56, 0.687, 0.851, 0.892, 0.0604, 0.093},
+     {0.99, 1.7, 2.56, 0, 0.0713, 0.0769}, {2.4, 0, 1.11, 0.819, 0.0905, 0.188},
+     {2.28, 0.482, 1.4, 1.17, 0.0789, 0.107}, {1.55, 1.25, 1.74, 0, 0.0721, 0.15},
+     {2.15, 1.74, 1.05, 0.967, 0.0666, 0.104}, {1.53, 1.54, 2.09, 0, 0.0851, 0.131},
+     {1.42, 2.12, 2.47, 0, 0.0761, 0.131}, {1.93, 3.94, 1.47, 1.29, 0.0614, 0.123},
+     {1.55, 2.35, 2.8, 0, 0.0893, 0.0819}}};
+
 template <int RT, int MT, int W, int D, bool GATED>
-void launch_few(const W8Args& a, hipStream_t s) {
-  const int cols = 16 * (GATED ? RT / 2 : RT);
-  const dim3 g(static_cast<unsigned>(cdiv(a.N, cols))), b(64 * W);
-  const bool any = a.K % 16 || a.ldx % 16 || a.ldw[0] % 16 || !aligned(a.x, 16) || !aligned(a.w[0], 16) ||
-                   (GATED && (a.ldw[1] % 16 || !aligned(a.w[1], 16)));
-  if (any) k_w8_few<RT, MT, W, 1, GATED, true><<<g, b, 0, s>>>(a);
-  else k_w8_few<RT, MT, W, D, GATED, false><<<g, b, 0, s>>>(a);
-}
-
-// Tiles per workgroup: the fewest that leave at most one workgroup per CU, with the
-// most waves. Beyond that 4 tiles, so that fewer workgroups read x, and 4 waves, of
-// which several fit a CU; but one tile where x is small beside the weight (us, RT = 1 /
-// 4: N = 28672, K = 8192, M = 1 39 / 46, M = 16 45 / 46; N = 32000, K = 4096, M = 16
-// 25 / 21; gated, RT = 2 / 4: N = 28672, K = 8192, M = 16 83 / 100, N = 14336, K = 4096
-// 23 / 20).
-template <int MT>
-void launch_linear(const W8Args& a, hipStream_t s) {
-  constexpr int W = MT == 8 ? 4 : 8;
-  const int64_t cus = device_cus(), tiles = cdiv(a.N, 16);
-  if (tiles <= cus) launch_few<1, MT, 8, MT == 1 ? 2 : 1, false>(a, s);
-  else if (tiles <= 2 * cus) launch_few<2, MT, W, 1, false>(a, s);
-  else if (tiles <= 3 * cus) launch_few<3, MT, W, 1, false>(a, s);
-  else if (a.M <= 8 || (a.M <= 16 && tiles > 6 * cus)) launch_few<1, MT, 8, MT == 1 ? 2 : 1, false>(a, s);
-  else launch_few<4, MT, 4, 1, false>(a, s);
-}
-
-template <int MT>
-void launch_gated(const W8Args& a, hipStream_t s) {
-  constexpr int W = MT == 8 ? 4 : 8;
-  const int64_t cus = device_cus(), tiles = cdiv(a.N, 16);
-  if (tiles <= cus || (a.M <= 32 && tiles > 6 * cus)) launch_few<2, MT, W, 1, true>(a, s);
-  else if (tiles <= 2 * cus) launch_few<4, MT, W, 1, true>(a, s);
-  else if (tiles <= 3 * cus) launch_few<6, MT, MT >= 4 ? 4 : 8, 1, true>(a, s);
-  else launch_few<4, MT, 4, 1, true>(a, s);
+void launch_few(W8Args a, bool any, hipStream_t s) {
+  const unsigned blocks_n = static_cast<unsigned>(cdiv(a.N, 16 * (GATED ? RT / 2 : RT)));
+  if constexpr (MT == 1) {
+    if (a.M <= 16) {
+      if (any) k_w8_few<RT, 1, W, 1, GATED, true, true><<<blocks_n, 64 * W, 0, s>>>(a);
+      else k_w8_few<RT, 1, W, D, GATED, false, true><<<blocks_n, 64 * W, 0, s>>>(a);
+      return;
+    }
+  }
+  a.tiles_m = static_cast<int>(cdiv(a.M, 16 * MT));
+  const unsigned g = static_cast<unsigned>(cdiv(blocks_n, 8)) * 8 * a.tiles_m;
+  if (any) k_w8_few<RT, MT, W, 1, GATED, true, false><<<g, 64 * W, 0, s>>>(a);
+  else k_w8_few<RT, MT, W, D, GATED, false, false><<<g, 64 * W, 0, s>>>(a);
 }
 
 }  // namespace
 
-void launch_w8a8_few(const W8Args& a, hipStream_t s) {
-  auto go = [&](auto mt) {
-    constexpr int MT = decltype(mt)::value;
-    if (a.act == kNoAct) launch_linear<MT>(a, s);
-    else launch_gated<MT>(a, s);
+FewPlan few_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, int cus) {
+  FewPlan best = {-1, 0.0};
+  for (int c = 0; c < kNumShapes; ++c) {
+    const FewShape& f = kShapes[c];
+    // Tiles of x that hold no rows cost what others do, and many blocks of 16 rows of x
+    // read the weight as often.
+    if (f.rt % proj || (f.rt == 6 && proj == 1) || (f.mt > 1 && M <= 8 * f.mt) || (f.mt == 1 && M > 64)) continue;
+    const int64_t wgs = cdiv(cdiv(N, 16 * (f.rt / proj)), 8) * 8 * cdiv(M, 16 * f.mt), steps = cdiv(cdiv(K, 128), f.waves);
+    const int64_t lds = f.waves * (rows == kRows16 ? f.depth : 1) * (f.rt + f.mt) * 2048 + f.rt * f.mt * 1024;
+    const int64_t per_cu = std::min<int64_t>(160 * 1024 / lds, 2048 / (64 * f.waves));
+    const int64_t full = wgs / (per_cu * cus), rem = wgs - full * per_cu * cus;
+    const int64_t rounds = full + (rem > 0), more = full * (per_cu - 1) + (rem > 0 ? cdiv(rem, cus) - 1 : 0);
+    const FewModel& m = kFewModels[rows][c];
+    const double mb = 1e-6 * static_cast<double>(proj * N * K);
+    const double us = m.call + rounds * m.round + static_cast<double>(steps) * (rounds * m.step + more * m.more) +
+                      mb * m.mb + std::max(0.0, mb - 90) * m.far;
+    if (best.shape < 0 || us < best.us) best = {c, us};
+  }
+  return best;
+}
+
+void launch_w8a8_few(const W8Args& a, int shape, bool any, hipStream_t s) {
+  auto go = [&](auto c) {
+    constexpr FewShape F = kShapes[decltype(c)::value];
+    if constexpr (F.rt % 2 == 0) {
+      if (a.act != kNoAct) return launch_few<F.rt, F.mt, F.waves, F.depth, true>(a, any, s);
+    }
+    if constexpr (F.rt < 6) launch_few<F.rt, F.mt, F.waves, F.depth, false>(a, any, s);
   };
-  if (a.M <= 16) go(std::integral_constant<int, 1>{});
-  else if (a.M <= 32) go(std::integral_constant<int, 2>{});
-  else if (a.M <= 64) go(std::integral_constant<int, 4>{});
-  else go(std::integral_constant<int, 8>{});
+  auto pick = [&](auto&& self, auto c) {
+    if (shape == decltype(c)::value) go(c);
+    else if constexpr (decltype(c)::value + 1 < kNumShapes)
+      self(self, std::integral_constant<int, decltype(c)::value + 1>{});
+  };
+  pick(pick, std::integral_constant<int, 0>{});
 }
 
 }  // namespace cbq

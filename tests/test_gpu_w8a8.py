@@ -58,6 +58,44 @@ def test_gated(shape, act):
     assert bool((err <= bound).all()), float((err / bound).max())
 
 
+# Sizes that between them take every tile and shape of workgroup: whole, with K cut into
+# ranges, with rows of 16 bytes, of words and of any bytes, copied first or not.
+LINEAR_FORMS = [
+    (954, 16384, 512), (196, 20352, 9984), (1339, 8704, 256), (130, 8881, 9152), (2529, 221, 960),
+    (2115, 155, 6032), (242, 5966, 16), (2252, 121, 2832), (218, 214, 16), (935, 204, 16), (316, 1150, 16),
+    (364, 746, 688), (921, 640, 640), (760, 1507, 160), (1393, 651, 544), (734, 20635, 268),
+    (132, 8995, 10616), (952, 1378, 28), (2145, 106, 6980), (76, 268, 44), (68, 1430, 44), (924, 416, 24),
+    (439, 635, 632), (755, 939, 524), (130, 7152, 216), (1853, 450, 556), (385, 31933, 486),
+    (7111, 2205, 397), (141, 7955, 8394), (1511, 7743, 186), (2360, 416, 555), (2334, 131, 5274),
+    (351, 5388, 25), (2471, 755, 21), (162, 849, 17538), (2222, 111, 2841), (89, 301, 34), (326, 406, 30),
+    (100, 3996, 23), (1489, 188, 517), (284, 2154, 569), (952, 1711, 37), (99, 6294, 714),
+    (129, 7041, 12032), (19, 102, 16), (33, 5295, 16), (1310, 385, 528), (18, 4098, 16), (17, 6550, 16),
+    (541, 393, 16), (1605, 135, 16), (19, 102, 20), (37, 5263, 20), (1176, 281, 524), (18, 4542, 20),
+    (33, 4157, 24), (1031, 272, 20), (1076, 150, 1076), (67, 11308, 2307), (17, 114, 17), (40, 2303, 17),
+    (17, 4496, 19), (34, 4322, 17), (19, 8352, 17)]
+GATED_FORMS = [
+    (1255, 6404, 432), (193, 8976, 11376), (825, 5287, 304), (135, 4464, 8272), (749, 1375, 464),
+    (67, 3316, 7360), (178, 5645, 16), (65, 5578, 7408), (75, 299, 32), (267, 738, 16), (119, 1388, 528),
+    (319, 1665, 160), (338, 776, 768), (129, 30593, 264), (129, 5996, 8636), (142, 3955, 40),
+    (133, 903, 13032), (125, 186, 40), (239, 973, 20), (82, 1409, 660), (852, 883, 132), (813, 362, 660),
+    (138, 30530, 429), (1235, 6441, 414), (131, 6100, 4211), (1093, 4885, 210), (2356, 179, 1041),
+    (893, 159, 12542), (228, 4360, 27), (714, 2173, 22), (88, 389, 13337), (67, 521, 26), (1226, 172, 23),
+    (69, 1599, 555), (665, 1263, 39), (1713, 174, 591),
+    (138, 4264, 9760), (2226, 107, 2768), (17, 101, 16), (18, 2089, 16), (18, 4816, 2608), (2254, 102,
+    1508), (19, 101, 20), (17, 4330, 20), (1087, 129, 24), (65, 100, 14398), (2303, 261, 10515), (20,
+    100, 17), (34, 2230, 17)]
+
+
+@pytest.mark.parametrize("i,shape", list(enumerate(LINEAR_FORMS)))
+def test_linear_by_every_form(i, shape):
+    test_linear_to_the_last_bit(i + 100, shape)
+
+
+@pytest.mark.parametrize("i,shape", list(enumerate(GATED_FORMS)))
+def test_gated_by_every_form(i, shape):
+    test_gated(shape, P.ACTS[i % 4])
+
+
 @pytest.mark.parametrize("m", [2, 40, 65, 300])
 def test_sums_of_the_largest_codes(m):
     """The longest rows of the largest codes, -128 among them: 2^14 K < 2^31."""
@@ -106,7 +144,7 @@ def test_less_workspace_gives_the_same():
     import ctypes
     from cublade_amd import _abi
     L = _abi.lib()
-    for m, n, k in ((200, 512, 8192), (900, 300, 1403), (700, 260, 11003)):
+    for m, n, k in ((2115, 155, 6032), (2360, 416, 555), (2334, 131, 5274)):
         (x, sx), (w, sw) = P.codes(m, k, 1), P.codes(n, k, 2)
         need = L.cbq_w8a8_ws_bytes(m, n, k, 1)
         assert need > _abi.WS_CTRL_BYTES
