@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -60,9 +61,15 @@ def _check_cuda(x: torch.Tensor, what: str) -> None:
         raise RuntimeError(f"{what}: x must be on CUDA, got {x.device}")
 
 
+@functools.lru_cache(maxsize=4096)
+def _ws_bytes(device: int | None, m: int, n: int, k: int, projections: int) -> int:
+    """Workspace of a call on the current device, by its sizes alone."""
+    return _abi.lib().cbq_w8a8_ws_bytes(m, n, k, projections)
+
+
 def _run(call, args, dev: torch.device, size, what: str) -> None:
     with _abi.on_device(dev):
-        need = _abi.lib().cbq_w8a8_ws_bytes(*size)
+        need = _ws_bytes(dev.index, *size)
         if need <= _abi.WS_CTRL_BYTES:      # one launch that passes nothing on
             rc = call(*args, None, 0, _abi.stream_handle(dev))
         else:
