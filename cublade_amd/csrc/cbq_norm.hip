@@ -19,6 +19,7 @@
 // A NaN or an infinity in a row makes its maximum NaN (maxima are taken over the bit
 // patterns of absolute values, where a NaN is above everything) and with it the scale:
 // the token's outputs of a product are NaN rather than those of zero codes.
+#include <algorithm>
 #include <type_traits>
 
 #include "cbq_device.h"
@@ -199,7 +200,7 @@ struct Norm {
 };
 
 __device__ __forceinline__ float rstd_of(float ss, const Norm& n) {
-  return __builtin_amdgcn_rsqf(ss * n.inv_h + n.eps);
+  return rsqrtf(ss * n.inv_h + n.eps);   // eps may be 0, and v_rsq_f32 takes no denormals
 }
 
 // The codes of 8 values, and the row's stored scale.
@@ -523,10 +524,29 @@ extern "C" int cbq_norm(const cbq_norm_args* p, cbq_stream_t stream) {
   if (a.gate && a.gate_channel_stride) odd = odd || !even(a.gate, a.gate_token_stride, g_size);
   hipStream_t s = as_stream(stream);
   const int rt = a.residual ? a.residual_dtype : a.x_dtype;
-  if (a.x_dtype == CBQ_F32) launch_norm<kF32, kF32>(args, odd, s);
-  else if (a.x_dtype == CBQ_F16 && rt == CBQ_F16) launch_norm<kF16, kF16>(args, odd, s);
-  else if (a.x_dtype == CBQ_F16) launch_norm<kF16, kF32>(args, odd, s);
-  else if (rt == CBQ_BF16) launch_norm<kBF16, kBF16>(args, odd, s);
-  else launch_norm<kBF16, kF32>(args, odd, s);
+  // A grid has fewer than 2^32 threads, up to 1024 for a row.
+  constexpr int64_t kRows = 1 << 21;
+  auto bytes = [](int dt) { return dt == CBQ_F32 ? 4 : dt == CBQ_I8 ? 1 : 2; };
+  const int64_t H = a.hidden, tokens = a.tokens;
+  for (int64_t t = 0; t < tokens; t += kRows) {
+    Args part = args;
+    cbq_norm_args& b = part.a;
+    auto skip = [&](auto& q, int64_t elements, int dt) {
+      using T = std::remove_reference_t<decltype(q)>;
+      if (q) q = reinterpret_cast<T>(reinterpret_cast<uintptr_t>(q) + elements * bytes(dt));
+    };
+    b.tokens = std::min(kRows, tokens - t);
+    skip(b.x, t * a.x_stride, a.x_dtype);
+    skip(b.residual, t * a.residual_stride, rt);
+    skip(b.gate, t * a.gate_token_stride, a.gate_dtype);
+    skip(b.h, t * H, rt);
+    skip(b.out, t * H, a.out_dtype);
+    if (b.scale) b.scale += t;
+    if (a.x_dtype == CBQ_F32) launch_norm<kF32, kF32>(part, odd, s);
+    else if (a.x_dtype == CBQ_F16 && rt == CBQ_F16) launch_norm<kF16, kF16>(part, odd, s);
+    else if (a.x_dtype == CBQ_F16) launch_norm<kF16, kF32>(part, odd, s);
+    else if (rt == CBQ_BF16) launch_norm<kBF16, kBF16>(part, odd, s);
+    else launch_norm<kBF16, kF32>(part, odd, s);
+  }
   return launch_status("cbq_norm");
 }

@@ -494,7 +494,8 @@ W8Plan w8_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, size_t room 
   // Copies read and write M K + N K bytes at 4 TB/s and take a launch. Where rows are no
   // whole words the tiles win that back from about 640 tokens on, else hardly ever.
   const size_t copies = align256(static_cast<size_t>(M + proj * N) * p.kp);
-  p.pad = rows == kRows1 && M >= 640 && p.part_off + copies <= room;
+  p.pad = rows == kRows1 && M >= 640 && p.part_off + copies <= room &&
+          copies < (static_cast<size_t>(1) << 36);   // a grid has fewer than 2^32 threads
   if (p.pad) {
     p.part_off += copies;
     rows = kRows16;
@@ -621,7 +622,7 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
   a.splits = 1;
   hipStream_t s = as_stream(stream);
   if (K < 16) {
-    CBQ_REQUIRE(cdiv(M * N, kBlock) < (1LL << 31), "%s: too many outputs", what);
+    CBQ_REQUIRE(M * N < (1LL << 32) - kBlock, "%s: fewer than 16 columns take less than 2^32 outputs", what);
     with_act(act, [&](auto c) {
       k_w8_short<decltype(c)::value><<<static_cast<unsigned>(cdiv(M * N, kBlock)), kBlock, 0, s>>>(a);
     });
@@ -645,7 +646,6 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
     const int64_t count[3] = {M, N, proj == 2 ? N : 0};
     for (int o = 0; o < 3; ++o) c.first[o + 1] = c.first[o] + count[o] * (p.kp / 16);
     const int64_t grid = cdiv(c.first[3], kBlock);
-    CBQ_REQUIRE(grid < (1LL << 31), "%s: too many rows", what);
     k_w8_pad<<<static_cast<unsigned>(grid), kBlock, 0, s>>>(c);
     a.x = c.dst;
     a.w[0] = c.dst + c.first[1] * 16;

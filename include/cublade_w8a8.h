@@ -72,7 +72,7 @@ int cbq_w8a8_gated(const cbq_i8_rows* x, const cbq_i8_rows* gate, const cbq_i8_r
  * gate[t gate_token_stride + c gate_channel_stride]. out: contiguous. scale:
  * [tokens]. Every tensor is aligned to its elements. h and out do not overlap
  * what is read. All in fp32: sums of squares overflow (n = 0) where a token's
- * elements pass about 2^63. One launch. */
+ * elements pass about 2^63. One launch for each 2^21 tokens. */
 enum { CBQ_NORM_RMS = 0, CBQ_NORM_LAYER = 1 };
 
 typedef struct {

@@ -172,6 +172,39 @@ def test_views_are_read_in_place():
         P.check_codes(n.data, n.scale, *P.norm(stored, zero, "rms", 1e-6, None, None))
 
 
+def test_more_tokens_than_a_launch_takes():
+    """2^21 tokens to a launch: tokens on both sides of the border and at the end."""
+    from cublade_amd.quantization import norm_tensor, residual_norm
+    m, hidden = 2 * (1 << 21) + 5, 8
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x, r = (torch.randn(m, hidden, generator=g, device="cuda") for _ in range(2))
+    gate = torch.rand(m, 1, generator=g, device="cuda")
+    q = norm_tensor(x)
+    h, n = residual_norm(x, r, gate=gate, dtype=F32)
+    zero = torch.zeros(64, hidden, dtype=torch.float64)
+    for at in (0, (1 << 21) - 32, (1 << 22) - 60, m - 64):
+        c = slice(at, at + 64)
+        P.check_codes(q.data[c], q.scale[c], *P.norm(x[c].cpu().double(), zero, "rms", 1e-6, None, None))
+        want, bound = P.residual(x[c].cpu(), r[c].cpu(), "rms", 1e-6, False, None, None,
+                                 gate[c].cpu().expand(64, hidden), 1.0, F32)
+        stored = h[c].cpu().double()
+        assert bool(((stored - want).abs() <= bound).all())
+        want, bound = P.norm(stored, zero, "rms", 1e-6, None, None)
+        assert bool(((n[c].cpu().double() - want).abs() <= bound + want.abs() * 2.0 ** -24).all())
+
+
+def test_small_values_without_eps():
+    """eps = 0: the mean square of 2^-64 is 2^-128, a denormal; rows of one value, so the
+    sums are exact and the norm is 1 up to the division's, the root's and the product's
+    roundings (each at most 2^-23)."""
+    from cublade_amd.quantization import norm_tensor
+    for hidden in (64, 1000, 8192, 40000):
+        x = torch.full((3, hidden), 2.0 ** -64, device="cuda")
+        y = norm_tensor(x, eps=0.0, dtype=F32)
+        # 1 / hidden is rounded, and a denormal sum to 2^-149: 2^-21 of 2^-128
+        assert bool(((y - 1).abs() <= 3 * 2.0 ** -23 + 2.0 ** -21).all()), float((y - 1).abs().max())
+
+
 def test_empty_and_refusals_on_the_gpu():
     from cublade_amd.quantization import norm_tensor, residual_norm
     e = torch.zeros(0, 64, dtype=F16, device="cuda")

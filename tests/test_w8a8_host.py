@@ -60,6 +60,7 @@ def test_c_entries_refuse_bad_arguments():
     _refused(linear(x=rows(step=2)), "scale_stride")
     _refused(linear(y=None), "y is null")
     _refused(linear(y=4097), "aligned")
+    _refused(linear(m=1 << 20, n=1 << 13, k=8), "2^32")
     _refused(gated(act=4), "activation")
     _refused(gated(act=-1), "activation")
     _refused(gated(up=rows(scale=None)), "up has a null")
