@@ -138,9 +138,11 @@ def test_workspace_sizes():
     for p in (1, 2):
         assert L.cbq_w8a8_ws_bytes(4096, 8192, 1403, p) == C + 1408 * (4096 + p * 8192)
     # few tiles of long rows: planes of int32 sums (here of whole tiles), for each projection
-    one, two = (L.cbq_w8a8_ws_bytes(256, 1024, 11008, p) - C for p in (1, 2))
-    assert one % (256 * 1024 * 4) == 0 and two % (2 * 256 * 1024 * 4) == 0
-    assert 2 <= one // (256 * 1024 * 4) <= 8 and 2 <= two // (2 * 256 * 1024 * 4) <= 8
+    one, two = (L.cbq_w8a8_ws_bytes(2304, 256, 11008, p) - C for p in (1, 2))
+    assert one % (2304 * 256 * 4) == 0 and two % (2 * 2304 * 256 * 4) == 0
+    assert 2 <= one // (2304 * 256 * 4) <= 8 and 2 <= two // (2 * 2304 * 256 * 4) <= 8
+    # a small product by another kernel, which cuts nothing
+    assert L.cbq_w8a8_ws_bytes(256, 1024, 11008, 1) == C
 
 
 def test_quantized_operands_are_checked():
