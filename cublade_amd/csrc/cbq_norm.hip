@@ -451,11 +451,13 @@ void launch_rows(const Args& args, hipStream_t s) {
   const unsigned quads = static_cast<unsigned>(cdiv(tokens, kBlock / kWave));
   auto threads = [](int64_t per) { return static_cast<unsigned>(cdiv(per, kWave) * kWave); };
   // One chunk per thread for few tokens, where the chain of a row counts; two for
-  // many, where more rows in flight and fewer reductions do.
+  // many, where more rows in flight and fewer reductions do (16384 x 1152, one / two:
+  // 26.9 / 24.4 us, 16384 x 1408 29.7 / 28.0), but odd rows from 2048 elements on
+  // (16384 x 1403: 36 / 40).
   const bool many = tokens > 2 * device_cus();
   if (chunks <= kWave) k_norm<XT, RT, 1, true, ODD><<<quads, kBlock, 0, s>>>(args);
   else if (chunks <= 2 * kWave) k_norm<XT, RT, 2, true, ODD><<<quads, kBlock, 0, s>>>(args);
-  else if (chunks <= 1024 && !(many && chunks > 256))
+  else if (chunks <= 1024 && !(many && chunks > (ODD ? 256 : 128)))
     k_norm<XT, RT, 1, false, ODD><<<rows, threads(chunks), 0, s>>>(args);
   else if (chunks <= 2048) k_norm<XT, RT, 2, false, ODD><<<rows, threads(cdiv(chunks, 2)), 0, s>>>(args);
   else if (!ODD && chunks <= 4096) k_norm<XT, RT, 4, false, false><<<rows, threads(cdiv(chunks, 4)), 0, s>>>(args);
