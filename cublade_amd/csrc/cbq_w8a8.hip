@@ -14,8 +14,9 @@
 // stages filled by LDS DMA; one barrier per k-step, in front of its last quarter.
 //
 // LDS layout of a stage: the tile's rows of x, then its weight rows, 128 bytes each;
-// 16-byte chunk c of row r at c ^ (r & 7). In quarter s of a k-step the lanes of half h
-// (lane / 32) take chunk 2 s + h of both operands.
+// 16-byte chunk c of row r at c ^ (r / 2 & 7): no bank conflicts, where c ^ (r & 7) cost a
+// read 8 cycles instead of 4 (at the same time: the reads hide behind the products). In
+// quarter s of a k-step the lanes of half h (lane / 32) take chunk 2 s + h of both operands.
 //
 // A = weight rows, B = activation rows: lane l holds the outputs of token m = l % 32
 // and n = 8 (v / 4) + 4 (l / 32) + v % 4. Outputs leave through LDS, 32 tokens at a
@@ -112,7 +113,7 @@ __global__ __launch_bounds__(256) void k_w8_tile(W8Args a) {
   // products are not stored. Chunks past K are the last one's (ANY: see there); x counts
   // as zero there.
   const int lrow = lane >> 3;
-  const int lk = ((lane & 7) ^ lrow) << 4;
+  const int lk = ((lane & 7) ^ (((wave & 1) << 2) | (lrow >> 1))) << 4;
   uint32_t off[LT];                                     // of the row, from its base
   const uint8_t* base[LT];
 #pragma unroll
@@ -147,7 +148,7 @@ __global__ __launch_bounds__(256) void k_w8_tile(W8Args a) {
   const uint32_t xr = (wm * WM + r32) * 128, wr = G::kX + (wn * WR + r32) * 128;
   uint32_t slot[4];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) slot[s] = static_cast<uint32_t>((2 * s + h) ^ (r32 & 7)) << 4;
+  for (int s = 0; s < 4; ++s) slot[s] = static_cast<uint32_t>((2 * s + h) ^ (r32 >> 1 & 7)) << 4;
   i16x acc[J][I];          // [token tile][weight tile]
 #pragma unroll
   for (int j = 0; j < J; ++j)
