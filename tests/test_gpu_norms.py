@@ -193,6 +193,23 @@ def test_more_tokens_than_a_launch_takes():
         assert bool(((n[c].cpu().double() - want).abs() <= bound + want.abs() * 2.0 ** -24).all())
 
 
+def test_offsets_past_32_bits():
+    """More than 2^32 bytes of every tensor: the last tokens are those of their own call
+    with as many tokens as make it the same kernel."""
+    from cublade_amd.quantization import residual_norm
+    for m, hidden in ((300_000, 8192), (1_600_000, 1403)):
+        g = torch.Generator(device="cuda").manual_seed(9)
+        x = torch.randn(m, hidden, generator=g, device="cuda", dtype=BF16)
+        gate = torch.rand(m, hidden, generator=g, device="cuda", dtype=BF16)
+        h, n = residual_norm(x, x, gate=gate, dtype=BF16)
+        t = slice(m - 1000, m)
+        h2, n2 = residual_norm(x[t], x[t], gate=gate[t], dtype=BF16)
+        assert x.numel() * 2 > 1 << 32 and torch.equal(h[t], h2) and torch.equal(n[t], n2)
+        want, bound = P.residual(x[t].cpu(), x[t].cpu(), "rms", 1e-6, False, None, None, gate[t].cpu(), 1.0, BF16)
+        assert bool(((h2.cpu().double() - want).abs() <= bound).all())
+        del x, gate, h, n
+
+
 def test_small_values_without_eps():
     """eps = 0: the mean square of 2^-64 is 2^-128, a denormal; rows of one value, so the
     sums are exact and the norm is 1 up to the division's, the root's and the product's

@@ -139,6 +139,36 @@ def test_strided_rows_and_offsets():
             assert torch.equal(y.cpu(), want), (m, off, k)
 
 
+def test_offsets_past_32_bits():
+    """Codes of more than 2^31 bytes on either side and outputs of more than 2^32: the
+    last rows and columns are those of a call on them alone (and of the oracle)."""
+    from cublade_amd.quantization import gated_w8a8, linear_w8a8
+    g = torch.Generator(device="cuda").manual_seed(3)
+    many, few = 1_100_000, 2000
+    for k in (2048, 2044):                                # by DMA, and through registers
+        big = torch.randint(-127, 128, (many, k), generator=g, device="cuda", dtype=torch.int8)
+        sb = torch.rand(many, generator=g, device="cuda") * 0.01
+        w, sw = P.codes(few, k, 4)
+        tail = slice(many - 70, many)
+        small = P.linear(big[tail], sb[tail], w, sw, None, torch.float16)
+        y = linear_w8a8(P.qt(big, sb, torch.float16), P.qt(w, sw))
+        assert y.numel() * 2 > 1 << 32 and torch.equal(y[tail].cpu(), small)
+        y = gated_w8a8(P.qt(big, sb, torch.float16), P.qt(w, sw), P.qt(w, sw), activation="relu")
+        ref = gated_w8a8(P.qt(big[tail].contiguous(), sb[tail], torch.float16), P.qt(w, sw), P.qt(w, sw),
+                         activation="relu")
+        assert torch.equal(y[tail], ref)
+        del y
+        for m in (3, 20, 70, 300):                        # the large side as the weight
+            y = linear_w8a8(P.qt(w[:m], sw[:m], torch.float16), P.qt(big, sb))
+            # the product of the scales the other way round: two roundings each
+            want = P.sums(w[:m], big[tail]).double() * sw[:m].cpu().double()[:, None] * sb[tail].cpu().double()
+            got = y[:, tail].cpu().double()
+            # three roundings to fp32 and one to fp16 (normal numbers: the scales see to it,
+            # smaller results are within 2^-25)
+            assert bool(((got - want).abs() <= want.abs() * (2.0 ** -11 + 3 * 2.0 ** -24) + 2.0 ** -25).all()), m
+        del big, y
+
+
 def test_less_workspace_gives_the_same():
     """Without a workspace K is not cut and unaligned rows are not copied."""
     import ctypes
