@@ -37,9 +37,11 @@ typedef u32x2 __attribute__((aligned(4))) u32x2_a4;
 // bytes each. Odd rows: the elements t, t + nt, ..., one by one; vector loads that are
 // not on a multiple of 4 pass the address unit lane by lane, and a row's partial chunk
 // element by element takes more instructions than the rest of the row.
+// 32-bit indices, rows at addresses the wave has in common: a load or store is then one
+// instruction with its offset in a register.
 template <bool ODD>
-__device__ __forceinline__ int64_t index_of(int t, int nt, int v, int k) {
-  return ODD ? t + static_cast<int64_t>(8 * v + k) * nt : (t + static_cast<int64_t>(v) * nt) * 8 + k;
+__device__ __forceinline__ uint32_t index_of(int t, int nt, int v, int k) {
+  return ODD ? t + (8 * v + k) * nt : (t + v * nt) * 8 + k;
 }
 
 // Eight elements as loaded: even rows' words (16-bit types: the first 4), or an odd
@@ -47,12 +49,12 @@ __device__ __forceinline__ int64_t index_of(int t, int nt, int v, int k) {
 struct Raw { uint32_t w[8]; };
 
 template <int DT, bool ODD, bool NT = false>
-__device__ __forceinline__ Raw ld_raw(const void* row, int t, int nt, int v, int64_t H) {
+__device__ __forceinline__ Raw ld_raw(const void* row, int t, int nt, int v, uint32_t H) {
   Raw r = {};
   if constexpr (ODD) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int64_t e = index_of<true>(t, nt, v, k);
+      const uint32_t e = index_of<true>(t, nt, v, k);
       if (e < H) {
         if constexpr (DT == kF32) r.w[k] = static_cast<const uint32_t*>(row)[e];
         else r.w[k] = static_cast<const uint16_t*>(row)[e];
@@ -87,7 +89,7 @@ __device__ __forceinline__ void widen(const Raw& r, float (&f)[8]) {
 
 // The same for a type known at run time only (the same for all threads).
 template <bool ODD>
-__device__ __forceinline__ Raw ld_raw(const void* row, int dt, int t, int nt, int v, int64_t H) {
+__device__ __forceinline__ Raw ld_raw(const void* row, int dt, int t, int nt, int v, uint32_t H) {
   return dt == kF32 ? ld_raw<kF32, ODD>(row, t, nt, v, H) : ld_raw<kF16, ODD>(row, t, nt, v, H);
 }
 template <bool ODD>
@@ -111,11 +113,11 @@ __device__ __forceinline__ Raw narrow(const float (&f)[8]) {
 }
 
 template <int DT, bool ODD>
-__device__ __forceinline__ void st_raw(void* row, int t, int nt, int v, int64_t H, const Raw& r) {
+__device__ __forceinline__ void st_raw(void* row, int t, int nt, int v, uint32_t H, const Raw& r) {
   if constexpr (ODD) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int64_t e = index_of<true>(t, nt, v, k);
+      const uint32_t e = index_of<true>(t, nt, v, k);
       if (e < H) {
         if constexpr (DT == kF32) static_cast<uint32_t*>(row)[e] = r.w[k];
         else static_cast<uint16_t*>(row)[e] = static_cast<uint16_t>(r.w[k]);
@@ -217,13 +219,13 @@ struct Args {
 template <bool ODD>
 __device__ __forceinline__ void st_out(const cbq_norm_args& a, int64_t token, int t, int nt, int v,
                                        const float (&f)[8], float inv) {
-  const int64_t H = a.hidden;
+  const uint32_t H = static_cast<uint32_t>(a.hidden);
   if (a.out_dtype == CBQ_I8) {
-    uint8_t* row = static_cast<uint8_t*>(a.out) + token * H;
+    uint8_t* row = static_cast<uint8_t*>(a.out) + token * a.hidden;
     if constexpr (ODD) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const int64_t e = index_of<true>(t, nt, v, k);
+        const uint32_t e = index_of<true>(t, nt, v, k);
         if (e < H) row[e] = static_cast<uint8_t>(q_int8(f[k] * inv));
       }
     } else if (index_of<false>(t, nt, v, 0) < H) {
@@ -232,7 +234,7 @@ __device__ __forceinline__ void st_out(const cbq_norm_args& a, int64_t token, in
     }
     return;
   }
-  char* row = static_cast<char*>(a.out) + token * H * (a.out_dtype == CBQ_F32 ? 4 : 2);
+  char* row = static_cast<char*>(a.out) + token * a.hidden * (a.out_dtype == CBQ_F32 ? 4 : 2);
   if (a.out_dtype == CBQ_F32) st_raw<kF32, ODD>(row, t, nt, v, H, narrow<kF32, ODD>(f));
   else if (a.out_dtype == CBQ_F16) st_raw<kF16, ODD>(row, t, nt, v, H, narrow<kF16, ODD>(f));
   else st_raw<kBF16, ODD>(row, t, nt, v, H, narrow<kBF16, ODD>(f));
@@ -254,8 +256,9 @@ template <int XT, int RT, int V, bool WAVE, bool ODD>
 __global__ __launch_bounds__(WAVE ? kBlock : 1024) void k_norm(Args args) {
   const cbq_norm_args& a = args.a;
   __shared__ uint32_t slots[5][2 * kMaxWaves];
-  const int64_t H = a.hidden;
-  const int64_t token = WAVE ? static_cast<int64_t>(blockIdx.x) * (kBlock / kWave) + threadIdx.x / kWave
+  const uint32_t H = static_cast<uint32_t>(a.hidden);
+  const int64_t token = WAVE ? blockIdx.x * (kBlock / kWave) +
+                                   __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave)
                              : blockIdx.x;
   if (WAVE && token >= a.tokens) return;
   const int t = WAVE ? threadIdx.x % kWave : threadIdx.x;
@@ -344,7 +347,7 @@ __global__ __launch_bounds__(WAVE ? kBlock : 1024) void k_norm(Args args) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[v][k] = r[k] + a.alpha * f[v][k];
       const Raw o = narrow<RT, ODD>(f[v]);
-      st_raw<RT, ODD>(static_cast<char*>(a.h) + token * H * elem_bytes<RT>(), t, nt, v, H, o);
+      st_raw<RT, ODD>(static_cast<char*>(a.h) + token * a.hidden * elem_bytes<RT>(), t, nt, v, H, o);
       widen<RT, ODD>(o, f[v]);
     }
     each([&](int v, int k) { f[v][k] = inside(v, k) ? f[v][k] : 0.0f; });
