@@ -48,16 +48,17 @@ __device__ __forceinline__ uint32_t index_of(int t, int nt, int v, int k) {
 // row's elements.
 struct Raw { uint32_t w[8]; };
 
-template <int DT, bool ODD, bool NT = false>
+template <int DT, bool ODD, bool CLAMP, bool NT = false>
 __device__ __forceinline__ Raw ld_raw(const void* row, int t, int nt, int v, uint32_t H) {
   Raw r = {};
   if constexpr (ODD) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const uint32_t e = index_of<true>(t, nt, v, k);
-      if (e < H) {
-        if constexpr (DT == kF32) r.w[k] = static_cast<const uint32_t*>(row)[e];
-        else r.w[k] = static_cast<const uint16_t*>(row)[e];
+      if (CLAMP || e < H) {
+        const uint32_t c = CLAMP ? min(e, H - 1) : e;
+        if constexpr (DT == kF32) r.w[k] = static_cast<const uint32_t*>(row)[c];
+        else r.w[k] = static_cast<const uint16_t*>(row)[c];
       }
     }
   } else if (index_of<false>(t, nt, v, 0) < H) {
@@ -88,9 +89,9 @@ __device__ __forceinline__ void widen(const Raw& r, float (&f)[8]) {
 }
 
 // The same for a type known at run time only (the same for all threads).
-template <bool ODD>
+template <bool ODD, bool CLAMP>
 __device__ __forceinline__ Raw ld_raw(const void* row, int dt, int t, int nt, int v, uint32_t H) {
-  return dt == kF32 ? ld_raw<kF32, ODD>(row, t, nt, v, H) : ld_raw<kF16, ODD>(row, t, nt, v, H);
+  return dt == kF32 ? ld_raw<kF32, ODD, CLAMP>(row, t, nt, v, H) : ld_raw<kF16, ODD, CLAMP>(row, t, nt, v, H);
 }
 template <bool ODD>
 __device__ __forceinline__ void widen(const Raw& r, int dt, float (&f)[8]) {
@@ -264,17 +265,21 @@ __global__ __launch_bounds__(WAVE ? kBlock : 1024) void k_norm(Args args) {
   const int t = WAVE ? threadIdx.x % kWave : threadIdx.x;
   const int nt = WAVE ? kWave : blockDim.x;
 
-  // All of the row's loads first.
+  // All of the row's loads first. Odd rows, one element at a time: loads past the row's end
+  // take the last element again, whose value is not used, since a load under a condition
+  // waits for the one before (3001 x 1403: 15.4 -> 13.9 us); not with two chunks, whose
+  // loads would all need registers at once.
+  constexpr bool CLAMP = V == 1;
   Raw rx[V], rr[V], rw[V];
   auto loads = [&](auto stream) {
     constexpr bool NT = decltype(stream)::value;
 #pragma unroll
     for (int v = 0; v < V; ++v)
-      rx[v] = ld_raw<XT, ODD, NT>(row_of<XT>(a.x, token, a.x_stride), t, nt, v, H);
+      rx[v] = ld_raw<XT, ODD, CLAMP, NT>(row_of<XT>(a.x, token, a.x_stride), t, nt, v, H);
     if (a.residual) {
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        rr[v] = ld_raw<RT, ODD, NT>(row_of<RT>(a.residual, token, a.residual_stride), t, nt, v, H);
+        rr[v] = ld_raw<RT, ODD, CLAMP, NT>(row_of<RT>(a.residual, token, a.residual_stride), t, nt, v, H);
     }
   };
   if (args.stream) loads(std::true_type{});
@@ -282,7 +287,7 @@ __global__ __launch_bounds__(WAVE ? kBlock : 1024) void k_norm(Args args) {
   constexpr bool HELD = V <= 2 && !ODD;   // else no registers to spare
   if (HELD && a.weight) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) rw[v] = ld_raw<ODD>(a.weight, a.param_dtype, t, nt, v, H);
+    for (int v = 0; v < V; ++v) rw[v] = ld_raw<ODD, CLAMP>(a.weight, a.param_dtype, t, nt, v, H);
   }
   float f[V][8];
 #pragma unroll
@@ -295,6 +300,7 @@ __global__ __launch_bounds__(WAVE ? kBlock : 1024) void k_norm(Args args) {
       for (int k = 0; k < 8; ++k) fn(v, k);
   };
   auto inside = [&](int v, int k) { return index_of<ODD>(t, nt, v, ODD ? k : 0) < H; };
+  if constexpr (ODD && CLAMP) each([&](int v, int k) { f[v][k] = inside(v, k) ? f[v][k] : 0.0f; });
   // layer: the mean leaves f. Elements past the row stay zero.
   auto centre = [&](uint32_t* s) {
     if (!args.n.layer) return;
@@ -314,7 +320,7 @@ __global__ __launch_bounds__(WAVE ? kBlock : 1024) void k_norm(Args args) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       float w[8];
-      widen<ODD>(held ? held[v] : ld_raw<ODD>(p, dt, t, nt, v, H), dt, w);
+      widen<ODD>(held ? held[v] : ld_raw<ODD, CLAMP>(p, dt, t, nt, v, H), dt, w);
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[v][k] = op(f[v][k], w[k]);
     }
@@ -455,12 +461,12 @@ void launch_rows(const Args& args, hipStream_t s) {
   auto threads = [](int64_t per) { return static_cast<unsigned>(cdiv(per, kWave) * kWave); };
   // One chunk per thread for few tokens, where the chain of a row counts; two for
   // many, where more rows in flight and fewer reductions do (16384 x 1152, one / two:
-  // 26.9 / 24.4 us, 16384 x 1408 29.7 / 28.0), but odd rows from 2048 elements on
-  // (16384 x 1403: 36 / 40).
+  // 26.9 / 24.4 us, 16384 x 1408 29.7 / 28.0), but for odd rows from 4096 elements on
+  // (4096 x 2049: 15.6 / 16.3, 4096 x 8001 54 / 51).
   const bool many = tokens > 2 * device_cus();
   if (chunks <= kWave) k_norm<XT, RT, 1, true, ODD><<<quads, kBlock, 0, s>>>(args);
   else if (chunks <= 2 * kWave) k_norm<XT, RT, 2, true, ODD><<<quads, kBlock, 0, s>>>(args);
-  else if (chunks <= 1024 && !(many && chunks > (ODD ? 256 : 128)))
+  else if (chunks <= 1024 && !(many && chunks > (ODD ? 512 : 128)))
     k_norm<XT, RT, 1, false, ODD><<<rows, threads(chunks), 0, s>>>(args);
   else if (chunks <= 2048) k_norm<XT, RT, 2, false, ODD><<<rows, threads(cdiv(chunks, 2)), 0, s>>>(args);
   else if (!ODD && chunks <= 4096) k_norm<XT, RT, 4, false, false><<<rows, threads(cdiv(chunks, 4)), 0, s>>>(args);
