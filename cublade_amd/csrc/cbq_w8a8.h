@@ -125,8 +125,8 @@ inline void with_act(int act, F&& f) {
 // What rows of codes and their strides are multiples of.
 enum { kRows16, kRows4, kRows1 };
 
-// cbq_w8a8_few.hip: few rows of x, or few outputs; K >= 16. The shape for these sizes and
-// its modelled time; any: rows that are no multiples of 16 bytes. Returns after queueing.
+// cbq_w8a8_few.hip: few rows of x, or few outputs; K >= 16. The shape for these sizes (-1:
+// none) and its modelled time; any: rows that are no multiples of 16 bytes. Returns after queueing.
 constexpr int kFewRows = 2048;
 struct FewPlan { int shape; double us; };
 FewPlan few_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, int cus);

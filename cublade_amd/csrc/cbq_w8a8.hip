@@ -489,7 +489,7 @@ W8Plan w8_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, size_t room 
   p.bytes = CBQ_WS_CTRL_BYTES;
   const FewPlan few = M <= kFewRows ? few_plan(M, N, K, proj, rows, cus) : FewPlan{-1, 0.0};
   p.few = few.shape;
-  if (M <= 64) return p;     // 64 x 11008 x 4096, gated: 24 us, by tiles 22; mostly a third of the tiles' time
+  if (M <= 64 && p.few >= 0) return p;   // 64 x 11008 x 4096, gated: 24 us, by tiles 22; mostly a third of the tiles' time
   p.kp = cdiv(K, 16) * 16;
   p.part_off = CBQ_WS_CTRL_BYTES;
   // Copies read and write M K + N K bytes at 4 TB/s and take a launch. Where rows are no

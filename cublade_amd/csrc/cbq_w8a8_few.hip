@@ -275,6 +275,7 @@ FewPlan few_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, int cus) {
     // read the weight as often.
     if (f.rt % proj || (f.rt == 6 && proj == 1) || (f.mt > 1 && M <= 8 * f.mt) || (f.mt == 1 && M > 64)) continue;
     const int64_t wgs = cdiv(cdiv(N, 16 * (f.rt / proj)), 8) * 8 * cdiv(M, 16 * f.mt), steps = cdiv(cdiv(K, 128), f.waves);
+    if (wgs * f.waves >= 1 << 26) continue;   // a grid has fewer than 2^32 threads
     const int64_t lds = f.waves * (rows == kRows16 ? f.depth : 1) * (f.rt + f.mt) * 2048 + f.rt * f.mt * 1024;
     const int64_t per_cu = std::min<int64_t>(160 * 1024 / lds, 2048 / (64 * f.waves));
     const int64_t full = wgs / (per_cu * cus), rem = wgs - full * per_cu * cus;

@@ -169,6 +169,22 @@ def test_offsets_past_32_bits():
         del big, y
 
 
+def test_more_channels_than_a_grid_of_few_rows_takes():
+    from cublade_amd.quantization import gated_w8a8, linear_w8a8
+    g = torch.Generator(device="cuda").manual_seed(5)
+    n, k = (1 << 27) + 40, 16
+    w = torch.randint(-127, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    sw = torch.rand(n, generator=g, device="cuda") * 0.01
+    for m in (1, 3):
+        x, sx = P.codes(m, k, 6)
+        y = linear_w8a8(P.qt(x, sx, torch.float32), P.qt(w, sw))
+        u = gated_w8a8(P.qt(x, sx, torch.float32), P.qt(w, sw), P.qt(w, sw), activation="relu")
+        for c in (slice(0, 200), slice(1 << 26, (1 << 26) + 200), slice(n - 200, n)):
+            want = P.linear(x, sx, w[c], sw[c], None, torch.float32)
+            assert torch.equal(y[:, c].cpu(), want)
+            assert torch.equal(u[:, c].cpu(), want.clamp(min=0) * want)
+
+
 def test_less_workspace_gives_the_same():
     """Without a workspace K is not cut and unaligned rows are not copied."""
     import ctypes
