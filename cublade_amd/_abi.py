@@ -136,6 +136,7 @@ class NormArgs(ctypes.Structure):
 
 
 W8A8_SIGNATURES = {
+    "cbq_quant_int8_tokens": (_I32, [_P, _I32, _I64, _I64, _F, _P, _SZ, _P, _P, _P]),
     "cbq_w8a8_ws_bytes": (_SZ, [_I64, _I64, _I64, _I32]),
     "cbq_w8a8_linear": (_I32, [_P, _P, _P, _I32, _I64, _I64, _I64, _P, _I32, _P, _SZ, _P]),
     "cbq_w8a8_gated": (_I32, [_P, _P, _P, _P, _P, _I32, _I32, _I64, _I64, _I64, _P, _I32, _P, _SZ,

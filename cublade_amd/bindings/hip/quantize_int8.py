@@ -84,6 +84,30 @@ def quantize_per_channel_int8(
     return q, scale
 
 
+def quantize_tokens_int8(x: torch.Tensor, eps: float = 1e-12) -> tuple[torch.Tensor, torch.Tensor]:
+    """quantize_per_channel_int8 of a [tokens, features] tensor (axis 0; the same
+    bits), but a token that holds a NaN or an infinity gets a NaN scale: a product's
+    row is then NaN, where codes that leave the NaN out would make it finite. An
+    extension: the activations of the W8A8 layers (include/cublade_w8a8.h)."""
+    code = check_float_input(x, allow_f32=True)
+    if x.dim() != 2:
+        raise RuntimeError(f"x must be [tokens, features], got {tuple(x.shape)}")
+    dev = x.device
+    tokens, features = x.shape
+    q = out_like(x, torch.int8)
+    if tokens == 0 or features == 0:
+        return q, torch.zeros((tokens,), dtype=torch.float32, device=dev)
+    scale = torch.empty((tokens,), dtype=torch.float32, device=dev)
+    L = _abi.lib()
+    with _abi.on_device(dev), _abi.workspace_lock(dev):
+        ws = _abi.workspace(dev, L.cbq_quant_int8_channel_ws_bytes(tokens, features, 0))
+        rc = L.cbq_quant_int8_tokens(_abi.ptr(x), code, tokens, features, float(eps), _abi.ptr(ws),
+                                     ws.numel(), _abi.ptr(q), _abi.ptr(scale),
+                                     _abi.stream_handle(dev))
+    _abi.check(rc, "quantize_tokens_int8")
+    return q, scale
+
+
 def quantize_per_group_int8(
     x_grouped: torch.Tensor,
     group_size: int,

@@ -160,11 +160,21 @@ __device__ __forceinline__ float ld1(const void* base, int64_t i) {
   }
 }
 
-// |x| max over a chunk. fmaxf returns the non-NaN operand, so NaN inputs are
-// ignored exactly as the reference's fmaxf fold does.
+// The larger of two absolute values. fmaxf returns the non-NaN operand, so NaN
+// inputs are ignored exactly as the reference's fmaxf fold does. KEEP: a NaN is
+// kept instead (as bits without a sign a NaN is above everything).
+template <bool KEEP = false>
+__device__ __forceinline__ float max_abs(float a, float b) {
+  if constexpr (!KEEP) return fmaxf(a, b);
+  const uint32_t u = __float_as_uint(a), v = __float_as_uint(b);
+  return __uint_as_float(u > v ? u : v);
+}
+
+// |x| max over a chunk.
+template <bool KEEP = false>
 __device__ __forceinline__ float absmax8(const float (&f)[8], float m) {
 #pragma unroll
-  for (int k = 0; k < 8; ++k) m = fmaxf(m, __builtin_fabsf(f[k]));
+  for (int k = 0; k < 8; ++k) m = max_abs<KEEP>(m, __builtin_fabsf(f[k]));
   return m;
 }
 
@@ -283,27 +293,28 @@ __device__ __forceinline__ float dpp_f32(float v) {
       float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, false));
 }
 
-template <int LPR>
+template <int LPR, bool KEEP = false>
 __device__ __forceinline__ float group_max(float m) {
   static_assert(LPR >= 1 && LPR <= 64 && (LPR & (LPR - 1)) == 0, "LPR");
-  if constexpr (LPR >= 2) m = fmaxf(m, dpp_f32<0xB1>(m));   // quad_perm [1,0,3,2]
-  if constexpr (LPR >= 4) m = fmaxf(m, dpp_f32<0x4E>(m));   // quad_perm [2,3,0,1]
-  if constexpr (LPR >= 8) m = fmaxf(m, dpp_f32<0x141>(m));  // row_half_mirror
-  if constexpr (LPR >= 16) m = fmaxf(m, dpp_f32<0x140>(m)); // row_mirror
-  if constexpr (LPR >= 32) m = fmaxf(m, __shfl_xor(m, 16, kWave));
-  if constexpr (LPR >= 64) m = fmaxf(m, __shfl_xor(m, 32, kWave));
+  if constexpr (LPR >= 2) m = max_abs<KEEP>(m, dpp_f32<0xB1>(m));   // quad_perm [1,0,3,2]
+  if constexpr (LPR >= 4) m = max_abs<KEEP>(m, dpp_f32<0x4E>(m));   // quad_perm [2,3,0,1]
+  if constexpr (LPR >= 8) m = max_abs<KEEP>(m, dpp_f32<0x141>(m));  // row_half_mirror
+  if constexpr (LPR >= 16) m = max_abs<KEEP>(m, dpp_f32<0x140>(m)); // row_mirror
+  if constexpr (LPR >= 32) m = max_abs<KEEP>(m, __shfl_xor(m, 16, kWave));
+  if constexpr (LPR >= 64) m = max_abs<KEEP>(m, __shfl_xor(m, 32, kWave));
   return m;
 }
 
 // Workgroup-wide max; every thread gets the result. `red` holds one slot per
 // wave. Contains a barrier: call from uniform control flow only.
+template <bool KEEP = false>
 __device__ __forceinline__ float block_max(float m, float* red) {
-  m = group_max<kWave>(m);
+  m = group_max<kWave, KEEP>(m);
   const int wave = threadIdx.x / kWave;
   if ((threadIdx.x % kWave) == 0) red[wave] = m;
   __syncthreads();
   float r = red[0];
-  for (int w = 1; w < static_cast<int>(blockDim.x) / kWave; ++w) r = fmaxf(r, red[w]);
+  for (int w = 1; w < static_cast<int>(blockDim.x) / kWave; ++w) r = max_abs<KEEP>(r, red[w]);
   __syncthreads();
   return r;
 }
@@ -413,6 +424,14 @@ constexpr int kAuxSc1 = 16;
 // is the same value; quantize_per_tensor_fp8.cu:99-102 intends the same).
 __device__ __forceinline__ float inv_scale(float amax, float eps, float qmax) {
   return qmax / fmaxf(amax, eps);
+}
+
+// The same for INT8 rows whose maximum kept a NaN (KEEP): NaN, and with it the stored
+// scale, where the row holds a NaN or an infinity.
+template <bool KEEP>
+__device__ __forceinline__ float row_inv(float amax, float eps) {
+  if (KEEP && !(amax <= 3.402823466e38f)) return __builtin_nanf("");
+  return inv_scale(amax, eps, kQmaxInt8);
 }
 
 }  // namespace cbq

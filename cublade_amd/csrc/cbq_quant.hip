@@ -81,6 +81,7 @@
 
 #include "cbq_device.h"
 #include "cbq_host.h"
+#include "cublade_w8a8.h"
 
 namespace cbq {
 namespace {
@@ -135,11 +136,12 @@ __global__ __launch_bounds__(kBlock) void k_amax_tensor(
 }
 
 // Maximum of the nparts partial maxima -> inv; every thread gets it.
+template <bool KEEP = false>
 __device__ __forceinline__ float reduce_partials(const float* __restrict__ partial, int nparts,
                                                  float* red) {
   float m = 0.0f;
-  for (int i = threadIdx.x; i < nparts; i += kBlock) m = fmaxf(m, partial[i]);
-  return block_max(m, red);
+  for (int i = threadIdx.x; i < nparts; i += kBlock) m = max_abs<KEEP>(m, partial[i]);
+  return block_max<KEEP>(m, red);
 }
 
 // Persistent grid (the amax pass's): each workgroup issues its first chunk
@@ -1043,7 +1045,7 @@ __global__ __launch_bounds__(kFusedBlock) void k_quant_tensor_small(
 // Rows of L = LPR * VPL * 8 elements; LPR lanes own a row, each lane holding
 // VPL chunks. A wave covers 64 / LPR rows per iteration and RI iterations,
 // all loads issued before the first reduction.
-template <int DT, int LPR, int VPL, int RI>
+template <int DT, int LPR, int VPL, int RI, bool KEEP>
 __global__ __launch_bounds__(kBlock) void k_rows_sub(
     const void* __restrict__ x, int64_t rows, float eps, int8_t* __restrict__ q,
     float* __restrict__ scale) {
@@ -1075,11 +1077,11 @@ __global__ __launch_bounds__(kBlock) void k_rows_sub(
 #pragma unroll
       for (int v = 0; v < VPL; ++v) {
         cvt8<DT>(r[it][v], f[v]);
-        m = absmax8(f[v], m);
+        m = absmax8<KEEP>(f[v], m);
       }
     }
-    m = group_max<LPR>(m);   // every lane participates
-    const float inv = inv_scale(m, eps, kQmaxInt8);
+    m = group_max<LPR, KEEP>(m);   // every lane participates
+    const float inv = row_inv<KEEP>(m, eps);
     if (ok) {
 #pragma unroll
       for (int v = 0; v < VPL; ++v)
@@ -1094,7 +1096,7 @@ __global__ __launch_bounds__(kBlock) void k_rows_sub(
 // k_rows_sub with LPR * VPL >= cg chunk slots per row, chunk j = v * LPR + lr
 // in slot (v, lr); slots past cg load the row's first chunk (in bounds), stay
 // out of the maximum and store nothing.
-template <int DT, int LPR, int VPL, int RI>
+template <int DT, int LPR, int VPL, int RI, bool KEEP>
 __global__ __launch_bounds__(kBlock) void k_rows_sub_any(
     const void* __restrict__ x, int64_t rows, int cg, float eps, int8_t* __restrict__ q,
     float* __restrict__ scale) {
@@ -1129,12 +1131,12 @@ __global__ __launch_bounds__(kBlock) void k_rows_sub_any(
 #pragma unroll
       for (int v = 0; v < VPL; ++v) {
         cvt8<DT>(r[it][v], f[v]);
-        const float mv = absmax8(f[v], 0.0f);
-        m = v * LPR + lr < cg ? fmaxf(m, mv) : m;
+        const float mv = absmax8<KEEP>(f[v], 0.0f);
+        m = v * LPR + lr < cg ? max_abs<KEEP>(m, mv) : m;
       }
     }
-    m = group_max<LPR>(m);   // every lane participates
-    const float inv = inv_scale(m, eps, kQmaxInt8);
+    m = group_max<LPR, KEEP>(m);   // every lane participates
+    const float inv = row_inv<KEEP>(m, eps);
     if (ok) {
 #pragma unroll
       for (int v = 0; v < VPL; ++v) {
@@ -1168,7 +1170,7 @@ __device__ __forceinline__ void pair_f32(uint32_t w, float* f) {
 // dequant pass in groups of 100, E = 2 -> 4: bf16 [8192, 8000] 146 -> 85 us, fp16
 // [4099, 1400] 16.9 -> 12.8; rows of 1004 [8000, 1004] 15.0 -> 13.1; fp32 quant
 // [8192, 8000] 111 -> 64.
-template <int DT, int LPR, int VPL, int RI, int E>
+template <int DT, int LPR, int VPL, int RI, int E, bool KEEP>
 __global__ __launch_bounds__(kBlock) void k_rows_sub_any1(
     const void* __restrict__ x, int64_t rows, int L, float eps, int8_t* __restrict__ q,
     float* __restrict__ scale) {
@@ -1224,12 +1226,12 @@ __global__ __launch_bounds__(kBlock) void k_rows_sub_any1(
       for (int v = 0; v < VPL; ++v) {
         float mv = __builtin_fabsf(f[it][v][0]);
 #pragma unroll
-        for (int k = 1; k < E; ++k) mv = fmaxf(mv, __builtin_fabsf(f[it][v][k]));
-        m = v * LPR + lr < U ? fmaxf(m, mv) : m;
+        for (int k = 1; k < E; ++k) mv = max_abs<KEEP>(mv, __builtin_fabsf(f[it][v][k]));
+        m = v * LPR + lr < U ? max_abs<KEEP>(m, mv) : m;
       }
     }
-    m = group_max<LPR>(m);   // every lane participates
-    const float inv = inv_scale(m, eps, kQmaxInt8);
+    m = group_max<LPR, KEEP>(m);   // every lane participates
+    const float inv = row_inv<KEEP>(m, eps);
     if (ok) {
 #pragma unroll
       for (int v = 0; v < VPL; ++v) {
@@ -1260,7 +1262,7 @@ __global__ __launch_bounds__(kBlock) void k_rows_sub_any1(
 // k_rows_split_max writes one partial maximum per slice; k_rows_split_cast
 // reduces its row's partials (L2) while its first loads are in flight, then
 // casts its slice. L % 8 == 0, 16-byte aligned x, 8-byte aligned q.
-template <int DT>
+template <int DT, bool KEEP>
 __global__ __launch_bounds__(kBlock) void k_rows_split_max(
     const void* __restrict__ x, int64_t L, int64_t sc, float* __restrict__ partial) {
   __shared__ float red[kBlock / kWave];
@@ -1282,15 +1284,15 @@ __global__ __launch_bounds__(kBlock) void k_rows_split_max(
       if (c < c_end) {
         float f[8];
         cvt8<DT>(r[u], f);
-        m = absmax8(f, m);
+        m = absmax8<KEEP>(f, m);
       }
     }
   }
-  m = block_max(m, red);
+  m = block_max<KEEP>(m, red);
   if (threadIdx.x == 0) partial[row * gridDim.x + blockIdx.x] = m;
 }
 
-template <int DT>
+template <int DT, bool KEEP>
 __global__ __launch_bounds__(kBlock) void k_rows_split_cast(
     const void* __restrict__ x, int64_t L, int64_t sc, const float* __restrict__ partial,
     float eps, int8_t* __restrict__ q, float* __restrict__ scale) {
@@ -1305,8 +1307,8 @@ __global__ __launch_bounds__(kBlock) void k_rows_split_cast(
     const int64_t c = c0 + static_cast<int64_t>(u) * kBlock;
     if (c < c_end) r[u] = ld8<DT>(x, base + c * 8);
   }
-  const float m = reduce_partials(partial + row * gridDim.x, static_cast<int>(gridDim.x), red);
-  const float inv = inv_scale(m, eps, kQmaxInt8);
+  const float m = reduce_partials<KEEP>(partial + row * gridDim.x, static_cast<int>(gridDim.x), red);
+  const float inv = row_inv<KEEP>(m, eps);
   if (blockIdx.x == 0 && threadIdx.x == 0) scale[row] = 1.0f / inv;
   for (;;) {
 #pragma unroll
@@ -1332,7 +1334,7 @@ __global__ __launch_bounds__(kBlock) void k_rows_split_cast(
 // registers. Workgroups stride over rows (the row loop is uniform per
 // workgroup). Measured on MI355X, rows of 8192 bf16 (C3 axis 0): 512 threads
 // x 2 chunks 110.0 us, 256 x 4 111.4-113.7 us, 1024 x 1 148 us.
-template <int DT, int VPL, int B = kBlock>
+template <int DT, int VPL, int B, bool KEEP>
 __global__ __launch_bounds__(B) void k_rows_wg(
     const void* __restrict__ x, int64_t rows, float eps, int8_t* __restrict__ q,
     float* __restrict__ scale) {
@@ -1347,10 +1349,10 @@ __global__ __launch_bounds__(B) void k_rows_wg(
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
       cvt8<DT>(r[v], f[v]);
-      m = absmax8(f[v], m);
+      m = absmax8<KEEP>(f[v], m);
     }
-    m = block_max(m, red);
-    const float inv = inv_scale(m, eps, kQmaxInt8);
+    m = block_max<KEEP>(m, red);
+    const float inv = row_inv<KEEP>(m, eps);
 #pragma unroll
     for (int v = 0; v < VPL; ++v)
       stg8(q + row * L + (v * B + threadIdx.x) * 8, pack8_int8(f[v], inv));
@@ -1361,7 +1363,7 @@ __global__ __launch_bounds__(B) void k_rows_wg(
 // Any row length: one workgroup per row (striding over rows), a reduce pass
 // then a cast pass. vec != 0 requires L % 8 == 0 and 16-byte / 8-byte
 // aligned x / q.
-template <int DT>
+template <int DT, bool KEEP>
 __global__ __launch_bounds__(kBlock) void k_rows_generic(
     const void* __restrict__ x, int64_t rows, int64_t L, int vec, float eps,
     int8_t* __restrict__ q, float* __restrict__ scale) {
@@ -1374,14 +1376,14 @@ __global__ __launch_bounds__(kBlock) void k_rows_generic(
       for (int64_t c = threadIdx.x; c < nc; c += kBlock) {
         float f[8];
         cvt8<DT>(ld8<DT>(x, base + c * 8), f);
-        m = absmax8(f, m);
+        m = absmax8<KEEP>(f, m);
       }
     } else {
       for (int64_t i = threadIdx.x; i < L; i += kBlock)
-        m = fmaxf(m, __builtin_fabsf(ld1<DT>(x, base + i)));
+        m = max_abs<KEEP>(m, __builtin_fabsf(ld1<DT>(x, base + i)));
     }
-    m = block_max(m, red);
-    const float inv = inv_scale(m, eps, kQmaxInt8);
+    m = block_max<KEEP>(m, red);
+    const float inv = row_inv<KEEP>(m, eps);
     if (vec) {
       const int64_t nc = L >> 3;
       for (int64_t c = threadIdx.x; c < nc; c += kBlock) {
@@ -1715,7 +1717,7 @@ __global__ __launch_bounds__(kBlock) void k_cast_cols_narrow1(
 // t holds chunks t, t + B, ..., up to V of them. Chunks past the channel's
 // end are loaded from its first chunk (in bounds) and left out of the
 // maximum, so the loads need no branch. Reads x once: 2N + N + 4C bytes.
-template <int DT, int V, int B>
+template <int DT, int V, int B, bool KEEP>
 __global__ __launch_bounds__(B) void k_chan_wg(
     const void* __restrict__ x, int64_t channels, int64_t inner, int nchunks, float eps,
     int8_t* __restrict__ q, float* __restrict__ scale) {
@@ -1738,15 +1740,15 @@ __global__ __launch_bounds__(B) void k_chan_wg(
   for (int v = 0; v < V; ++v) {
     float f[8];
     cvt8<DT>(r[v], f);
-    const float mv = absmax8(f, 0.0f);
-    m = v * B + static_cast<int>(threadIdx.x) < nchunks ? fmaxf(m, mv) : m;
+    const float mv = absmax8<KEEP>(f, 0.0f);
+    m = v * B + static_cast<int>(threadIdx.x) < nchunks ? max_abs<KEEP>(m, mv) : m;
   }
   // the cast converts from the raw words again instead of keeping the
   // first conversion's fp32 values live
 #pragma unroll
   for (int v = 0; v < V; ++v) reload_barrier<DT>(r[v]);
-  m = block_max(m, red);
-  const float inv = inv_scale(m, eps, kQmaxInt8);
+  m = block_max<KEEP>(m, red);
+  const float inv = row_inv<KEEP>(m, eps);
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     if (v * B + static_cast<int>(threadIdx.x) >= nchunks) continue;
@@ -2144,13 +2146,13 @@ unsigned wg_rows_grid(int64_t rows) {
 }
 
 // Rows of length L (elements) -> fastest kernel shape that fits.
-template <int DT, int LPR, int VPL>
+template <int DT, int LPR, int VPL, bool KEEP>
 void launch_rows_sub(const void* x, int64_t rows, float eps, int8_t* q, float* scale,
                      hipStream_t s) {
   constexpr int RI = (LPR * VPL >= 64) ? 2 : 4;
   constexpr int64_t rows_per_wg = static_cast<int64_t>(kBlock / kWave) * RI * (kWave / LPR);
   const int64_t grid = cdiv(rows, rows_per_wg);
-  k_rows_sub<DT, LPR, VPL, RI><<<dim3(static_cast<unsigned>(grid)), dim3(kBlock), 0, s>>>(
+  k_rows_sub<DT, LPR, VPL, RI, KEEP><<<dim3(static_cast<unsigned>(grid)), dim3(kBlock), 0, s>>>(
       x, rows, eps, q, scale);
 }
 
@@ -2174,7 +2176,7 @@ bool chan_wg_applies(const void* x, const void* q, int64_t outer, int64_t inner)
          chunks <= static_cast<int64_t>(kChanWgThreads) * kChanWgMaxV;
 }
 
-template <int DT>
+template <int DT, bool KEEP>
 int chan_wg_quant_t(const void* x, int64_t outer, int64_t channels, int64_t inner, float eps,
                     int8_t* q, float* scale, hipStream_t s, const char* what) {
   const int nchunks = static_cast<int>(outer * (inner >> 3));
@@ -2182,15 +2184,15 @@ int chan_wg_quant_t(const void* x, int64_t outer, int64_t channels, int64_t inne
   if (nchunks <= kChanWgSmall) {
     const int v = static_cast<int>(cdiv(nchunks, 256));
     const dim3 b(256);
-    if (v <= 2) k_chan_wg<DT, 2, 256><<<g, b, 0, s>>>(x, channels, inner, nchunks, eps, q, scale);
-    else if (v <= 4) k_chan_wg<DT, 4, 256><<<g, b, 0, s>>>(x, channels, inner, nchunks, eps, q, scale);
-    else k_chan_wg<DT, 8, 256><<<g, b, 0, s>>>(x, channels, inner, nchunks, eps, q, scale);
+    if (v <= 2) k_chan_wg<DT, 2, 256, KEEP><<<g, b, 0, s>>>(x, channels, inner, nchunks, eps, q, scale);
+    else if (v <= 4) k_chan_wg<DT, 4, 256, KEEP><<<g, b, 0, s>>>(x, channels, inner, nchunks, eps, q, scale);
+    else k_chan_wg<DT, 8, 256, KEEP><<<g, b, 0, s>>>(x, channels, inner, nchunks, eps, q, scale);
     return launch_status(what);
   }
   const int v = static_cast<int>(cdiv(nchunks, kChanWgThreads));
   const dim3 b(kChanWgThreads);
-  if (v <= 8) k_chan_wg<DT, 8, kChanWgThreads><<<g, b, 0, s>>>(x, channels, inner, nchunks, eps, q, scale);
-  else k_chan_wg<DT, kChanWgMaxV, kChanWgThreads><<<g, b, 0, s>>>(x, channels, inner, nchunks, eps, q, scale);
+  if (v <= 8) k_chan_wg<DT, 8, kChanWgThreads, KEEP><<<g, b, 0, s>>>(x, channels, inner, nchunks, eps, q, scale);
+  else k_chan_wg<DT, kChanWgMaxV, kChanWgThreads, KEEP><<<g, b, 0, s>>>(x, channels, inner, nchunks, eps, q, scale);
   return launch_status(what);
 }
 
@@ -2203,31 +2205,31 @@ int chan_wg_quant_t(const void* x, int64_t outer, int64_t channels, int64_t inne
 // 112.7 us); G = 3584 117.5 us against 134.2 us in k_chan_wg, rows of 2056
 // 24.7 against 35.5 us.
 constexpr int kRowsAnyMaxChunks = 512;
-template <int DT, int LPR, int VPL>
+template <int DT, int LPR, int VPL, bool KEEP>
 void launch_rows_sub_any(const void* x, int64_t rows, int cg, float eps, int8_t* q, float* scale,
                          hipStream_t s) {
   constexpr int RI = (LPR * VPL >= 64) ? 2 : 4;
   constexpr int64_t rows_per_wg = static_cast<int64_t>(kBlock / kWave) * RI * (kWave / LPR);
-  k_rows_sub_any<DT, LPR, VPL, RI><<<dim3(static_cast<unsigned>(cdiv(rows, rows_per_wg))),
+  k_rows_sub_any<DT, LPR, VPL, RI, KEEP><<<dim3(static_cast<unsigned>(cdiv(rows, rows_per_wg))),
                                      dim3(kBlock), 0, s>>>(x, rows, cg, eps, q, scale);
 }
 
-template <int DT>
+template <int DT, bool KEEP>
 void rows_quant_any(const void* x, int64_t rows, int cg, float eps, int8_t* q, float* scale,
                     hipStream_t s) {
-  if (cg <= 1) launch_rows_sub_any<DT, 1, 1>(x, rows, cg, eps, q, scale, s);
-  else if (cg <= 2) launch_rows_sub_any<DT, 2, 1>(x, rows, cg, eps, q, scale, s);
-  else if (cg <= 4) launch_rows_sub_any<DT, 4, 1>(x, rows, cg, eps, q, scale, s);
-  else if (cg <= 8) launch_rows_sub_any<DT, 8, 1>(x, rows, cg, eps, q, scale, s);
-  else if (cg <= 16) launch_rows_sub_any<DT, 16, 1>(x, rows, cg, eps, q, scale, s);
-  else if (cg <= 32) launch_rows_sub_any<DT, 32, 1>(x, rows, cg, eps, q, scale, s);
-  else if (cg <= 64) launch_rows_sub_any<DT, 64, 1>(x, rows, cg, eps, q, scale, s);
-  else if (cg <= 128) launch_rows_sub_any<DT, 64, 2>(x, rows, cg, eps, q, scale, s);
-  else if (cg <= 256) launch_rows_sub_any<DT, 64, 4>(x, rows, cg, eps, q, scale, s);
-  else launch_rows_sub_any<DT, 64, 8>(x, rows, cg, eps, q, scale, s);
+  if (cg <= 1) launch_rows_sub_any<DT, 1, 1, KEEP>(x, rows, cg, eps, q, scale, s);
+  else if (cg <= 2) launch_rows_sub_any<DT, 2, 1, KEEP>(x, rows, cg, eps, q, scale, s);
+  else if (cg <= 4) launch_rows_sub_any<DT, 4, 1, KEEP>(x, rows, cg, eps, q, scale, s);
+  else if (cg <= 8) launch_rows_sub_any<DT, 8, 1, KEEP>(x, rows, cg, eps, q, scale, s);
+  else if (cg <= 16) launch_rows_sub_any<DT, 16, 1, KEEP>(x, rows, cg, eps, q, scale, s);
+  else if (cg <= 32) launch_rows_sub_any<DT, 32, 1, KEEP>(x, rows, cg, eps, q, scale, s);
+  else if (cg <= 64) launch_rows_sub_any<DT, 64, 1, KEEP>(x, rows, cg, eps, q, scale, s);
+  else if (cg <= 128) launch_rows_sub_any<DT, 64, 2, KEEP>(x, rows, cg, eps, q, scale, s);
+  else if (cg <= 256) launch_rows_sub_any<DT, 64, 4, KEEP>(x, rows, cg, eps, q, scale, s);
+  else launch_rows_sub_any<DT, 64, 8, KEEP>(x, rows, cg, eps, q, scale, s);
 }
 
-template <int DT, int LPR, int VPL, int E>
+template <int DT, int LPR, int VPL, int E, bool KEEP>
 void launch_rows_sub_any1(const void* x, int64_t rows, int L, float eps, int8_t* q, float* scale,
                           hipStream_t s) {
   // rows per wave and lane group: with E = 4 and one unit per lane four where
@@ -2238,46 +2240,46 @@ void launch_rows_sub_any1(const void* x, int64_t rows, int L, float eps, int8_t*
   constexpr int64_t kPer = static_cast<int64_t>(kBlock / kWave) * (kWave / LPR);
   if constexpr (kRows == 4) {
     if (cdiv(rows, kPer * kRows) < 2LL * device_cus()) {
-      k_rows_sub_any1<DT, LPR, VPL, 1, E>
+      k_rows_sub_any1<DT, LPR, VPL, 1, E, KEEP>
           <<<dim3(static_cast<unsigned>(cdiv(rows, kPer))), dim3(kBlock), 0, s>>>(x, rows, L, eps, q, scale);
       return;
     }
   }
-  k_rows_sub_any1<DT, LPR, VPL, kRows, E>
+  k_rows_sub_any1<DT, LPR, VPL, kRows, E, KEEP>
       <<<dim3(static_cast<unsigned>(cdiv(rows, kPer * kRows))), dim3(kBlock), 0, s>>>(x, rows, L, eps, q, scale);
 }
 
 constexpr int kRowsAny1Max = 2048;
 
-template <int DT, int E>
+template <int DT, int E, bool KEEP>
 void rows_quant_any1_e(const void* x, int64_t rows, int L, float eps, int8_t* q, float* scale,
                        hipStream_t s) {
   const int U = L / E;   // load units per row
-  if (U <= 1) launch_rows_sub_any1<DT, 1, 1, E>(x, rows, L, eps, q, scale, s);
-  else if (U <= 2) launch_rows_sub_any1<DT, 2, 1, E>(x, rows, L, eps, q, scale, s);
-  else if (U <= 4) launch_rows_sub_any1<DT, 4, 1, E>(x, rows, L, eps, q, scale, s);
-  else if (U <= 8) launch_rows_sub_any1<DT, 8, 1, E>(x, rows, L, eps, q, scale, s);
-  else if (U <= 16) launch_rows_sub_any1<DT, 16, 1, E>(x, rows, L, eps, q, scale, s);
-  else if (U <= 32) launch_rows_sub_any1<DT, 32, 1, E>(x, rows, L, eps, q, scale, s);
-  else if (U <= 64) launch_rows_sub_any1<DT, 64, 1, E>(x, rows, L, eps, q, scale, s);
-  else if (U <= 128) launch_rows_sub_any1<DT, 64, 2, E>(x, rows, L, eps, q, scale, s);
-  else if (U <= 256) launch_rows_sub_any1<DT, 64, 4, E>(x, rows, L, eps, q, scale, s);
-  else if (U <= 512) launch_rows_sub_any1<DT, 64, 8, E>(x, rows, L, eps, q, scale, s);
-  else if constexpr (E < 4) launch_rows_sub_any1<DT, 64, 16, E>(x, rows, L, eps, q, scale, s);
+  if (U <= 1) launch_rows_sub_any1<DT, 1, 1, E, KEEP>(x, rows, L, eps, q, scale, s);
+  else if (U <= 2) launch_rows_sub_any1<DT, 2, 1, E, KEEP>(x, rows, L, eps, q, scale, s);
+  else if (U <= 4) launch_rows_sub_any1<DT, 4, 1, E, KEEP>(x, rows, L, eps, q, scale, s);
+  else if (U <= 8) launch_rows_sub_any1<DT, 8, 1, E, KEEP>(x, rows, L, eps, q, scale, s);
+  else if (U <= 16) launch_rows_sub_any1<DT, 16, 1, E, KEEP>(x, rows, L, eps, q, scale, s);
+  else if (U <= 32) launch_rows_sub_any1<DT, 32, 1, E, KEEP>(x, rows, L, eps, q, scale, s);
+  else if (U <= 64) launch_rows_sub_any1<DT, 64, 1, E, KEEP>(x, rows, L, eps, q, scale, s);
+  else if (U <= 128) launch_rows_sub_any1<DT, 64, 2, E, KEEP>(x, rows, L, eps, q, scale, s);
+  else if (U <= 256) launch_rows_sub_any1<DT, 64, 4, E, KEEP>(x, rows, L, eps, q, scale, s);
+  else if (U <= 512) launch_rows_sub_any1<DT, 64, 8, E, KEEP>(x, rows, L, eps, q, scale, s);
+  else if constexpr (E < 4) launch_rows_sub_any1<DT, 64, 16, E, KEEP>(x, rows, L, eps, q, scale, s);
 }
 
-template <int DT>
+template <int DT, bool KEEP>
 void rows_quant_any1(const void* x, int64_t rows, int L, float eps, int8_t* q, float* scale,
                      hipStream_t s) {
   constexpr uintptr_t pair = DT == kF32 ? 8 : 4;
   if (L % 4 == 0 && aligned(x, 2 * pair) && aligned(q, 4))   // L <= 2048: U <= 512
-    rows_quant_any1_e<DT, 4>(x, rows, L, eps, q, scale, s);
+    rows_quant_any1_e<DT, 4, KEEP>(x, rows, L, eps, q, scale, s);
   else if (L % 2 == 0 && aligned(x, pair) && aligned(q, 2))
-    rows_quant_any1_e<DT, 2>(x, rows, L, eps, q, scale, s);
+    rows_quant_any1_e<DT, 2, KEEP>(x, rows, L, eps, q, scale, s);
   else if (L <= 1024)
-    rows_quant_any1_e<DT, 1>(x, rows, L, eps, q, scale, s);
+    rows_quant_any1_e<DT, 1, KEEP>(x, rows, L, eps, q, scale, s);
   else
-    launch_rows_sub_any1<DT, 64, 32, 1>(x, rows, L, eps, q, scale, s);
+    launch_rows_sub_any1<DT, 64, 32, 1, KEEP>(x, rows, L, eps, q, scale, s);
 }
 
 // Slices per row for the split-row path: enough workgroups for about four
@@ -2307,18 +2309,18 @@ size_t row_split_ws_bytes(int64_t rows, int64_t L) {
   return sp > 1 ? CBQ_WS_CTRL_BYTES + static_cast<size_t>(rows * sp) * 4 : CBQ_WS_CTRL_BYTES;
 }
 
-template <int DT>
+template <int DT, bool KEEP>
 int rows_split_quant_t(const void* x, int64_t rows, int64_t L, int64_t sp, float eps, void* ws,
                        int8_t* q, float* scale, hipStream_t s, const char* what) {
   float* partial = reinterpret_cast<float*>(static_cast<char*>(ws) + CBQ_WS_CTRL_BYTES);
   const int64_t sc = cdiv(L >> 3, sp);
   const dim3 g(static_cast<unsigned>(sp), static_cast<unsigned>(rows)), b(kBlock);
-  k_rows_split_max<DT><<<g, b, 0, s>>>(x, L, sc, partial);
-  k_rows_split_cast<DT><<<g, b, 0, s>>>(x, L, sc, partial, eps, q, scale);
+  k_rows_split_max<DT, KEEP><<<g, b, 0, s>>>(x, L, sc, partial);
+  k_rows_split_cast<DT, KEEP><<<g, b, 0, s>>>(x, L, sc, partial, eps, q, scale);
   return launch_status(what);
 }
 
-template <int DT>
+template <int DT, bool KEEP>
 int rows_quant_t(const void* x, int64_t rows, int64_t L, float eps, int8_t* q, float* scale,
                  hipStream_t s, const char* what, void* ws = nullptr, size_t ws_bytes = 0) {
   CBQ_REQUIRE(rows <= 0x7fffffffLL, "%s: too many rows (%lld)", what, (long long)rows);
@@ -2327,54 +2329,57 @@ int rows_quant_t(const void* x, int64_t rows, int64_t L, float eps, int8_t* q, f
     // few long rows: slices of each row spread over the CUs
     const int64_t sp = row_splits(rows, L);
     if (sp > 1 && ws_bytes >= row_split_ws_bytes(rows, L))
-      return rows_split_quant_t<DT>(x, rows, L, sp, eps, ws, q, scale, s, what);
+      return rows_split_quant_t<DT, KEEP>(x, rows, L, sp, eps, ws, q, scale, s, what);
   }
   if (vec) {
     switch (L) {
-      case 8: launch_rows_sub<DT, 1, 1>(x, rows, eps, q, scale, s); return launch_status(what);
-      case 16: launch_rows_sub<DT, 2, 1>(x, rows, eps, q, scale, s); return launch_status(what);
-      case 32: launch_rows_sub<DT, 4, 1>(x, rows, eps, q, scale, s); return launch_status(what);
-      case 64: launch_rows_sub<DT, 8, 1>(x, rows, eps, q, scale, s); return launch_status(what);
-      case 128: launch_rows_sub<DT, 16, 1>(x, rows, eps, q, scale, s); return launch_status(what);
-      case 256: launch_rows_sub<DT, 32, 1>(x, rows, eps, q, scale, s); return launch_status(what);
-      case 512: launch_rows_sub<DT, 64, 1>(x, rows, eps, q, scale, s); return launch_status(what);
-      case 1024: launch_rows_sub<DT, 64, 2>(x, rows, eps, q, scale, s); return launch_status(what);
-      case 2048: launch_rows_sub<DT, 64, 4>(x, rows, eps, q, scale, s); return launch_status(what);
+      case 8: launch_rows_sub<DT, 1, 1, KEEP>(x, rows, eps, q, scale, s); return launch_status(what);
+      case 16: launch_rows_sub<DT, 2, 1, KEEP>(x, rows, eps, q, scale, s); return launch_status(what);
+      case 32: launch_rows_sub<DT, 4, 1, KEEP>(x, rows, eps, q, scale, s); return launch_status(what);
+      case 64: launch_rows_sub<DT, 8, 1, KEEP>(x, rows, eps, q, scale, s); return launch_status(what);
+      case 128: launch_rows_sub<DT, 16, 1, KEEP>(x, rows, eps, q, scale, s); return launch_status(what);
+      case 256: launch_rows_sub<DT, 32, 1, KEEP>(x, rows, eps, q, scale, s); return launch_status(what);
+      case 512: launch_rows_sub<DT, 64, 1, KEEP>(x, rows, eps, q, scale, s); return launch_status(what);
+      case 1024: launch_rows_sub<DT, 64, 2, KEEP>(x, rows, eps, q, scale, s); return launch_status(what);
+      case 2048: launch_rows_sub<DT, 64, 4, KEEP>(x, rows, eps, q, scale, s); return launch_status(what);
       case 4096:
-        k_rows_wg<DT, 2><<<dim3(wg_rows_grid(rows)), dim3(kBlock), 0, s>>>(x, rows, eps, q, scale);
+        k_rows_wg<DT, 2, kBlock, KEEP><<<dim3(wg_rows_grid(rows)), dim3(kBlock), 0, s>>>(x, rows, eps, q, scale);
         return launch_status(what);
       case 8192:
-        k_rows_wg<DT, 2, 512><<<dim3(wg_rows_grid(rows)), dim3(512), 0, s>>>(x, rows, eps, q, scale);
+        k_rows_wg<DT, 2, 512, KEEP><<<dim3(wg_rows_grid(rows)), dim3(512), 0, s>>>(x, rows, eps, q, scale);
         return launch_status(what);
       case 16384:
-        k_rows_wg<DT, 8><<<dim3(wg_rows_grid(rows)), dim3(kBlock), 0, s>>>(x, rows, eps, q, scale);
+        k_rows_wg<DT, 8, kBlock, KEEP><<<dim3(wg_rows_grid(rows)), dim3(kBlock), 0, s>>>(x, rows, eps, q, scale);
         return launch_status(what);
       default: break;
     }
     // other lengths: below 512 chunks several rows per wave, up to 8192 one
     // workgroup per row, in registers either way
     if ((L >> 3) < kRowsAnyMaxChunks) {
-      rows_quant_any<DT>(x, rows, static_cast<int>(L >> 3), eps, q, scale, s);
+      rows_quant_any<DT, KEEP>(x, rows, static_cast<int>(L >> 3), eps, q, scale, s);
       return launch_status(what);
     }
     if (chan_wg_applies(x, q, 1, L))
-      return chan_wg_quant_t<DT>(x, 1, rows, L, eps, q, scale, s, what);
+      return chan_wg_quant_t<DT, KEEP>(x, 1, rows, L, eps, q, scale, s, what);
   } else if (L <= kRowsAny1Max) {
     // no 16-byte loads: several rows per wave with element loads
-    rows_quant_any1<DT>(x, rows, static_cast<int>(L), eps, q, scale, s);
+    rows_quant_any1<DT, KEEP>(x, rows, static_cast<int>(L), eps, q, scale, s);
     return launch_status(what);
   }
-  k_rows_generic<DT><<<dim3(wg_rows_grid(rows)), dim3(kBlock), 0, s>>>(
+  k_rows_generic<DT, KEEP><<<dim3(wg_rows_grid(rows)), dim3(kBlock), 0, s>>>(
       x, rows, L, vec ? 1 : 0, eps, q, scale);
   return launch_status(what);
 }
 
+// KEEP: a row with a NaN or an infinity gets a NaN scale, where the reference's
+// maximum leaves NaN out.
+template <bool KEEP = false>
 int rows_quant(const void* x, int dt, int64_t rows, int64_t L, float eps, int8_t* q, float* scale,
                hipStream_t s, const char* what, void* ws = nullptr, size_t ws_bytes = 0) {
   switch (dt) {
-    case kF16: return rows_quant_t<kF16>(x, rows, L, eps, q, scale, s, what, ws, ws_bytes);
-    case kBF16: return rows_quant_t<kBF16>(x, rows, L, eps, q, scale, s, what, ws, ws_bytes);
-    default: return rows_quant_t<kF32>(x, rows, L, eps, q, scale, s, what, ws, ws_bytes);
+    case kF16: return rows_quant_t<kF16, KEEP>(x, rows, L, eps, q, scale, s, what, ws, ws_bytes);
+    case kBF16: return rows_quant_t<kBF16, KEEP>(x, rows, L, eps, q, scale, s, what, ws, ws_bytes);
+    default: return rows_quant_t<kF32, KEEP>(x, rows, L, eps, q, scale, s, what, ws, ws_bytes);
   }
 }
 
@@ -2850,6 +2855,18 @@ extern "C" int cbq_quant_int8_channel(const void* x, int dtype, int64_t rows, in
   }
 }
 
+extern "C" int cbq_quant_int8_tokens(const void* x, int dtype, int64_t rows, int64_t cols, float eps,
+                                     void* ws, size_t ws_bytes, int8_t* q, float* scale,
+                                     cbq_stream_t stream) {
+  clear_error();
+  const char* what = "cbq_quant_int8_tokens";
+  CBQ_REQUIRE(valid_dtype(dtype, true), "%s: unsupported input dtype code %d", what, dtype);
+  CBQ_REQUIRE(rows >= 0 && cols >= 0, "%s: negative shape", what);
+  if (rows == 0 || cols == 0) return CBQ_OK;
+  CBQ_REQUIRE(x && q && scale, "%s: null pointer", what);
+  return rows_quant<true>(x, dtype, rows, cols, eps, q, scale, as_stream(stream), what, ws, ws_bytes);
+}
+
 extern "C" size_t cbq_quant_int8_channel_nd_ws_bytes(int64_t outer, int64_t channels,
                                                      int64_t inner) {
   if (outer <= 0 || channels <= 0 || inner <= 0) return CBQ_WS_CTRL_BYTES;
@@ -2877,9 +2894,9 @@ extern "C" int cbq_quant_int8_channel_nd(const void* x, int dtype, int64_t outer
               (long long)channels);
   if (chan_wg_applies(x, q, outer, inner)) {
     switch (dtype) {
-      case kF16: return chan_wg_quant_t<kF16>(x, outer, channels, inner, eps, q, scale, as_stream(stream), what);
-      case kBF16: return chan_wg_quant_t<kBF16>(x, outer, channels, inner, eps, q, scale, as_stream(stream), what);
-      default: return chan_wg_quant_t<kF32>(x, outer, channels, inner, eps, q, scale, as_stream(stream), what);
+      case kF16: return chan_wg_quant_t<kF16, false>(x, outer, channels, inner, eps, q, scale, as_stream(stream), what);
+      case kBF16: return chan_wg_quant_t<kBF16, false>(x, outer, channels, inner, eps, q, scale, as_stream(stream), what);
+      default: return chan_wg_quant_t<kF32, false>(x, outer, channels, inner, eps, q, scale, as_stream(stream), what);
     }
   }
   const int64_t cols = channels * inner;

@@ -13,7 +13,7 @@ import torch.nn as nn
 
 from .quantizers import quantize_tensor
 from .tensor import QuantizedTensor
-from cublade_amd.bindings.hip.quantize_int8 import quantize_per_channel_int8
+from cublade_amd.bindings.hip.quantize_int8 import quantize_tokens_int8
 from cublade_amd.bindings.hip.w8a8 import w8a8_gated, w8a8_linear
 
 
@@ -83,13 +83,13 @@ def gated_w8a8(x: QuantizedTensor, gate: QuantizedTensor, up: QuantizedTensor, *
 
 def _tokens(x, features: int):
     """(codes, scales, leading shape, dtype) of a layer's input: a tensor is
-    quantized with one scale for each token."""
+    quantized with one scale for each token, NaN where the token is not finite."""
     if isinstance(x, QuantizedTensor):
         _check(x, "x")
         if x.data.size(1) != features:
             raise ValueError(f"x must have {features} features, got {x.data.size(1)}")
         return x.data, x.scale, (x.data.size(0),), x.original_dtype
-    q, scale = quantize_per_channel_int8(x.detach().reshape(-1, features).contiguous())
+    q, scale = quantize_tokens_int8(x.detach().reshape(-1, features).contiguous())
     return q, scale, x.shape[:-1], x.dtype
 
 
@@ -99,7 +99,8 @@ class cuBladeW8A8LinearLayer(nn.Module):
 
     The input is a fp16, bf16 or fp32 GPU tensor [..., in_features], or a
     QuantizedTensor [tokens, in_features] as norm_tensor gives it, which is
-    taken as it is. The output has the input's (original) dtype.
+    taken as it is. The output has the input's (original) dtype. A token that holds
+    a NaN or an infinity comes out as NaN.
 
     Storage: int8_weights int8 [out, in], scales float32 [out], bias parameter
     [out] in `dtype`, or None.

@@ -26,6 +26,14 @@ typedef struct {
   int64_t scale_stride;
 } cbq_i8_rows;
 
+/* Activations: codes of x's rows (tokens) with a scale for each, by the kernels and with the
+ * workspace of cbq_quant_int8_channel (axis 0) and the same bits, but for rows that hold a NaN
+ * or an infinity: those get a NaN scale (and codes 0), so that a product's row is NaN. There,
+ * NaN inputs are left out of the maximum, as in the reference. */
+int cbq_quant_int8_tokens(const void* x, int dtype, int64_t rows, int64_t cols, float eps,
+                          void* ws, size_t ws_bytes, int8_t* q, float* scale,
+                          cbq_stream_t stream);
+
 /* Activations of the gated product. GELU: with the error function, or its
  * approximation by tanh. */
 enum { CBQ_ACT_SILU = 0, CBQ_ACT_GELU = 1, CBQ_ACT_GELU_TANH = 2, CBQ_ACT_RELU = 3 };
