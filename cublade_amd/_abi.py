@@ -135,9 +135,15 @@ class NormArgs(ctypes.Structure):
                 ("eps", _F), ("alpha", _F)]
 
 
+class W8A8Form(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("kernel", "weight_rows", "x_rows", "threads", "stages",
+                                              "ranges", "copies")] + [("workgroups", _I64)]
+
+
 W8A8_SIGNATURES = {
     "cbq_quant_int8_tokens": (_I32, [_P, _I32, _I64, _I64, _F, _P, _SZ, _P, _P, _P]),
     "cbq_w8a8_ws_bytes": (_SZ, [_I64, _I64, _I64, _I32]),
+    "cbq_w8a8_form_of": (_I32, [_I64, _I64, _I64, _I32, _I32, _P]),
     "cbq_w8a8_linear": (_I32, [_P, _P, _P, _I32, _I64, _I64, _I64, _P, _I32, _P, _SZ, _P]),
     "cbq_w8a8_gated": (_I32, [_P, _P, _P, _P, _P, _I32, _I32, _I64, _I64, _I64, _P, _I32, _P, _SZ,
                               _P]),

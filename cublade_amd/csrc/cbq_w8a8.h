@@ -131,5 +131,6 @@ constexpr int kFewRows = 2048;
 struct FewPlan { int shape; double us; };
 FewPlan few_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, int cus);
 void launch_w8a8_few(const W8Args& a, int shape, bool any, hipStream_t s);
+cbq_w8a8_form few_form(int shape, int64_t M, int64_t N, int proj, int rows);
 
 }  // namespace cbq

@@ -481,6 +481,8 @@ double w8_time(const W8Model& f, int tile, int64_t tiles, int64_t steps_all, int
   return sp > 1 ? t + f.join + f.sum * static_cast<double>(sp * out) : t;
 }
 
+constexpr int64_t kMaxTiles = 1 << 24;    // a grid has fewer than 2^32 threads, 256 to a tile
+
 // room: bytes of workspace, or all that is wanted.
 W8Plan w8_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, size_t room = ~static_cast<size_t>(0)) {
   const int cus = device_cus();
@@ -502,9 +504,11 @@ W8Plan w8_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, size_t room 
     rows = kRows16;
   }
   double best = -1;
+  p.splits = 1;
   for (int tile = 0; tile < kTiles; ++tile) {
     if (rows != kRows16 && (tile == kT192 || tile == kT128)) continue;
     const int64_t tiles = cdiv(M, 64 * kTileJ[tile]) * cdiv(N, 64 * kTileI[tile] / proj);
+    if (tiles >= kMaxTiles) continue;
     const size_t plane = static_cast<size_t>(tiles) * kTileJ[tile] * kTileI[tile] * 16384;   // bytes of sums
     for (int64_t sp = 1; sp <= 8; ++sp) {
       const size_t bytes = p.part_off + (sp > 1 ? sp * plane : 0);
@@ -635,7 +639,7 @@ int w8_run(const char* what, const cbq_i8_rows* x, const cbq_i8_rows* const (&w)
     return launch_status(what);
   }
   const int64_t tiles_m = cdiv(M, 64 * kTileJ[p.tile]), tiles_n = cdiv(N, 64 * kTileI[p.tile] / proj);
-  CBQ_REQUIRE(tiles_m * tiles_n * p.splits < (1LL << 31), "%s: too many tiles", what);
+  CBQ_REQUIRE(tiles_m * tiles_n * p.splits < kMaxTiles, "%s: too many tiles", what);
   a.tiles_m = static_cast<int>(tiles_m);
   a.tiles_n = static_cast<int>(tiles_n);
   a.splits = p.splits;
@@ -669,6 +673,32 @@ extern "C" size_t cbq_w8a8_ws_bytes(int64_t M, int64_t N, int64_t K, int project
   if (M <= 0 || N <= 0 || K < 16 || K > 131071 || projections < 1 || projections > 2)
     return CBQ_WS_CTRL_BYTES;
   return w8_plan(M, N, K, projections, K % 16 == 0 ? kRows16 : K % 4 == 0 ? kRows4 : kRows1).bytes;
+}
+
+extern "C" int cbq_w8a8_form_of(int64_t M, int64_t N, int64_t K, int projections, int multiple,
+                                cbq_w8a8_form* form) {
+  clear_error();
+  const char* what = "cbq_w8a8_form_of";
+  CBQ_REQUIRE(form, "%s: form is null", what);
+  CBQ_REQUIRE(M > 0 && N > 0 && M < (1LL << 31) - 256 && N < (1LL << 31) - 256 && K >= 0 && K <= 131071,
+              "%s: unsupported sizes", what);
+  CBQ_REQUIRE(projections == 1 || projections == 2, "%s: projections must be 1 or 2, got %d", what, projections);
+  CBQ_REQUIRE((multiple == 16 || multiple == 4 || multiple == 1) && K % multiple == 0,
+              "%s: multiple must be 16, 4 or 1 and divide K, got %d", what, multiple);
+  if (K < 16) {
+    *form = {CBQ_W8A8_SHORT, 1, 1, kBlock, 0, 1, 0, cdiv(M * N, kBlock)};
+    return CBQ_OK;
+  }
+  const int rows = multiple == 16 ? kRows16 : multiple == 4 ? kRows4 : kRows1;
+  const W8Plan p = w8_plan(M, N, K, projections, rows);
+  if (p.few >= 0) {
+    *form = few_form(p.few, M, N, projections, rows);
+    return CBQ_OK;
+  }
+  const int x_rows = 64 * kTileJ[p.tile], w_rows = 64 * kTileI[p.tile];
+  *form = {CBQ_W8A8_TILES, w_rows, x_rows, 256, p.tile == kT128 ? 4 : 2, p.splits, p.pad,
+           cdiv(M, x_rows) * cdiv(N, w_rows / projections) * p.splits};
+  return CBQ_OK;
 }
 
 extern "C" int cbq_w8a8_linear(const cbq_i8_rows* x, const cbq_i8_rows* w, const void* bias,

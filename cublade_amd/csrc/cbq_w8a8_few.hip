@@ -267,6 +267,14 @@ void launch_few(W8Args a, bool any, hipStream_t s) {
 
 }  // namespace
 
+cbq_w8a8_form few_form(int shape, int64_t M, int64_t N, int proj, int rows) {
+  const FewShape& f = kShapes[shape];
+  cbq_w8a8_form r = {CBQ_W8A8_FEW, 16 * f.rt, 16 * f.mt, 64 * f.waves, rows == kRows16 ? f.depth : 1, 1, 0, 0};
+  r.workgroups = cdiv(N, 16 * (f.rt / proj));
+  if (f.mt > 1 || M > 16) r.workgroups = cdiv(r.workgroups, 8) * 8 * cdiv(M, r.x_rows);   // see launch_few
+  return r;
+}
+
 FewPlan few_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, int cus) {
   FewPlan best = {-1, 0.0};
   for (int c = 0; c < kNumShapes; ++c) {

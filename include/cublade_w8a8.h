@@ -64,6 +64,24 @@ int cbq_w8a8_gated(const cbq_i8_rows* x, const cbq_i8_rows* gate, const cbq_i8_r
                    int64_t M, int64_t N, int64_t K, void* y, int out_dtype, void* ws,
                    size_t ws_bytes, cbq_stream_t stream);
 
+/* How a product of these sizes is computed (projections as above), for tests and tuning; nothing
+ * is launched. multiple: what the rows of all operands are multiples of (address, stride and K,
+ * in bytes): 16, 4 or 1. With the workspace that cbq_w8a8_ws_bytes names. */
+enum { CBQ_W8A8_SHORT = 0, CBQ_W8A8_FEW = 1, CBQ_W8A8_TILES = 2 };
+
+typedef struct {
+  int32_t kernel;
+  int32_t weight_rows, x_rows;   /* that a workgroup owns (weight rows: of all projections) */
+  int32_t threads;               /* of a workgroup */
+  int32_t stages;                /* in LDS, of a wave (FEW) or a workgroup (TILES) */
+  int32_t ranges;                /* of K, each with workgroups of its own */
+  int32_t copies;                /* 1: x and the weights are copied to rows of whole 16 bytes */
+  int64_t workgroups;
+} cbq_w8a8_form;
+
+int cbq_w8a8_form_of(int64_t M, int64_t N, int64_t K, int projections, int multiple,
+                     cbq_w8a8_form* form);
+
 /* The norms before and after a block, with the block's gate and residual scale:
  *   t = post ? norm(x; post_weight, post_bias) : x
  *   h = residual + alpha gate t            (rounded to the residual's type)
