@@ -46,7 +46,8 @@ __device__ __forceinline__ float activate(float g) {
   // 1/2 (1 + tanh(u)) = sigmoid(2 u)
   else if constexpr (ACT == CBQ_ACT_GELU_TANH)
     return g * sigmoid_of(g * (1.59576912f + 0.0713548163f * (g * g)));
-  else if constexpr (ACT == CBQ_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.707106781f));
+  // 1 + erf(t) = erfc(-t), which keeps its digits where g is negative
+  else if constexpr (ACT == CBQ_ACT_GELU) return 0.5f * g * erfcf(g * -0.707106781f);
   else if constexpr (ACT == CBQ_ACT_RELU) return g < 0.0f ? 0.0f : g;
   else return g;
 }
