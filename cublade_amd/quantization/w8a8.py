@@ -8,6 +8,8 @@ integer sums are exact.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn as nn
 
@@ -89,7 +91,10 @@ def _tokens(x, features: int):
         if x.data.size(1) != features:
             raise ValueError(f"x must have {features} features, got {x.data.size(1)}")
         return x.data, x.scale, (x.data.size(0),), x.original_dtype
-    q, scale = quantize_tokens_int8(x.detach().reshape(-1, features).contiguous())
+    if x.dim() == 0 or x.shape[-1] != features:
+        raise ValueError(f"x must have {features} features, got {tuple(x.shape)}")
+    rows = x.detach().reshape(math.prod(x.shape[:-1]), features)
+    q, scale = quantize_tokens_int8(rows.contiguous())
     return q, scale, x.shape[:-1], x.dtype
 
 
