@@ -17,7 +17,8 @@
 // monotonic, so max |v weight| rstd is the largest of the rounded products.
 //
 // A NaN or an infinity in a row makes its maximum NaN (maxima are taken over the bit
-// patterns of absolute values, where a NaN is above everything) and with it the scale:
+// patterns of absolute values, where a NaN is above everything) and with it the scale, as
+// does a norm that is infinite itself (a weight, a bias, a product past fp32):
 // the token's outputs of a product are NaN rather than those of zero codes.
 #include <algorithm>
 #include <type_traits>
@@ -195,6 +196,8 @@ __device__ __forceinline__ Stat row_stat(Stat v, uint32_t* slots) {
   return {__uint_as_float(s), t};
 }
 
+constexpr float kEps = 1e-12f;   // of a row's maximum, as in the quantizers
+
 struct Norm {
   int layer;               // else rms
   float eps;
@@ -204,11 +207,6 @@ struct Norm {
 
 __device__ __forceinline__ float rstd_of(float ss, const Norm& n) {
   return rsqrtf(ss * n.inv_h + n.eps);   // eps may be 0, and v_rsq_f32 takes no denormals
-}
-
-// The codes of 8 values, and the row's stored scale.
-__device__ __forceinline__ float row_inv(float amax) {
-  return amax == amax ? inv_scale(amax, 1e-12f, kQmaxInt8) : amax;
 }
 
 struct Args {
@@ -377,7 +375,7 @@ __global__ __launch_bounds__(WAVE ? kBlock : 1024) void k_norm(Args args) {
     }
   }
   if (a.out_dtype == CBQ_I8) {
-    inv = row_inv(amax);
+    inv = row_inv<true>(amax, kEps);
     if (t == 0) a.scale[token] = 1.0f / inv;
   }
 #pragma unroll
@@ -441,7 +439,7 @@ __global__ __launch_bounds__(1024) void k_norm_long(Args args) {
   if (a.out_dtype == CBQ_I8) {
     uint32_t top = 0u;
     each([&](int64_t e) { top = max_u32(top, abs_bits(normed(ld_v(e), e, mean, rstd, a.weight, a.bias))); });
-    inv = row_inv(__uint_as_float(row_stat<false>({0.0f, top}, slots[4]).top));
+    inv = row_inv<true>(__uint_as_float(row_stat<false>({0.0f, top}, slots[4]).top), kEps);
     if (threadIdx.x == 0) a.scale[token] = 1.0f / inv;
   }
   each([&](int64_t e) {

@@ -39,8 +39,9 @@ def norm_tensor(x: torch.Tensor, weight: torch.Tensor | None = None,
     it of the norm in fp32, and original_dtype x's; or a tensor like x in `dtype`.
     Sums and the norm are fp32 (the sum of squares of elements beyond about 2^63
     overflows, and the result is 0); their order, and so a result's last bits, may
-    differ with the number of tokens and the tensors' alignment. A token with a NaN or an infinity gets a NaN
-    scale and reads back as NaN. The result carries no gradient.
+    differ with the number of tokens and the tensors' alignment. A token with a NaN or
+    an infinity, in x or in the norm, gets a NaN scale and reads back as NaN. The
+    result carries no gradient.
     """
     if dtype is None:
         raise ValueError("norm_tensor: dtype is None")

@@ -90,7 +90,7 @@ int cbq_w8a8_form_of(int64_t M, int64_t N, int64_t K, int projections, int multi
  * elements; CBQ_NORM_RMS: mean = 0. A null weight is 1, a null bias 0, a null
  * gate 1. out_dtype CBQ_I8: codes of n and a scale for each token, as by
  * cbq_quant_int8_channel (axis 0) of n in fp32; a token with a NaN or an
- * infinity gets a NaN scale. Otherwise n in out_dtype. out null: h only.
+ * infinity, in x or in n, gets a NaN scale. Otherwise n in out_dtype. out null: h only.
  *
  * x: [tokens, hidden], rows x_stride elements apart, in x_dtype. residual (or
  * null): likewise, in x's type or CBQ_F32. h: [tokens, hidden] in the residual's
