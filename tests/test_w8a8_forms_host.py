@@ -44,3 +44,27 @@ def test_bad_arguments_of_the_query():
         assert L.cbq_w8a8_form_of(*args, ctypes.byref(f)) == 1 and needle in L.cbq_last_error().decode()
     assert L.cbq_w8a8_form_of(8, 8, 64, 1, 16, None) == 1
     assert F.form(8, 8, 7, 1).kernel == F.SHORT
+
+
+def test_every_form_is_among_the_cases():
+    """The forms that random sizes choose are those that some case of the GPU tests has: a
+    change of the choice shows here where it leaves a kernel without a test."""
+    import random
+    from tests import test_gpu_w8a8 as T
+    from tests import test_gpu_w8a8_forms as N
+    gated = next(m for m in T.test_gated.pytestmark if m.args[0] == "shape").args[1]
+    for cases in (N.LINEAR, N.GATED):
+        for form, shape in cases:
+            assert F.key(*shape, form[1] if form[0] == "short" else form[4]) == form, shape
+    tested = {F.key(*s, 1) for s in T.SHAPES + T.LINEAR_FORMS} | {F.key(*s, 2) for s in gated + T.GATED_FORMS}
+    tested |= {form for form, _ in N.LINEAR + N.GATED}
+    rng = random.Random(1)
+
+    def size(lo, hi):
+        return round(2 ** rng.uniform(lo, hi))
+
+    for _ in range(60000):
+        m, n, k, projections = size(0, 12), size(0, 15.3), size(3.5, 14.3), rng.choice((1, 2))
+        rows = rng.choice((1, 4, 16))
+        k = max(rows, k // rows * rows)
+        assert F.key(m, n, k, projections) in tested, (m, n, k, projections)
