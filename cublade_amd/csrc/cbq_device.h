@@ -162,12 +162,12 @@ __device__ __forceinline__ float ld1(const void* base, int64_t i) {
 
 // The larger of two absolute values. fmaxf returns the non-NaN operand, so NaN
 // inputs are ignored exactly as the reference's fmaxf fold does. KEEP: a NaN is
-// kept instead (as bits without a sign a NaN is above everything).
+// kept instead (v_maximum3_f32, which like v_max_f32 takes |x| at no cost; as
+// integers without a sign bf16 [8192, 8192] took 35.2 us instead of 32.2).
 template <bool KEEP = false>
 __device__ __forceinline__ float max_abs(float a, float b) {
-  if constexpr (!KEEP) return fmaxf(a, b);
-  const uint32_t u = __float_as_uint(a), v = __float_as_uint(b);
-  return __uint_as_float(u > v ? u : v);
+  if constexpr (KEEP) return __builtin_elementwise_maximum(a, b);
+  else return fmaxf(a, b);
 }
 
 // |x| max over a chunk.
