@@ -66,12 +66,13 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor 
         post_norm, post_weight, post_bias: the norm after the block. All weights
             and biases have one dtype.
         gate: any shape that broadcasts to x's (of a channel, of a token, of
-            both), fp32, fp16 or bf16.
+            both), fp32, fp16 or bf16. One that repeats some tokens' rows but not
+            all (as [batch, 1, hidden] does) is expanded to x's size in the call.
         scale: of the block's part of the sum.
 
     Returns (h, n): h in x's shape and the residual's dtype, n as norm_tensor
-    (h) gives it: n is taken of h as rounded to its dtype. Neither carries a
-    gradient.
+    (h) gives it: n is taken of h as rounded to its dtype; as codes it is [tokens,
+    hidden], its leading dimensions flattened. Neither carries a gradient.
     """
     h, out, s = norm(x, residual, weight, bias, kind, eps, dtype, post_norm, post_weight, post_bias,
                      gate, float(scale))

@@ -51,6 +51,12 @@ def linear_w8a8(x: QuantizedTensor, weight: QuantizedTensor, bias: torch.Tensor 
     Returns [tokens, out_features]. The integer sums are exact (in_features at
     most 131071); scales and bias are applied in fp32, then one rounding to
     out_dtype. The result carries no gradient.
+
+    Codes are read in place, but for rows that are not contiguous, more than 2^22
+    bytes apart, or, with in_features a multiple of 16, at addresses that are none:
+    those are copied in every call. in_features that is no multiple of 16 is slower;
+    where it is no multiple of 4 either, both operands are copied in the call from
+    640 tokens on.
     """
     _check(x, "x")
     _check(weight, "weight")
@@ -102,9 +108,10 @@ class cuBladeW8A8LinearLayer(nn.Module):
     """nn.Linear with INT8 weights (one scale for each output channel) and INT8
     activations (one scale for each token, found in the call).
 
-    The input is a fp16, bf16 or fp32 GPU tensor [..., in_features], or a
-    QuantizedTensor [tokens, in_features] as norm_tensor gives it, which is
-    taken as it is. The output has the input's (original) dtype. A token that holds
+    The input is a fp16, bf16 or fp32 GPU tensor [..., in_features], whose leading
+    dimensions the output keeps, or a QuantizedTensor [tokens, in_features] as
+    norm_tensor gives it, which is taken as it is: its output is [tokens,
+    out_features], to be viewed in the shape of the hidden states. The output has the input's (original) dtype. A token that holds
     a NaN or an infinity comes out as NaN.
 
     Storage: int8_weights int8 [out, in], scales float32 [out], bias parameter
