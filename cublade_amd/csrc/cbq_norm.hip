@@ -201,7 +201,6 @@ constexpr float kEps = 1e-12f;   // of a row's maximum, as in the quantizers
 struct Norm {
   int layer;               // else rms
   float eps;
-  int64_t H;
   float inv_h;
 };
 
@@ -518,7 +517,7 @@ extern "C" int cbq_norm(const cbq_norm_args* p, cbq_stream_t stream) {
                   element_aligned(a.post_bias, a.param_dtype) && element_aligned(a.gate, a.gate_dtype) &&
                   (a.out_dtype == CBQ_I8 || element_aligned(a.out, a.out_dtype)),
               "cbq_norm: tensors must be aligned to their elements");
-  args.n = Norm{a.kind == CBQ_NORM_LAYER, a.eps, a.hidden, 1.0f / static_cast<float>(a.hidden)};
+  args.n = Norm{a.kind == CBQ_NORM_LAYER, a.eps, 1.0f / static_cast<float>(a.hidden)};
   // Inputs that the Infinity Cache cannot still hold are read past it (8192 x 8192 with a
   // residual, 268 MB: 78 us against 85), others through it (16384 x 1408, 46 MB: 19
   // against 24).

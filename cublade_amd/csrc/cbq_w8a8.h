@@ -30,7 +30,7 @@ struct W8Args {
   int vec;                 // y's rows may be stored 16 bytes at a time
   int M, N, K;
   int tiles_m, tiles_n;
-  int splits, split_steps; // K in ranges of split_steps 64-byte steps
+  int splits, split_steps; // K in ranges of split_steps 128-byte steps
   int* part;               // sums of the ranges: [splits][tiles], as the tiles' registers hold them
 };
 
@@ -128,6 +128,7 @@ enum { kRows16, kRows4, kRows1 };
 
 // cbq_w8a8_few.hip: few rows of x, or few outputs; K >= 16. The shape for these sizes (-1:
 // none) and its modelled time; any: rows that are no multiples of 16 bytes. Returns after queueing.
+// The model was fitted up to 1024 rows; past kFewRows only tiles are considered.
 constexpr int kFewRows = 2048;
 struct FewPlan { int shape; double us; };
 FewPlan few_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, int cus);

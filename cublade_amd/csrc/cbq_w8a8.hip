@@ -5,7 +5,8 @@
 //   y[m, n] = sx[m] sw[n] sum_k x[m, k] w[n, k] + bias[n]
 //   y[m, n] = act(g) u,  g and u as above with the gate's and the up rows
 //
-// Sums are int32 and exact (K <= 131071). M <= 64, and small products: cbq_w8a8_few.hip.
+// Sums are int32 and exact (K <= 131071). M <= 64, and products of up to kFewRows rows where its
+// model is the faster one: cbq_w8a8_few.hip.
 //
 // k_w8_tile<J, I, NS, ACT, SPLIT, ANY>: tiles of 64 J tokens x 64 I weight rows (gated:
 // 32 I columns of each projection side by side, so that a lane holds g and u of the
@@ -74,7 +75,6 @@ __global__ __launch_bounds__(256) void k_w8_tile(W8Args a) {
   constexpr int LX = G::kLX, LT = G::kLX + G::kLW, NW = G::kWaves;
   constexpr int WM = 32 * J, WR = 32 * I;               // a wave's tokens, weight rows
   constexpr int WN = GATED ? WR / 2 : WR;               // and output columns
-  constexpr int IO = GATED ? I / 2 : I;                 // 32-column tiles it puts out
   __shared__ __attribute__((aligned(1024))) uint8_t smem[NS * G::kSB];
   __shared__ __attribute__((aligned(16))) float s_x[G::kTM], s_w[G::kTN], s_b[G::kTN];
 
@@ -491,7 +491,9 @@ W8Plan w8_plan(int64_t M, int64_t N, int64_t K, int proj, int rows, size_t room 
   p.bytes = CBQ_WS_CTRL_BYTES;
   const FewPlan few = M <= kFewRows ? few_plan(M, N, K, proj, rows, cus) : FewPlan{-1, 0.0};
   p.few = few.shape;
-  if (M <= 64 && p.few >= 0) return p;   // 64 x 11008 x 4096, gated: 24 us, by tiles 22; mostly a third of the tiles' time
+  // Mostly a third of the tiles' time, so the tiles' model is not asked; where they are close the
+  // tiles may win (64 x 11008 x 4096, gated: 24 us, by tiles 22).
+  if (M <= 64 && p.few >= 0) return p;
   p.kp = cdiv(K, 16) * 16;
   p.part_off = CBQ_WS_CTRL_BYTES;
   // Copies read and write M K + N K bytes at 4 TB/s and take a launch. Where rows are no

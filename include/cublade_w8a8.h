@@ -43,6 +43,8 @@ enum { CBQ_ACT_SILU = 0, CBQ_ACT_GELU = 1, CBQ_ACT_GELU_TANH = 2, CBQ_ACT_RELU =
  * exact for any codes. y: [M, N] in out_dtype, contiguous. bias (or null): [N]
  * in bias_dtype. The sum becomes fp32 (rounded once past 2^24), the rest is
  * fp32 with each product and sum rounded, then one rounding to out_dtype.
+ * A launch takes fewer than 2^32 threads, so K < 16 takes M N below 2^32 - 256, and others
+ * fewer than 2^24 tiles of 256 x 256.
  *
  * ws: cbq_w8a8_ws_bytes(M, N, K, 1) bytes, 256-byte aligned, of which the
  * control block is not used. With less, or none, K is not cut into ranges, and
@@ -57,7 +59,7 @@ int cbq_w8a8_linear(const cbq_i8_rows* x, const cbq_i8_rows* w, const void* bias
                     size_t ws_bytes, cbq_stream_t stream);
 
 /* y[m, n] = act(g) u, with g and u the products above of the same x with the
- * rows of `gate` and of `up` (biases: both or neither may be null). ws:
+ * rows of `gate` and of `up` (each bias may be null; both have bias_dtype). ws:
  * cbq_w8a8_ws_bytes(M, N, K, 2). */
 int cbq_w8a8_gated(const cbq_i8_rows* x, const cbq_i8_rows* gate, const cbq_i8_rows* up,
                    const void* gate_bias, const void* up_bias, int bias_dtype, int activation,
